@@ -448,6 +448,67 @@ T0B_API int32_t t0b_embedding_bwd(t0b_ctx* ctx, uint64_t grad_table, uint64_t id
                                   uint32_t dim, uint32_t vocab, uint64_t scratch, size_t scratch_bytes, int32_t async);
 
 /* ------------------------------------------------------------------------------------------------
+ * Vocabulary losses: cross entropy and distillation over a large vocabulary, with their gradients.  They stand beside
+ * t0b_softmax_ce (src/t0/ce_loss_kernels.rs:26-192), which needs the f32 logits in memory; the reference has neither form.
+ *
+ * Every row r has a sparse target distribution q over the vocabulary -- one word with q = 1 (cross entropy), or the softmax
+ * of a teacher's top logits -- and the student's p = softmax(z / T):
+ *   losses[r] = sum_k q_rk (log q_rk - log p_r,id_rk)          f32, unweighted
+ *   dz        = (p sum(q) - q) * scale * row_weights[r] / T    the gradient of scale * sum_r row_weights[r] losses[r]
+ * A row is left out when it has no target (target T0B_NO_WORD; no teacher word other than T0B_NO_WORD whose logit is above
+ * -inf) or no logit above -inf: its loss, its log-sum-exp and its gradients are 0, whatever its logits, hidden state, weight
+ * and teacher logits hold.  An index >= vocab that is not T0B_NO_WORD counts as T0B_NO_WORD and sets the device status word
+ * to 110.  A NaN or +inf logit makes its row's loss and gradient NaN; a masked word (-inf logit) has p = 0 and, where it
+ * is a target, an infinite loss.  Outputs must not overlap inputs or each other, except as said below.
+ * ---------------------------------------------------------------------------------------------- */
+#define T0B_NO_WORD 0xffffffffu
+#define T0B_MAX_TOPK 1024
+
+/* Distillation on given logits.  logits [rows, cols] f32 or bf16 (logits_dtype: T0B_OUT_*) at a pitch of ld elements;
+ * ids u32 and teacher f32 [rows, topk] at a pitch of ldk, topk <= T0B_MAX_TOPK, in any order: the words the teacher scored
+ * and its logits, of which q is the softmax at the same temperature T.  A word that a row names twice counts twice.
+ * losses f32[rows] or 0; dlogits [rows, cols] f32 or bf16 (grad_dtype), same ld, or 0 -- it may be `logits` itself when the
+ * types agree; row_weights f32[rows] or 0 (all 1). */
+T0B_API int32_t t0b_topk_distill(t0b_ctx* ctx, uint64_t logits, int32_t logits_dtype, uint64_t ids, uint64_t teacher,
+                                 uint64_t row_weights, uint64_t losses, uint64_t dlogits, int32_t grad_dtype, uint32_t rows,
+                                 uint32_t cols, uint64_t ld, uint32_t topk, uint64_t ldk, float temperature, float scale,
+                                 int32_t async);
+
+/* The same losses straight from the hidden states x [rows, dim] (f32 or bf16; f32 is rounded to bf16) and the bf16 head w,
+ * without logits in memory: the head's product keeps the softmax statistics of every row in its epilogue.  w is
+ * [dim, vocab] as Linear stores it (trans_w = 0) or [vocab, dim] as an embedding table (trans_w = 1); any sizes and pitches
+ * (elements), copied into the scratch first where TMA cannot address them.
+ * With dx and dw 0 only the losses (and lse[r] = log sum exp(z / T)) are computed.  With dx and / or dw, which have the
+ * shapes of x and w in f32 or bf16, the exponentials of a piece of the rows (at most 1 GiB; piece_rows rows where that is
+ * not 0) stand in the scratch until the piece's gradient is done; dw sums over the pieces in f32.  The operands of the two
+ * gradient products are bf16 (dz is rounded to it), their sums f32; results do not depend on run, stream or scratch.
+ * scratch: 256-byte aligned, t0b_linear_loss_scratch_bytes() bytes; 0 = a workspace of the context that grows as needed.  A
+ * call that is being captured into a graph must bring its own and keep it as long as the graph; graphs (or contexts) that
+ * may run at the same time need one each. */
+typedef struct t0b_linear_loss {
+    uint64_t x, w;
+    uint64_t ldx, ldw;
+    uint64_t row_weights;       /* f32[rows], or 0 */
+    uint64_t losses, lse;       /* f32[rows], or 0 */
+    uint64_t dx, dw;            /* or 0 */
+    uint64_t lddx, lddw;
+    uint64_t scratch, scratch_bytes;
+    uint32_t rows, dim, vocab;
+    uint32_t trans_w;
+    uint32_t piece_rows;        /* 0 = as many as the piece's bound allows */
+    int32_t x_dtype, dx_dtype, dw_dtype;   /* T0B_OUT_F32 / T0B_OUT_BF16 */
+    float scale;
+} t0b_linear_loss;
+/* Scratch of a call with these sizes, pitches and outputs (pointers count only as 0 or not, and by their alignment);
+ * topk = 0 for t0b_linear_ce.  The choice of tiles behind it follows t0b_tune: ask again after tuning. */
+T0B_API size_t t0b_linear_loss_scratch_bytes(t0b_ctx* ctx, const t0b_linear_loss* loss, uint32_t topk);
+/* Softmax cross entropy, targets u32[rows]. */
+T0B_API int32_t t0b_linear_ce(t0b_ctx* ctx, const t0b_linear_loss* loss, uint64_t targets, int32_t async);
+/* Distillation; ids, teacher, topk, ldk and temperature as for t0b_topk_distill. */
+T0B_API int32_t t0b_linear_topk_distill(t0b_ctx* ctx, const t0b_linear_loss* loss, uint64_t ids, uint64_t teacher, uint32_t topk,
+                                        uint64_t ldk, float temperature, int32_t async);
+
+/* ------------------------------------------------------------------------------------------------
  * tile_ir front end: TileGemm specs with M/N/K edge handling and an epilogue chain (src/t0/tile_ir.rs).
  * ---------------------------------------------------------------------------------------------- */
 enum { T0B_TILE_NT = 0, T0B_TILE_NN = 1 };          /* TileTranspose, src/t0/tile_ir.rs:72-78 */

@@ -63,6 +63,32 @@ pub struct t0b_gemm_plan {
 }
 
 #[repr(C)] #[derive(Clone, Copy, Debug, Default, PartialEq)]
+pub struct t0b_linear_loss {
+    pub x: u64,
+    pub w: u64,
+    pub ldx: u64,
+    pub ldw: u64,
+    pub row_weights: u64,
+    pub losses: u64,
+    pub lse: u64,
+    pub dx: u64,
+    pub dw: u64,
+    pub lddx: u64,
+    pub lddw: u64,
+    pub scratch: u64,
+    pub scratch_bytes: u64,
+    pub rows: u32,
+    pub dim: u32,
+    pub vocab: u32,
+    pub trans_w: u32,
+    pub piece_rows: u32,
+    pub x_dtype: i32,
+    pub dx_dtype: i32,
+    pub dw_dtype: i32,
+    pub scale: f32,
+}
+
+#[repr(C)] #[derive(Clone, Copy, Debug, Default, PartialEq)]
 pub struct t0b_tile_gemm {
     pub tile_m: u32,
     pub tile_n: u32,
@@ -167,6 +193,10 @@ extern "C" {
     pub fn t0b_embedding_fwd(ctx: *mut t0b_ctx, table: u64, ids: u64, out: u64, num_tokens: u32, dim: u32, vocab: u32, is_async: i32) -> i32;
     pub fn t0b_embedding_bwd_scratch_bytes(num_tokens: u32) -> usize;
     pub fn t0b_embedding_bwd(ctx: *mut t0b_ctx, grad_table: u64, ids: u64, grad_out: u64, num_tokens: u32, dim: u32, vocab: u32, scratch: u64, scratch_bytes: usize, is_async: i32) -> i32;
+    pub fn t0b_topk_distill(ctx: *mut t0b_ctx, logits: u64, logits_dtype: i32, ids: u64, teacher: u64, row_weights: u64, losses: u64, dlogits: u64, grad_dtype: i32, rows: u32, cols: u32, ld: u64, topk: u32, ldk: u64, temperature: f32, scale: f32, is_async: i32) -> i32;
+    pub fn t0b_linear_loss_scratch_bytes(ctx: *mut t0b_ctx, loss: *const t0b_linear_loss, topk: u32) -> usize;
+    pub fn t0b_linear_ce(ctx: *mut t0b_ctx, loss: *const t0b_linear_loss, targets: u64, is_async: i32) -> i32;
+    pub fn t0b_linear_topk_distill(ctx: *mut t0b_ctx, loss: *const t0b_linear_loss, ids: u64, teacher: u64, topk: u32, ldk: u64, temperature: f32, is_async: i32) -> i32;
     pub fn t0b_tile_preset(name: *const c_char, out: *mut t0b_tile_gemm) -> i32;
     pub fn t0b_tile_name(spec: *const t0b_tile_gemm, buf: *mut c_char, cap: usize) -> i32;
     pub fn t0b_tile_wg_size(spec: *const t0b_tile_gemm) -> u32;

@@ -26,6 +26,13 @@ class TileGemmC(C.Structure):
         "n_epilogue")] + [("epilogue", C.c_int32 * 4)]
 
 
+class LinearLossC(C.Structure):
+    _fields_ = ([(n, C.c_uint64) for n in ("x", "w", "ldx", "ldw", "row_weights", "losses", "lse", "dx", "dw", "lddx", "lddw", "scratch",
+                                           "scratch_bytes")]
+                + [(n, C.c_uint32) for n in ("rows", "dim", "vocab", "trans_w", "piece_rows")]
+                + [(n, C.c_int32) for n in ("x_dtype", "dx_dtype", "dw_dtype")] + [("scale", C.c_float)])
+
+
 _u32, _u64, _i32, _sz, _f = C.c_uint32, C.c_uint64, C.c_int32, C.c_size_t, C.c_float
 _ctx = C.c_void_p
 _cfgp = C.POINTER(GemmConfigC)
@@ -105,6 +112,10 @@ SIGNATURES = {
     "t0b_embedding_fwd": (_i32, [_ctx, _u64, _u64, _u64, _u32, _u32, _u32, _i32]),
     "t0b_embedding_bwd_scratch_bytes": (_sz, [_u32]),
     "t0b_embedding_bwd": (_i32, [_ctx, _u64, _u64, _u64, _u32, _u32, _u32, _u64, _sz, _i32]),
+    "t0b_topk_distill": (_i32, [_ctx, _u64, _i32, _u64, _u64, _u64, _u64, _u64, _i32, _u32, _u32, _u64, _u32, _u64, _f, _f, _i32]),
+    "t0b_linear_loss_scratch_bytes": (_sz, [_ctx, C.POINTER(LinearLossC), _u32]),
+    "t0b_linear_ce": (_i32, [_ctx, C.POINTER(LinearLossC), _u64, _i32]),
+    "t0b_linear_topk_distill": (_i32, [_ctx, C.POINTER(LinearLossC), _u64, _u64, _u32, _u64, _f, _i32]),
     "t0b_tile_preset": (_i32, [C.c_char_p, C.POINTER(TileGemmC)]),
     "t0b_tile_name": (_i32, [C.POINTER(TileGemmC), C.c_char_p, _sz]),
     "t0b_tile_wg_size": (_u32, [C.POINTER(TileGemmC)]),

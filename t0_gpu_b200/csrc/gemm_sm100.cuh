@@ -8,12 +8,15 @@
 // the K tail contributes zeros, :768-787) -- here the zero fill is TMA's out-of-bounds fill, so callers
 // do not have to pad.
 //
+// HEAD = 1 replaces the store of C by the softmax epilogue of a vocabulary head (HeadParams).
+//
 // Roles per CTA: warp 0 = TMA producer, warp 1 = TMEM owner + MMA issuer, then four or eight epilogue warps
 // (TMEM -> registers -> shared-memory transpose tile -> TMA store or coalesced row stores): 192 threads for the
 // 64-column tile, 320 otherwise.  Every wait is bounded: when a wait runs out the CTA records a status code, raises
 // its abort flag, drains, frees its TMEM and returns.
 #pragma once
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cstdint>
 
 #include "ptx_sm100.cuh"
@@ -58,6 +61,23 @@ enum DeviceStatus : int {
 
 constexpr int kMaxDst = 8;
 
+// The softmax epilogue of a vocabulary head (kernels with HEAD = 1): instead of the products z of a tile, every epilogue
+// warp leaves, for each of its 32 rows and its own columns (a "part" of the row, GemmTraits::kPartCols wide),
+//   part[j] = (max z, sum of exp((z - max) / T)),
+// which a later kernel joins over the parts of the row; the raw z of the columns that the row asks for (`ids`); and, when a
+// gradient follows, u = exp((z - max) / T) in fp16 through the third tensor map.  u lies in [0, 1] with at least one 1 in
+// every part, so fp16 keeps 11 significant bits of everything above 2^-14 of the part's largest exponential and is off by
+// at most 2^-25 of it below; bf16 would lose three bits on the probabilities that carry the gradient.
+struct HeadParams {
+    float2* part;            // [parts][part_ld]
+    long long part_ld;       // rows, padded
+    float c;                 // log2(e) / T: exp(v / T) = 2^(c v)
+    const uint32_t* ids;     // [rows][n_ids], ascending within a row; entries >= N are never met
+    int n_ids;
+    float* z_sel;            // [rows][n_ids]: z of those columns
+    int store_u;
+};
+
 struct GemmParams {
     void* c_dst[kMaxDst];   // destinations of the epilogue store: [0] local, [1..] peers of a column-sharded GEMM
     int n_dst;
@@ -82,6 +102,8 @@ struct GemmParams {
 #ifdef T0B_TRACE
     unsigned long long* trace;   // timeline build only: [CTA][16] stamps of this launch (null = no stamps)
 #endif
+    int accumulate;         // 1: C += the product (f32 output, one destination, no split-K)
+    HeadParams head;        // HEAD kernels only
     int cluster_sk;         // > 1: split-K inside a thread-block cluster of that many CTAs (one per K range): the partial
                             // tiles stay in shared memory and are summed over distributed shared memory; 0 = slabs
 };
@@ -129,6 +151,7 @@ struct GemmTraits {
     static constexpr int kThreads = 64 + 32 * kEpiWarps;
     static constexpr int kBm = kBmCta * CG * kATiles;    // rows of the cluster tile
     static constexpr int kTileN = BN * kBTiles;          // columns of the cluster tile
+    static constexpr int kPartCols = BN / kEpiSplit;     // columns of one epilogue warp (softmax epilogue: one part)
 };
 
 struct WorkItem {
@@ -258,9 +281,13 @@ __device__ __forceinline__ float apply_chain(float v, const EpiChain& e, float b
 
 // Store one thread's 32 consecutive output columns of one row.
 __device__ __forceinline__ void store_chunk_f32(float* base, long long ld, int row, int col0, int ncols_valid,
-                                                const float (&v)[32], bool vec_ok) {
+                                                const float (&v)[32], bool vec_ok, bool add = false) {
     float* dst = base + static_cast<long long>(row) * ld + col0;
-    if (vec_ok && ncols_valid >= 32) {
+    if (add) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (j < ncols_valid) dst[j] += v[j];
+    } else if (vec_ok && ncols_valid >= 32) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             reinterpret_cast<float4*>(dst)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
@@ -309,7 +336,7 @@ __device__ __forceinline__ void stage_chunk_f32(uint32_t stage, int lane, const 
     }
 }
 __device__ __forceinline__ void flush_chunk_f32(uint32_t stage, int lane, float* base, long long ld, int row0, int col0,
-                                                int M, int N) {
+                                                int M, int N, bool add = false) {
     const int c = lane & 7;
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
@@ -317,8 +344,14 @@ __device__ __forceinline__ void flush_chunk_f32(uint32_t stage, int lane, float*
         const uint32_t addr = stage + r * 128 + ((c ^ (r & 7)) << 4);
         float4 q;
         asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(q.x), "=f"(q.y), "=f"(q.z), "=f"(q.w) : "r"(addr));
-        if (row0 + r < M && col0 + c * 4 < N)   // N % 4 == 0 on this path, so a piece is all in or all out
-            *reinterpret_cast<float4*>(base + static_cast<long long>(row0 + r) * ld + col0 + c * 4) = q;
+        if (row0 + r < M && col0 + c * 4 < N) {  // N % 4 == 0 on this path, so a piece is all in or all out
+            float4* dst = reinterpret_cast<float4*>(base + static_cast<long long>(row0 + r) * ld + col0 + c * 4);
+            if (add) {
+                const float4 o = *dst;
+                q = make_float4(o.x + q.x, o.y + q.y, o.z + q.z, o.w + q.w);
+            }
+            *dst = q;
+        }
     }
 }
 // TMA-store path: every 32x32 chunk goes out through two 2 KiB half tiles (rows of 64 bytes, 64-byte TMA swizzle:
@@ -378,7 +411,39 @@ __device__ __forceinline__ void flush_pair_bf16(uint32_t stage, int lane, __nv_b
     }
 }
 
-template <int BN, int CG, int MT, int ND = 0>
+// Element j of a register array, as a tree of selects (dynamic indexing would put the array in local memory).
+template <int W>
+__device__ __forceinline__ float pick_reg(const float* v, uint32_t j) {
+    if constexpr (W == 1) return v[0];
+    else {
+        const float a = pick_reg<W / 2>(v, j), b = pick_reg<W / 2>(v + W / 2, j);
+        return (j & (W / 2)) ? b : a;
+    }
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// fp16 form of stage_chunk_bf16_sw64.
+__device__ __forceinline__ void stage_chunk_f16_sw64(uint32_t half_tile, int lane, const float* v) {
+    const uint32_t row = half_tile + lane * 64;
+    const int x = (lane >> 1) & 3;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t h[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const __half2 t = __floats2half2_rn(v[8 * j + 2 * e], v[8 * j + 2 * e + 1]);
+            h[e] = *reinterpret_cast<const uint32_t*>(&t);
+        }
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + ((j ^ x) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+    }
+}
+
+template <int BN, int CG, int MT, int ND = 0, int HEAD = 0>
 __global__ void __launch_bounds__(GemmTraits<BN, CG, MT, ND>::kThreads, 1)
 gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                          const __grid_constant__ CUtensorMap tmap_c, const GemmParams p) {
@@ -633,6 +698,87 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
             const int n_base = wi.n0 + (ND == 1 ? group * BN : 0);
             const int row = row0 + lane;
             const uint32_t t_row = tmem_base + static_cast<uint32_t>(slot * BN) + (static_cast<uint32_t>(q * 32) << 16);
+            if constexpr (HEAD != 0) {
+                // Softmax epilogue: the warp's columns come into registers in one go (the accumulator is free again at
+                // once), so the maximum is known before the first exponential and nothing is rescaled.
+                constexpr int W = T::kPartCols;
+                uint32_t raw[W];
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) ptx::tmem_ld_32x32(t_row + (c_begin + c) * 32, *reinterpret_cast<uint32_t(*)[32]>(raw + 32 * c));
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) ptx::tmem_ld_wait_regs(*reinterpret_cast<uint32_t(*)[32]>(raw + 32 * c));
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (CG == 1) ptx::mbar_arrive(tempty_bar(slot));
+                    else ptx::mbar_arrive_cluster(ptx::mapa(tempty_bar(slot), 0));
+                }
+                const int col0 = n_base + c_begin * 32;
+                const int ncols = p.N - col0;
+                if (row0 < p.M && ncols > 0) {   // warp-uniform
+                    float v[W];
+#pragma unroll
+                    for (int j = 0; j < W; ++j) v[j] = (j < ncols) ? __uint_as_float(raw[j]) : -INFINITY;
+                    const HeadParams& hp = p.head;
+                    if (hp.n_ids > 0) {
+                        // The columns this row asks for: ids ascend, so the ones of this part are consecutive.
+                        const uint32_t* rid = hp.ids + static_cast<long long>(row < p.M ? row : 0) * hp.n_ids;
+                        int at = 0;
+                        if (hp.n_ids > 1) {
+                            int hi = hp.n_ids;
+                            while (at < hi) {
+                                const int mid = (at + hi) >> 1;
+                                if (rid[mid] < static_cast<uint32_t>(col0)) at = mid + 1;
+                                else hi = mid;
+                            }
+                        }
+                        uint32_t j = at < hp.n_ids ? rid[at] - static_cast<uint32_t>(col0) : 0xffffffffu;
+                        bool hit = row < p.M && j < static_cast<uint32_t>(W);
+                        while (__any_sync(0xffffffffu, hit)) {
+                            const float z = pick_reg<W>(v, j);
+                            if (hit) {
+                                hp.z_sel[static_cast<long long>(row) * hp.n_ids + at] = z;
+                                ++at;
+                                j = at < hp.n_ids ? rid[at] - static_cast<uint32_t>(col0) : 0xffffffffu;
+                                hit = j < static_cast<uint32_t>(W);
+                            }
+                        }
+                    }
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int j = 0; j < W; j += 4)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], v[j + e]);
+                    const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    // A part whose every z is -inf: its exponentials are 0, not exp(-inf + inf).
+                    const float ref = m == -INFINITY ? 0.0f : m;
+                    float sm[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int j = 0; j < W; ++j) {
+                        v[j] = exp2_approx((v[j] - ref) * hp.c);
+                        sm[j & 3] += v[j];
+                    }
+                    if (row < p.M) hp.part[static_cast<long long>(col0 / W) * hp.part_ld + row] = make_float2(m, (sm[0] + sm[1]) + (sm[2] + sm[3]));
+                    if (hp.store_u) {
+#pragma unroll
+                        for (int c = 0; c < kChunks; ++c) {
+                            const uint32_t half_tile = stage + static_cast<uint32_t>(c & 1) * 2048u;
+                            if (lane == 0) ptx::bulk_wait_group_read<1>();   // the store that last used this half has read it
+                            __syncwarp();
+                            stage_chunk_f16_sw64(half_tile, lane, v + 32 * c);
+                            ptx::fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0) {
+                                if (32 * c < ncols) ptx::tma_store_2d(&tmap_c, half_tile, col0 + 32 * c, row0);
+                                ptx::bulk_commit_group();   // one group per half, empty or not: the wait above counts groups
+                            }
+                        }
+                    }
+                }
+                slot ^= 1;
+                if (slot == 0) slot_phase ^= 1u;
+                continue;
+            }
             // The TMEM read of chunk c+1 is in flight while chunk c is transposed and stored.
             uint32_t nxt[32];
             ptx::tmem_ld_32x32(t_row + c_begin * 32, nxt);
@@ -736,9 +882,12 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                                 stage_half_f32_sw64(half_tile, lane, v + 16 * h);
                                 ptx::fence_proxy_async_smem();
                                 __syncwarp();
-                                if (lane == 0 && col0 + 16 * h < p.N) {
-                                    ptx::tma_store_2d(&tmap_c, half_tile, col0 + 16 * h, row0);
-                                    ptx::bulk_commit_group();
+                                if (lane == 0) {
+                                    if (col0 + 16 * h < p.N) {
+                                        if (p.accumulate) ptx::tma_reduce_add_2d(&tmap_c, half_tile, col0 + 16 * h, row0);
+                                        else ptx::tma_store_2d(&tmap_c, half_tile, col0 + 16 * h, row0);
+                                    }
+                                    ptx::bulk_commit_group();   // one group per half, empty or not: the wait above counts groups
                                 }
                             }
                             continue;
@@ -751,7 +900,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                                             row0, col0, p.M, p.N);
                         } else {
                             for (int d = 0; d < p.n_dst; ++d)
-                                flush_chunk_f32(stage, lane, static_cast<float*>(p.c_dst[d]), ld_out, row0, col0, p.M, p.N);
+                                flush_chunk_f32(stage, lane, static_cast<float*>(p.c_dst[d]), ld_out, row0, col0, p.M, p.N, p.accumulate != 0);
                         }
                     }
                 } else if (row < p.M && ncols > 0) {
@@ -774,7 +923,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                             store_chunk_bf16(static_cast<__nv_bfloat16*>(p.c_dst[d]), ld_out, row, col0, ncols, v, vec_ok);
                     } else {
                         for (int d = 0; d < p.n_dst; ++d)
-                            store_chunk_f32(static_cast<float*>(p.c_dst[d]), ld_out, row, col0, ncols, v, vec_ok);
+                            store_chunk_f32(static_cast<float*>(p.c_dst[d]), ld_out, row, col0, ncols, v, vec_ok, p.accumulate != 0);
                     }
                 }
             }

@@ -82,6 +82,7 @@ struct GemmCall {
     bool slabs_only;        // leave unreduced split-K slabs in c_dst[0] (reference contract)
     uint32_t force_split;   // for slabs_only: the exact number of slabs the caller expects
     bool no_auto_split;     // an automatically chosen config keeps the whole contraction in one tile (fixed summation order)
+    bool accumulate;        // C += A*B (f32 output, one destination, never split)
 };
 
 // Expand the public single-op epilogue code into a chain (EPI_BIAS_RELU = bias add, then ReLU).
@@ -125,6 +126,53 @@ int32_t launch_reduce(t0b_ctx* ctx, const float* partial, uint32_t sk, uint32_t 
     return check_cuda(ctx, cudaGetLastError(), "splitk_reduce launch");
 }
 
+// The config a call runs: its own, else a forced preset (T0_FORCE_CONFIG), else measured in this process (t0b_tune), else
+// the table shipped with the library, else the cost model.
+int32_t choose_config(t0b_ctx* ctx, const GemmCall& g, t0b_gemm_config* cfg, const char** source) {
+    if (g.cfg) {
+        *cfg = *g.cfg;
+        return T0B_OK;
+    }
+    int tuned_source = 0;
+    if (!ctx->force_config.empty()) {
+        if (t0b_config_preset(ctx->force_config.c_str(), cfg) != T0B_OK)
+            return set_error(ctx, T0B_ERR_INVALID, "gemm: T0_FORCE_CONFIG=%s is not a preset name", ctx->force_config.c_str());
+        *source = "forced";
+    } else if (tuned_lookup(g.m, g.n, g.k, g.trans_a, g.trans_b, g.out_bf16, cfg, &tuned_source)) {
+        *source = tuned_source == 2 ? "tuned in this process" : "shipped table";
+    } else {
+        default_b200_config(g.m, g.k, g.n, ctx->num_sms, cfg);
+        *source = "cost model";
+    }
+    if (g.no_auto_split) cfg->split_k = 0;
+    return T0B_OK;
+}
+
+// Whether the split-K of this plan runs inside thread-block clusters (no slabs in global memory).
+bool splitk_in_cluster(t0b_ctx* ctx, const GemmCall& g, const t0b_gemm_plan& plan) {
+    if (g.slabs_only || plan.split_k <= 1 || plan.split_k > 8 || (plan.split_k & (plan.split_k - 1)) != 0 || g.n_dst != 1 || !plan.use_tma ||
+        plan.cta_group != 1 || plan.m_tiles != 1 || plan.n_tiles != 1 || !ctx->cluster_splitk)
+        return false;
+    if (plan.split_k > 4) {
+        // Eight-CTA clusters do not tile every GPC: when the tiles need more clusters than fit at once, the second wave
+        // costs more than the slab round trip saves.
+        const int tiles = static_cast<int>(((g.m + plan.bm - 1) / plan.bm) * ((g.n + plan.bn - 1) / plan.bn));
+        const int fit = plan.bn == 256 ? max_active_splitk_clusters<256>(ctx, plan.split_k)
+                                       : (plan.bn == 128 ? max_active_splitk_clusters<128>(ctx, plan.split_k)
+                                                         : max_active_splitk_clusters<64>(ctx, plan.split_k));
+        if (tiles > fit) return false;
+    }
+    return true;
+}
+
+// Rasterisation group width: concurrently running tiles should cover a square-ish patch of C, so that A and B panels are
+// shared through L2: group * bm ~= (clusters / group) * bn.
+int raster_group(t0b_ctx* ctx, uint32_t bm, uint32_t bn, uint32_t cta_group, bool swap_grid) {
+    const double clusters = static_cast<double>(ctx->num_sms) / cta_group;
+    const int grp = static_cast<int>(std::lround(std::sqrt(clusters * (swap_grid ? bn : bm) / static_cast<double>(swap_grid ? bm : bn))));
+    return std::max(1, std::min(grp, 16));
+}
+
 int32_t run_gemm(t0b_ctx* ctx, const GemmCall& g) {
     if (g.m == 0 || g.n == 0) return T0B_OK;
     if (!g.a || !g.b || g.n_dst < 1 || g.n_dst > kMaxDst)
@@ -163,24 +211,10 @@ int32_t run_gemm(t0b_ctx* ctx, const GemmCall& g) {
 
     t0b_gemm_config cfg;
     const char* cfg_source = "caller";
-    int tuned_source = 0;
-    if (g.cfg) cfg = *g.cfg;
-    else {
-        // A forced preset (T0_FORCE_CONFIG), else measured in this process (t0b_tune), else the table shipped with the
-        // library, else the cost model.
-        if (!ctx->force_config.empty()) {
-            if (t0b_config_preset(ctx->force_config.c_str(), &cfg) != T0B_OK)
-                return set_error(ctx, T0B_ERR_INVALID, "gemm: T0_FORCE_CONFIG=%s is not a preset name", ctx->force_config.c_str());
-            cfg_source = "forced";
-        } else if (tuned_lookup(g.m, g.n, g.k, g.trans_a, g.trans_b, g.out_bf16, &cfg, &tuned_source)) {
-            cfg_source = tuned_source == 2 ? "tuned in this process" : "shipped table";
-        } else {
-            default_b200_config(g.m, g.k, g.n, ctx->num_sms, &cfg);
-            cfg_source = "cost model";
-        }
-        if (g.no_auto_split) cfg.split_k = 0;
-    }
+    int32_t rc_cfg = choose_config(ctx, g, &cfg, &cfg_source);
+    if (rc_cfg != T0B_OK) return rc_cfg;
     if (g.slabs_only) cfg.split_k = g.force_split;
+    if (g.accumulate) cfg.split_k = 0;
     if (cfg.split_k > 1 && (cfg.split_k & (cfg.split_k - 1)) != 0)
         return set_error(ctx, T0B_ERR_INVALID, "gemm: split_k=%u must be a power of 2", cfg.split_k);
 
@@ -197,8 +231,11 @@ int32_t run_gemm(t0b_ctx* ctx, const GemmCall& g) {
                       plan.bm, plan.bn, plan.cta_group, plan.stages, plan.split_k, plan.use_tma ? "" : " (CUDA-core kernel)");
         if (ctx->dumped.emplace(line, 1).second) std::fprintf(stderr, "%s\n", line);
     }
+    if (g.accumulate && (g.out_bf16 || g.n_dst != 1 || g.slabs_only || !plan.use_tma))
+        return set_error(ctx, T0B_ERR_INVALID, "gemm: accumulation needs one f32 destination and operands TMA can address");
     const size_t elem = g.out_bf16 ? 2 : 4;
     if (g.k == 0) {
+        if (g.accumulate) return T0B_OK;
         // Empty contraction: every accumulator is +0.0, so the result is epilogue(0).
         if (g.slabs_only) {
             // Every slab the caller expects carries an empty K range (the slabs are dense and adjacent).
@@ -230,18 +267,7 @@ int32_t run_gemm(t0b_ctx* ctx, const GemmCall& g) {
     }
 
     // Split-K inside clusters (see below) needs no slabs at all.
-    bool cluster_sk_possible = !g.slabs_only && plan.split_k > 1 && plan.split_k <= 8 && (plan.split_k & (plan.split_k - 1)) == 0 &&
-                               g.n_dst == 1 && plan.use_tma && plan.cta_group == 1 && plan.m_tiles == 1 && plan.n_tiles == 1 &&
-                               ctx->cluster_splitk;
-    if (cluster_sk_possible && plan.split_k > 4) {
-        // Eight-CTA clusters do not tile every GPC: when the tiles need more clusters than fit at once, the second wave
-        // costs more than the slab round trip saves.
-        const int tiles = static_cast<int>(((g.m + plan.bm - 1) / plan.bm) * ((g.n + plan.bn - 1) / plan.bn));
-        const int fit = plan.bn == 256 ? max_active_splitk_clusters<256>(ctx, plan.split_k)
-                                       : (plan.bn == 128 ? max_active_splitk_clusters<128>(ctx, plan.split_k)
-                                                         : max_active_splitk_clusters<64>(ctx, plan.split_k));
-        if (tiles > fit) cluster_sk_possible = false;
-    }
+    const bool cluster_sk_possible = splitk_in_cluster(ctx, g, plan);
     // Where do split-K partials go?
     float* partial = nullptr;
     uint64_t slab_stride = static_cast<uint64_t>(g.m) * g.n, ld_partial = g.n;
@@ -338,14 +364,10 @@ int32_t run_gemm(t0b_ctx* ctx, const GemmCall& g) {
         p.a_mn_major = g.trans_a ? 1 : 0;     // A stored [K,M]: M contiguous
         p.b_mn_major = g.trans_b ? 0 : 1;     // B stored [K,N]: N contiguous
         p.out_bf16 = g.out_bf16;
+        p.accumulate = g.accumulate ? 1 : 0;
         p.raster_along_n = cfg.swap_grid ? 0 : 1;
         {
-            // Concurrently running tiles should cover a square-ish patch of C, so that A and B panels are shared
-            // through L2: group * bm ~= (clusters / group) * bn.
-            const double clusters = static_cast<double>(ctx->num_sms) / plan.cta_group;
-            int grp = static_cast<int>(std::lround(std::sqrt(clusters * (cfg.swap_grid ? plan.bn : plan.bm) /
-                                                             static_cast<double>(cfg.swap_grid ? plan.bm : plan.bn))));
-            p.group = std::max(1, std::min(grp, 16));
+            p.group = raster_group(ctx, plan.bm, plan.bn, plan.cta_group, cfg.swap_grid != 0);
             // A measured group width travels in the config (lds_pad, the reference's RDNA3 padding knob, has no other
             // meaning here): the tuner tries a few and the shipped table keeps the winner -- on tall shapes the panel
             // order is worth up to a fifth of the run time.
@@ -423,10 +445,110 @@ __global__ void __launch_bounds__(256) fill_random_bf16_kernel(__nv_bfloat16* ds
     }
 }
 
+GemmCall call_of(const InnerGemm& d) {
+    GemmCall g{};
+    g.trans_a = d.trans_a; g.trans_b = d.trans_b; g.a = d.a; g.b = d.b;
+    g.c_dst[0] = d.c; g.n_dst = 1; g.m = d.m; g.n = d.n; g.k = d.k; g.lda = d.lda; g.ldb = d.ldb; g.ldc = d.ldc;
+    g.out_bf16 = d.out_bf16; g.accumulate = d.accumulate; g.workspace = d.slabs; g.workspace_bytes = d.slab_bytes;
+    g.no_auto_split = d.accumulate || d.no_split;
+    return g;
+}
+
 uint32_t rd_u32(const uint8_t* p) { return p[0] | (p[1] << 8) | (p[2] << 16) | (static_cast<uint32_t>(p[3]) << 24); }
 uint64_t rd_u64(const uint8_t* p) { return rd_u32(p) | (static_cast<uint64_t>(rd_u32(p + 4)) << 32); }
 
 }  // namespace
+
+namespace t0b {
+
+size_t inner_gemm_slab_bytes(t0b_ctx* ctx, const InnerGemm& d) {
+    const GemmCall g = call_of(d);
+    t0b_gemm_config cfg;
+    const char* source = "";
+    if (g.accumulate || choose_config(ctx, g, &cfg, &source) != T0B_OK) return 0;
+    t0b_gemm_plan plan;
+    const PlanInput pin{g.m, g.n, g.k, g.trans_a, g.trans_b, g.lda, g.ldb, g.a, g.b, ctx->num_sms};
+    resolve_plan(&cfg, pin, &plan);
+    if (plan.split_k <= 1 || splitk_in_cluster(ctx, g, plan)) return 0;
+    return static_cast<size_t>(plan.split_k) * g.m * g.n * 4;
+}
+
+int32_t inner_gemm(t0b_ctx* ctx, const InnerGemm& d) {
+    GemmCall g = call_of(d);
+    // The caller's slabs were sized for the config of that moment; a table entry that appeared since may want more.  The
+    // context's own workspace is never used here: it may be freed by a later call while a captured graph still holds it.
+    if (inner_gemm_slab_bytes(ctx, d) > d.slab_bytes) g.no_auto_split = true;
+    return run_gemm(ctx, g);
+}
+
+HeadPlan head_plan(t0b_ctx* ctx, uint32_t rows, uint32_t vocab, uint32_t dim) {
+    // The three tiles of the softmax epilogue by the cost model of the plain product (cycles per 64-deep K block and the
+    // epilogue that bounds a tile with a short contraction): a CTA pair shares each head column block between 256 rows; one
+    // CTA takes 128 rows, in 256 or 128 columns, whichever fills the last wave better.
+    struct Cand { uint32_t bm, bn, cg; double kb_cycles, epi_cycles; };
+    static const Cand cands[] = {{256, 256, 2, 780.0, 4000.0}, {128, 256, 1, 760.0, 4000.0}, {128, 128, 1, 700.0, 2200.0}};
+    const double kb = (dim + 63) / 64;
+    HeadPlan best{};
+    double best_cost = 1e300;
+    for (const Cand& c : cands) {
+        const uint64_t tiles = static_cast<uint64_t>((rows + c.bm - 1) / c.bm) * ((vocab + c.bn - 1) / c.bn);
+        const uint64_t clusters = static_cast<uint64_t>(ctx->num_sms) / c.cg;
+        const double waves = static_cast<double>((tiles + clusters - 1) / clusters);
+        const double cost = waves * std::max(kb * c.kb_cycles, c.epi_cycles) + c.epi_cycles;
+        if (cost < best_cost) {
+            best_cost = cost;
+            best.bm = c.bm; best.bn = c.bn; best.cta_group = c.cg;
+            best.part_cols = c.bn / 2;
+        }
+    }
+    return best;
+}
+
+int32_t head_gemm(t0b_ctx* ctx, const HeadGemm& d) {
+    const HeadPlan& plan = d.plan;
+    CUtensorMap ta, tb, tc;
+    int32_t rc = get_tmap(ctx, d.x, d.dim, d.rows, d.ldx, 64, 128, &ta);
+    if (rc != T0B_OK) return rc;
+    if (d.trans_w) rc = get_tmap(ctx, d.w, d.dim, d.vocab, d.ldw, 64, plan.bn / plan.cta_group, &tb);
+    else rc = get_tmap(ctx, d.w, d.vocab, d.dim, d.ldw, 64, 64, &tb);
+    if (rc != T0B_OK) return rc;
+    tc = ta;
+    if (d.u) {
+        rc = get_tmap(ctx, d.u, d.ldu, d.rows, d.ldu, 32, 32, &tc);   // 16-bit elements, moved as they are
+        if (rc != T0B_OK) return rc;
+    }
+    GemmParams p{};
+    p.n_dst = 1;
+    p.M = static_cast<int>(d.rows); p.N = static_cast<int>(d.vocab); p.K = static_cast<int>(d.dim);
+    p.tiles_m = static_cast<int>((d.rows + plan.bm - 1) / plan.bm);
+    p.tiles_n = static_cast<int>((d.vocab + plan.bn - 1) / plan.bn);
+    p.split_k = 1;
+    p.kb_total = static_cast<int>((d.dim + 63) / 64);
+    p.kb_per_split = p.kb_total;
+    p.b_mn_major = d.trans_w ? 0 : 1;
+    p.raster_along_n = d.rows >= d.vocab ? 0 : 1;
+    p.group = raster_group(ctx, plan.bm, plan.bn, plan.cta_group, d.rows >= d.vocab);
+    p.mn_lbo = 8192; p.mn_sbo = 1024; p.mn_kstep = 2048;
+    p.status = ctx->status_dev;
+    p.wait_limit_ns = ctx->wait_limit_ns;
+    p.wait_hint_ns = ctx->wait_hint_ns;
+    p.tma_store = d.u ? 1 : 0;
+    p.head.part = reinterpret_cast<float2*>(d.part);
+    p.head.part_ld = static_cast<long long>(d.part_ld);
+    p.head.c = d.c;
+    p.head.ids = reinterpret_cast<const uint32_t*>(d.ids);
+    p.head.n_ids = static_cast<int>(d.n_ids);
+    p.head.z_sel = reinterpret_cast<float*>(d.z_sel);
+    p.head.store_u = d.u ? 1 : 0;
+    const int num_work = p.tiles_m * p.tiles_n;
+    if (plan.cta_group == 2) rc = launch_variant<256, 2, 1, 0, 1>(ctx, ta, tb, tc, p, num_work);
+    else if (plan.bn == 256) rc = launch_variant<256, 1, 1, 0, 1>(ctx, ta, tb, tc, p, num_work);
+    else rc = launch_variant<128, 1, 1, 0, 1>(ctx, ta, tb, tc, p, num_work);
+    if (rc == T0B_OK) ++ctx->launches;
+    return rc;
+}
+
+}  // namespace t0b
 
 extern "C" {
 

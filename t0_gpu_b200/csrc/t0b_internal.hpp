@@ -6,6 +6,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <string>
@@ -46,6 +47,9 @@ struct t0b_ctx {
     // Grow-only split-K workspace.
     void* ws = nullptr;
     size_t ws_bytes = 0;
+    // Grow-only workspace of the vocabulary losses (from the pool; never used by a call that is being captured).
+    uint64_t loss_ws = 0;
+    size_t loss_ws_bytes = 0;
     // bf16 copies of f32 weight buffers, by caller-chosen tensor id (GpuRuntime::bf16_cache, src/ignis/gpu_context.rs:392-432).
     struct Bf16Entry { uint64_t ptr; size_t n; };
     std::unordered_map<uint64_t, Bf16Entry> bf16_cache;
@@ -90,6 +94,10 @@ int32_t check_cuda(t0b_ctx* ctx, cudaError_t e, const char* what);
 // Status-word code of a kernel that met an index outside its table (the access is skipped); 101..105 are the GEMM's
 // bounded waits.
 constexpr int kDevBadIndex = 110;
+// Buffers that start one of the runtime's own allocations must fit in it: an undersized one is reported instead of faulting
+// on the device.  (Pointers from elsewhere, or into the middle of a buffer, are not known; null ones are skipped.)
+struct Extent { const char* name; uint64_t ptr; uint64_t bytes; };
+int32_t check_fits(t0b_ctx* ctx, const char* what, std::initializer_list<Extent> extents);
 int32_t precheck(t0b_ctx* ctx);                 // null / poisoned checks, sets the device
 // Launch-error check (+ sync and status-word check when !async). `count` kernels are added to the launch counter.
 int32_t finish(t0b_ctx* ctx, int32_t async, const char* what, int count = 1);
@@ -113,6 +121,39 @@ struct PlanInput {
     int num_sms;
 };
 void resolve_plan(const t0b_gemm_config* cfg, const PlanInput& in, t0b_gemm_plan* out);
+// Products inside other operators (t0b_gemm.cu): the same kernels and choice of tile as t0b_gemm.  Operands are 16-byte
+// aligned with pitches of whole 16 bytes.  `slabs` holds inner_gemm_slab_bytes() bytes for a split-K through global memory.
+struct InnerGemm {
+    int trans_a, trans_b;
+    uint64_t a, b, c;
+    uint32_t m, n, k;
+    uint64_t lda, ldb, ldc;
+    int out_bf16;
+    bool accumulate;   // C += A*B, f32
+    bool no_split;
+    uint64_t slabs;
+    size_t slab_bytes;
+};
+size_t inner_gemm_slab_bytes(t0b_ctx* ctx, const InnerGemm& d);
+int32_t inner_gemm(t0b_ctx* ctx, const InnerGemm& d);
+
+// The product x * head whose epilogue leaves softmax statistics instead of logits (HeadParams, gemm_sm100.cuh).
+struct HeadPlan { uint32_t bm, bn, cta_group, part_cols; };
+HeadPlan head_plan(t0b_ctx* ctx, uint32_t rows, uint32_t vocab, uint32_t dim);
+struct HeadGemm {
+    HeadPlan plan;
+    uint64_t x, w;               // bf16; w [dim, vocab], or [vocab, dim] with trans_w
+    uint64_t ldx, ldw;
+    uint32_t rows, dim, vocab;
+    int trans_w;
+    float c;                     // log2(e) / temperature
+    uint64_t part, part_ld;      // float2 [ceil(vocab / part_cols)][part_ld]
+    uint64_t ids, z_sel;         // u32 / f32 [rows][n_ids]
+    uint32_t n_ids;
+    uint64_t u, ldu;             // fp16 [rows][ldu], ldu a multiple of 8; 0 = statistics alone
+};
+int32_t head_gemm(t0b_ctx* ctx, const HeadGemm& d);
+
 // tile_ir front end (t0b_tile_ir.cpp): spec validation and the offsets of the epilogue arguments in its kernarg blob.
 bool tile_spec_valid(const t0b_tile_gemm* spec);
 size_t tile_kernarg_layout(const t0b_tile_gemm* spec, size_t* bias_off, size_t* scale_off, size_t* clamp_off);

@@ -1,0 +1,641 @@
+// The vocabulary losses straight from the hidden states and the head, without the [rows, vocab] logits:
+//   z = x * head,  p = softmax(z / T),  loss_r = sum_k q_rk (log q_rk - log p_r,id_rk)
+// with a sparse target distribution q per row: one word with q = 1 (cross entropy), or the softmax of a teacher's top logits.
+//   dz = (p sum(q) - q) * scale * weight_r / T,   dx = dz * head^T,   dhead = x^T * dz
+// The vocabulary goes through the tensor cores in tiles whose epilogue keeps the maximum and the sum of exponentials of every
+// row's part (head_gemm); a join over the parts gives the row's log-sum-exp and its loss.  That is all that an evaluation
+// does: 2 rows dim vocab operations, and nothing of the size rows x vocab is written.
+// For the gradient the same epilogue also leaves the exponentials of a piece of the rows, relative to their part's maximum,
+// in 16 bits (at most 1 GiB, whatever the number of rows); one pass turns them into dz in place, and two products give dx
+// and the head's gradient, which sums over the pieces in f32.  6 rows dim vocab operations in all: computing the exponentials
+// anew once the sums are known would cost 8, and the pass over 16-bit exponentials costs 4 bytes per element against
+// 2 dim operations (at dim 4096: 4 % of the step instead of 33 %).
+// Roundings: products of bf16 operands with f32 sums; exponentials to fp16 (HeadParams), dz to bf16 -- the operand type of
+// the two gradient products -- computed in f32 from the f32 logit at every word of q, where it is largest.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "ptx_sm100.cuh"
+#include "t0b_internal.hpp"
+
+using namespace t0b;
+
+namespace {
+
+constexpr uint32_t kNoWord = 0xffffffffu;
+constexpr uint64_t kPieceBytes = 1ull << 30;       // exponentials of one piece of rows
+constexpr uint64_t kPartBytes = 1ull << 28;        // per-part statistics of one piece of rows
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void join_stats(float& m, float& s, float m2, float s2, float c) {
+    const float mm = fmaxf(m, m2);
+    const float ref = mm == -INFINITY ? 0.0f : mm;
+    s = s * exp2_approx((m - ref) * c) + s2 * exp2_approx((m2 - ref) * c);
+    m = mm;
+}
+
+// ------------------------------------------------------------------------------------------------ the teacher's words
+// One row per threadIdx.y, one word per threadIdx.x (P = a power of two >= topk): q = softmax(t / T) over the words that are
+// there, entropy = sum q log q, and the words in ascending order of id (what the head's epilogue searches).  A word named
+// more than once keeps its first place with the sum of its q; the other places get q = -1.
+__global__ void __launch_bounds__(1024) teacher_words_kernel(const uint32_t* __restrict__ ids, const float* __restrict__ teacher,
+                                                             unsigned long long ldk, uint32_t rows, uint32_t topk, uint32_t vocab,
+                                                             float inv_t, uint32_t* __restrict__ out_ids, float* __restrict__ out_q,
+                                                             float* __restrict__ entropy, uint32_t* __restrict__ live, int* status) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    const uint32_t P = blockDim.x, x = threadIdx.x, y = threadIdx.y;
+    unsigned long long* key = reinterpret_cast<unsigned long long*>(smem) + static_cast<size_t>(y) * P;
+    float* val = reinterpret_cast<float*>(smem + static_cast<size_t>(blockDim.y) * P * 8) + static_cast<size_t>(y) * P;
+    const uint32_t row = blockIdx.x * blockDim.y + y;
+    const bool in = row < rows && x < topk;
+    uint32_t id = kNoWord;
+    float t = -INFINITY;
+    if (in) {
+        id = ids[row * ldk + x];
+        if (id != kNoWord && id >= vocab) {
+            *reinterpret_cast<volatile int*>(status) = kDevBadIndex;   // the word is left out
+            id = kNoWord;
+        }
+        if (id != kNoWord) t = teacher[row * ldk + x];
+    }
+    auto reduce = [&](float v, bool is_max) -> float {
+        __syncthreads();
+        val[x] = v;
+        __syncthreads();
+        for (uint32_t o = P >> 1; o > 0; o >>= 1) {
+            if (x < o) val[x] = is_max ? fmaxf(val[x], val[x + o]) : val[x] + val[x + o];
+            __syncthreads();
+        }
+        return val[0];
+    };
+    const float mx = reduce(t, true);
+    const float ref = mx == -INFINITY ? 0.0f : mx;
+    const float e = id == kNoWord ? 0.0f : expf((t - ref) * inv_t);
+    const float sum = reduce(e, false);
+    const bool some = sum > 0.0f || sum != sum;
+    const float lq = (t - ref) * inv_t - logf(sum);
+    const float q = (some && id != kNoWord) ? e / sum : 0.0f;
+    const float ent = reduce(q != 0.0f ? q * lq : 0.0f, false);
+    __syncthreads();
+    key[x] = (static_cast<unsigned long long>(some ? id : kNoWord) << 32) | x;
+    val[x] = q;
+    __syncthreads();
+    for (uint32_t size = 2; size <= P; size <<= 1)
+        for (uint32_t stride = size >> 1; stride > 0; stride >>= 1) {
+            const uint32_t other = x ^ stride;
+            if (other > x) {
+                const unsigned long long a = key[x], b = key[other];
+                if ((a > b) == ((x & size) == 0)) {
+                    key[x] = b;
+                    key[other] = a;
+                }
+            }
+            __syncthreads();
+        }
+    if (in) {
+        const uint32_t my = static_cast<uint32_t>(key[x] >> 32);
+        float qs = val[static_cast<uint32_t>(key[x])];
+        if (my != kNoWord) {
+            if (x > 0 && static_cast<uint32_t>(key[x - 1] >> 32) == my) qs = -1.0f;
+            else
+                for (uint32_t i = x + 1; i < P && static_cast<uint32_t>(key[i] >> 32) == my; ++i) qs += val[static_cast<uint32_t>(key[i])];
+        }
+        out_ids[static_cast<size_t>(row) * topk + x] = my;
+        out_q[static_cast<size_t>(row) * topk + x] = qs;
+        if (x == 0) {
+            entropy[row] = some ? ent : 0.0f;
+            live[row] = some ? 1u : 0u;
+        }
+    }
+}
+
+// --------------------------------------------------------------------------------------------------- rows as operands
+// out[r, c] = bf16(in[r, c]), rows of `cols` elements at a pitch of whole 16 bytes; a row that has no target is written as
+// zeros, whatever it holds (its hidden state may be anything, and 0 * NaN would reach the head's gradient).
+template <typename IN>
+__global__ void __launch_bounds__(256) pack_rows_kernel(const IN* __restrict__ in, unsigned long long ld, __nv_bfloat16* __restrict__ out,
+                                                        uint32_t ld_out, uint32_t rows, uint32_t cols, const uint32_t* __restrict__ targets,
+                                                        uint32_t vocab, const uint32_t* __restrict__ live) {
+    const uint32_t per_row = ld_out / 8;
+    const unsigned long long total = static_cast<unsigned long long>(rows) * per_row;
+    const bool vec = (reinterpret_cast<uintptr_t>(in) & 15) == 0 && ld % (16 / sizeof(IN)) == 0;
+    for (unsigned long long i = blockIdx.x * 256ull + threadIdx.x; i < total; i += gridDim.x * 256ull) {
+        const uint32_t r = static_cast<uint32_t>(i / per_row), c = static_cast<uint32_t>(i % per_row) * 8;
+        const bool on = targets ? targets[r] < vocab : (live ? live[r] != 0 : true);
+        uint4 o = make_uint4(0, 0, 0, 0);
+        if (on) {
+            const IN* src = in + r * ld + c;
+            if constexpr (sizeof(IN) == 2) {
+                if (vec && c + 8 <= cols) o = *reinterpret_cast<const uint4*>(src);
+                else {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t a = c + 2 * e < cols ? *reinterpret_cast<const uint16_t*>(src + 2 * e) : 0u;
+                        const uint32_t b = c + 2 * e + 1 < cols ? *reinterpret_cast<const uint16_t*>(src + 2 * e + 1) : 0u;
+                        w[e] = a | (b << 16);
+                    }
+                    o = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            } else {
+                float v[8];
+                if (vec && c + 8 <= cols) {
+                    const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+                    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? static_cast<float>(src[e]) : 0.0f;
+                }
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+                    w[e] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+                o = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+        *reinterpret_cast<uint4*>(out + static_cast<unsigned long long>(r) * ld_out + c) = o;
+    }
+}
+
+// out[r, c] = bf16(acc[r, c]): the head's gradient summed in f32 over several pieces, rounded once.
+__global__ void __launch_bounds__(256) round_rows_kernel(const float* __restrict__ acc, uint32_t ld_acc, __nv_bfloat16* __restrict__ out,
+                                                         unsigned long long ld, uint32_t rows, uint32_t cols) {
+    const uint32_t per_row = (cols + 7) / 8;
+    const unsigned long long total = static_cast<unsigned long long>(rows) * per_row;
+    const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && ld % 8 == 0;
+    for (unsigned long long i = blockIdx.x * 256ull + threadIdx.x; i < total; i += gridDim.x * 256ull) {
+        const uint32_t r = static_cast<uint32_t>(i / per_row), c = static_cast<uint32_t>(i % per_row) * 8;
+        const float4* src = reinterpret_cast<const float4*>(acc + static_cast<unsigned long long>(r) * ld_acc + c);   // pitch: whole 8 elements
+        const float4 a = __ldcs(src), b = __ldcs(src + 1);
+        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        __nv_bfloat16* dst = out + r * ld + c;
+        if (vec && c + 8 <= cols) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+                w[e] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c + e < cols) dst[e] = __float2bfloat16_rn(v[e]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------- joining the parts
+// What the join and the gradient pass know about the targets of a row.
+struct Targets {
+    const uint32_t* ids;      // [rows][n_ids]
+    const float* q;           // [rows][n_ids], null: cross entropy (one word, q = 1)
+    const float* entropy;     // [rows], with q
+    const uint32_t* live;     // [rows], with q
+    const float* z_sel;       // [rows][n_ids]
+    uint32_t n_ids, vocab;
+};
+__device__ __forceinline__ bool row_live(const Targets& t, uint32_t row) { return t.q ? t.live[row] != 0 : t.ids[row] < t.vocab; }
+
+// One block per 32 rows: warps walk the parts (a warp's load is 32 neighbouring rows of one part), the warps' results meet in
+// shared memory, then warp i finishes row i: stats[row] = (max z, sum of exp), the loss and log-sum-exp.
+__global__ void __launch_bounds__(1024) join_parts_kernel(const float2* __restrict__ part, unsigned long long part_ld, uint32_t parts, uint32_t rows,
+                                                          float c, float inv_t, Targets tg, float2* __restrict__ stats,
+                                                          float* __restrict__ losses, float* __restrict__ lse_out, int* status) {
+    __shared__ float2 sh[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t row = blockIdx.x * 32 + lane;
+    float m = -INFINITY, s = 0.0f;
+    if (row < rows) {
+        for (uint32_t i = warp; i < parts; i += 128) {
+            float2 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = i + 32 * u < parts ? part[(i + 32 * u) * part_ld + row] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) join_stats(m, s, v[u].x, v[u].y, c);
+        }
+    }
+    sh[warp][lane] = make_float2(m, s);
+    __syncthreads();
+    const uint32_t r = blockIdx.x * 32 + warp;
+    if (r >= rows) return;
+    m = sh[lane][warp].x;
+    s = sh[lane][warp].y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+        join_stats(m, s, m2, s2, c);
+    }
+    const bool none = m == -INFINITY && s == 0.0f;       // every logit is -inf: the row has no distribution
+    const bool live = row_live(tg, r) && !none;
+    const float log_s = logf(s);
+    float cross = 0.0f;
+    if (live) {
+        if (tg.q) {
+            for (uint32_t k = lane; k < tg.n_ids; k += 32) {
+                const float q = tg.q[static_cast<size_t>(r) * tg.n_ids + k];
+                if (tg.ids[static_cast<size_t>(r) * tg.n_ids + k] == kNoWord || q == 0.0f || q < 0.0f) continue;
+                cross += q * (log_s - (tg.z_sel[static_cast<size_t>(r) * tg.n_ids + k] - m) * inv_t);
+            }
+            cross = warp_sum(cross) + tg.entropy[r];
+        } else {
+            cross = log_s - (tg.z_sel[r] - m) * inv_t;
+        }
+    }
+    if (lane == 0) {
+        stats[r] = make_float2(m, s);
+        if (losses) losses[r] = live ? cross : 0.0f;
+        if (lse_out) lse_out[r] = live ? m * inv_t + log_s : 0.0f;
+        if (!tg.q && tg.ids[r] >= tg.vocab && tg.ids[r] != kNoWord) *reinterpret_cast<volatile int*>(status) = kDevBadIndex;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- the gradient of z
+// u (fp16, relative to its part's maximum) becomes dz (bf16) in place: a block takes kGradCols columns of one row.  The
+// words of the targets are written last, from their f32 logit.  Bound by HBM: 2 bytes in, 2 bytes out per element.
+constexpr int kGradVecs = 4;
+constexpr uint32_t kGradCols = 256 * 8 * kGradVecs;
+__global__ void __launch_bounds__(256) dz_kernel(__half* __restrict__ u, unsigned long long ldu, uint32_t rows, const float2* __restrict__ part,
+                                                 unsigned long long part_ld, uint32_t part_shift, const float2* __restrict__ stats,
+                                                 const float* __restrict__ weights, float scale, float c, Targets tg) {
+    const uint32_t row = blockIdx.y;
+    const uint32_t c0 = blockIdx.x * kGradCols;
+    __half* ur = u + row * ldu;
+    __nv_bfloat16* gr = reinterpret_cast<__nv_bfloat16*>(ur);
+    const float2 st = stats[row];
+    const bool live = row_live(tg, row) && !(st.x == -INFINITY && st.y == 0.0f);
+    const float a = live ? scale * (weights ? weights[row] : 1.0f) : 0.0f;
+    const float inv = 1.0f / st.y;
+    uint4 raw[kGradVecs];
+#pragma unroll
+    for (int i = 0; i < kGradVecs; ++i) {
+        const uint32_t col = c0 + (i * 256 + threadIdx.x) * 8;
+        if (live && col < ldu) raw[i] = *reinterpret_cast<const uint4*>(ur + col);
+    }
+#pragma unroll
+    for (int i = 0; i < kGradVecs; ++i) {
+        const uint32_t col = c0 + (i * 256 + threadIdx.x) * 8;
+        if (col >= ldu) continue;
+        uint4 o = make_uint4(0, 0, 0, 0);
+        if (live) {
+            const float f = a * (exp2_approx((part[(col >> part_shift) * part_ld + row].x - st.x) * c) * inv);
+            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+            uint32_t g[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v.x * f, v.y * f);
+                g[e] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            o = make_uint4(g[0], g[1], g[2], g[3]);
+        }
+        *reinterpret_cast<uint4*>(gr + col) = o;
+    }
+    if (!live) return;
+    __syncthreads();
+    for (uint32_t k = threadIdx.x; k < tg.n_ids; k += 256) {
+        const size_t at = static_cast<size_t>(row) * tg.n_ids + k;
+        const uint32_t id = tg.ids[at];
+        if (id - c0 >= kGradCols || id >= tg.vocab) continue;
+        const float q = tg.q ? tg.q[at] : 1.0f;
+        if (q < 0.0f) continue;
+        gr[id] = __float2bfloat16_rn(a * (exp2_approx((tg.z_sel[at] - st.x) * c) * inv - q));
+    }
+}
+
+uint64_t align256(uint64_t x) { return (x + 255) & ~255ull; }
+uint64_t round8(uint64_t x) { return (x + 7) & ~7ull; }
+
+// Everything a call will do, from its arguments alone: pieces, tile, operand copies, scratch layout.
+struct Plan {
+    bool grads, dx, dw;
+    uint32_t piece, pieces;
+    HeadPlan head;
+    uint32_t parts;
+    uint64_t part_ld;
+    uint64_t ldu;
+    bool copy_x, copy_w;
+    uint64_t ldx, ldw;                 // pitches of the operands as the products read them
+    uint64_t w_rows, w_cols;
+    bool acc_dw;                       // bf16 gradient of the head over several pieces: summed in f32 in the scratch
+    uint64_t ld_acc;
+    uint64_t x, w, ids, q, entropy, live, z_sel, part, stats, u, acc, slabs;   // offsets
+    uint64_t slab_bytes, total;
+};
+
+bool tma_ok(uint64_t ptr, uint64_t ld) { return ptr % 16 == 0 && ld % 8 == 0; }
+
+InnerGemm dx_gemm(const t0b_linear_loss& d, const Plan& p, uint64_t u, uint64_t w, uint32_t r0, uint32_t n) {
+    InnerGemm g{};
+    g.trans_a = 0;
+    g.trans_b = d.trans_w ? 0 : 1;
+    g.a = u; g.b = w;
+    g.c = d.dx + static_cast<uint64_t>(r0) * d.lddx * (d.dx_dtype == T0B_OUT_BF16 ? 2 : 4);
+    g.m = n; g.n = d.dim; g.k = d.vocab;
+    g.lda = p.ldu; g.ldb = p.ldw; g.ldc = d.lddx;
+    g.out_bf16 = d.dx_dtype == T0B_OUT_BF16;
+    return g;
+}
+
+InnerGemm dw_gemm(const t0b_linear_loss& d, const Plan& p, uint64_t u, uint64_t x, uint64_t acc, uint32_t r0, uint32_t n) {
+    InnerGemm g{};
+    const uint64_t xr = x + static_cast<uint64_t>(r0) * p.ldx * 2;
+    g.trans_a = 1;
+    g.trans_b = 0;
+    if (d.trans_w) { g.a = u; g.b = xr; g.m = d.vocab; g.n = d.dim; g.lda = p.ldu; g.ldb = p.ldx; }
+    else { g.a = xr; g.b = u; g.m = d.dim; g.n = d.vocab; g.lda = p.ldx; g.ldb = p.ldu; }
+    g.k = n;
+    g.c = p.acc_dw ? acc : d.dw;
+    g.ldc = p.acc_dw ? p.ld_acc : d.lddw;
+    g.out_bf16 = !p.acc_dw && d.dw_dtype == T0B_OUT_BF16;
+    g.accumulate = r0 > 0;
+    g.no_split = p.pieces > 1;
+    return g;
+}
+
+Plan make_plan(t0b_ctx* ctx, const t0b_linear_loss& d, uint32_t n_ids, bool teacher) {
+    Plan p{};
+    p.dx = d.dx != 0;
+    p.dw = d.dw != 0;
+    p.grads = p.dx || p.dw;
+    p.ldu = round8(d.vocab);
+    // Pieces of rows: whole 256-row tiles, as even as they come.
+    uint64_t fit = p.grads ? kPieceBytes / (p.ldu * 2) : kPartBytes / ((d.vocab / 64 + 1) * 8ull);
+    fit = std::max<uint64_t>(256, fit / 256 * 256);
+    if (d.piece_rows > 0) fit = d.piece_rows;
+    p.pieces = static_cast<uint32_t>((d.rows + fit - 1) / fit);
+    p.piece = (d.rows + p.pieces - 1) / p.pieces;
+    if (p.pieces > 1 && d.piece_rows == 0) p.piece = (p.piece + 255) / 256 * 256;
+    if (p.pieces > 1 && d.piece_rows > 0) p.piece = d.piece_rows;
+    p.pieces = (d.rows + p.piece - 1) / p.piece;
+    p.head = head_plan(ctx, p.piece, d.vocab, d.dim);
+    p.parts = (d.vocab + p.head.part_cols - 1) / p.head.part_cols;
+    p.part_ld = (p.piece + 31ull) / 32 * 32;
+    p.copy_x = p.grads || d.x_dtype != T0B_OUT_BF16 || !tma_ok(d.x, d.ldx);
+    p.ldx = p.copy_x ? round8(d.dim) : d.ldx;
+    p.w_rows = d.trans_w ? d.vocab : d.dim;
+    p.w_cols = d.trans_w ? d.dim : d.vocab;
+    p.copy_w = !tma_ok(d.w, d.ldw);
+    p.ldw = p.copy_w ? round8(p.w_cols) : d.ldw;
+    p.acc_dw = p.dw && p.pieces > 1 && d.dw_dtype == T0B_OUT_BF16;
+    p.ld_acc = round8(p.w_cols);
+    uint64_t off = 0;
+    auto take = [&](uint64_t bytes) { const uint64_t at = off; off += align256(bytes); return at; };
+    const uint64_t rows = d.rows;
+    p.stats = take(rows * 8);
+    p.z_sel = take(rows * n_ids * 4);
+    if (teacher) {
+        p.ids = take(rows * n_ids * 4);
+        p.q = take(rows * n_ids * 4);
+        p.entropy = take(rows * 4);
+        p.live = take(rows * 4);
+    }
+    if (p.copy_x) p.x = take(rows * p.ldx * 2);
+    if (p.copy_w) p.w = take(p.w_rows * p.ldw * 2);
+    p.part = take(p.parts * p.part_ld * 8);
+    if (p.grads) p.u = take(p.piece * p.ldu * 2);
+    if (p.acc_dw) p.acc = take(p.w_rows * p.ld_acc * 4);
+    // Slabs of a split contraction, for whichever product of whichever piece wants most; the products run one after another.
+    for (uint32_t r0 = 0; p.grads && r0 < d.rows; r0 += p.piece) {
+        const uint32_t n = std::min(p.piece, d.rows - r0);
+        if (r0 > 0 && n == p.piece) continue;   // like the first
+        if (p.dx) p.slab_bytes = std::max<uint64_t>(p.slab_bytes, inner_gemm_slab_bytes(ctx, dx_gemm(d, p, 256, 256, r0, n)));
+        if (p.dw) p.slab_bytes = std::max<uint64_t>(p.slab_bytes, inner_gemm_slab_bytes(ctx, dw_gemm(d, p, 256, 256, 256, r0, n)));
+    }
+    p.slabs = take(p.slab_bytes);
+    p.total = std::max<uint64_t>(off, 256);
+    return p;
+}
+
+int32_t check_desc(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d) {
+    auto bad = [&](const char* msg) { return set_error(ctx, T0B_ERR_INVALID, "%s: %s", what, msg); };
+    if (!d.x || !d.w) return bad("null x or w");
+    if (d.dim == 0 || d.vocab == 0) return bad("an empty head");
+    if (d.rows > 0x7fffff00u || d.dim > 0x7fffff00u || d.vocab > 0x7fffff00u) return bad("a size is over 2^31");
+    if (!d.losses && !d.lse && !d.dx && !d.dw) return bad("no output is asked for");
+    if (d.ldx < d.dim || d.ldw < (d.trans_w ? d.dim : d.vocab) || (d.dx && d.lddx < d.dim) || (d.dw && d.lddw < (d.trans_w ? d.dim : d.vocab)))
+        return bad("a pitch is smaller than its row");
+    if (d.x_dtype != T0B_OUT_F32 && d.x_dtype != T0B_OUT_BF16) return bad("unknown x_dtype");
+    if ((d.dx && d.dx_dtype != T0B_OUT_F32 && d.dx_dtype != T0B_OUT_BF16) || (d.dw && d.dw_dtype != T0B_OUT_F32 && d.dw_dtype != T0B_OUT_BF16))
+        return bad("unknown gradient type");
+    if (!std::isfinite(d.scale)) return bad("scale is not finite");
+    const uint64_t xe = d.x_dtype == T0B_OUT_BF16 ? 2 : 4, dxe = d.dx_dtype == T0B_OUT_BF16 ? 2 : 4, dwe = d.dw_dtype == T0B_OUT_BF16 ? 2 : 4;
+    if (d.x % xe || d.w % 2 || (d.dx && d.dx % dxe) || (d.dw && d.dw % dwe) || d.losses % 4 || d.lse % 4 || d.row_weights % 4)
+        return bad("a pointer is not aligned to its element");
+    if (d.rows == 0) return T0B_OK;
+    const uint64_t wr = d.trans_w ? d.vocab : d.dim, wc = d.trans_w ? d.dim : d.vocab;
+    return check_fits(ctx, what, {{"x", d.x, ((d.rows - 1ull) * d.ldx + d.dim) * xe}, {"w", d.w, ((wr - 1) * d.ldw + wc) * 2},
+                                  {"dx", d.dx, ((d.rows - 1ull) * d.lddx + d.dim) * dxe}, {"dw", d.dw, ((wr - 1) * d.lddw + wc) * dwe},
+                                  {"losses", d.losses, d.rows * 4ull}, {"lse", d.lse, d.rows * 4ull}, {"row_weights", d.row_weights, d.rows * 4ull}});
+}
+
+// The scratch of a call: the caller's, else the context's, which grows as needed.  A captured call has to bring its own: the
+// context's may be replaced by a later, larger call while the graph still refers to it.
+int32_t get_scratch(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d, uint64_t need, uint64_t* at) {
+    if (d.scratch) {
+        if (d.scratch % 256 || d.scratch_bytes < need)
+            return set_error(ctx, T0B_ERR_INVALID, "%s: scratch must be 256-byte aligned and hold %llu bytes (got %llu)", what,
+                             static_cast<unsigned long long>(need), static_cast<unsigned long long>(d.scratch_bytes));
+        *at = d.scratch;
+        return check_fits(ctx, what, {{"scratch", d.scratch, need}});
+    }
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    int32_t rc = check_cuda(ctx, cudaStreamIsCapturing(ctx->stream, &st), "cudaStreamIsCapturing");
+    if (rc != T0B_OK) return rc;
+    if (ctx->capturing || st != cudaStreamCaptureStatusNone)
+        return set_error(ctx, T0B_ERR_INVALID, "%s: a captured call needs a scratch of its own (%llu bytes)", what, static_cast<unsigned long long>(need));
+    if (ctx->loss_ws_bytes < need) {
+        const uint64_t old = ctx->loss_ws;
+        ctx->loss_ws = 0;
+        ctx->loss_ws_bytes = 0;
+        if (old) {
+            rc = t0b_free(ctx, old);   // waits for the stream
+            if (rc != T0B_OK) return rc;
+        }
+        rc = t0b_alloc(ctx, need, &ctx->loss_ws);
+        if (rc != T0B_OK) return rc;
+        ctx->loss_ws_bytes = need;
+    }
+    *at = ctx->loss_ws;
+    return T0B_OK;
+}
+
+uint32_t lin_blocks(t0b_ctx* ctx, uint64_t items) {
+    return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>((items + 255) / 256, static_cast<uint64_t>(ctx->num_sms) * 8)));
+}
+
+struct Teacher { uint64_t ids, logits, ldk; uint32_t topk; };   // cross entropy: ids = targets, topk = 1, logits = 0
+
+int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d, const Teacher& te, float temperature, int32_t async) {
+    const uint64_t dwe = d.dw_dtype == T0B_OUT_BF16 ? 2 : 4;
+    if (d.rows == 0) {
+        if (!d.dw) return T0B_OK;
+        const uint64_t wr = d.trans_w ? d.vocab : d.dim, wc = d.trans_w ? d.dim : d.vocab;
+        const int32_t rc = check_cuda(ctx, cudaMemset2DAsync(reinterpret_cast<void*>(d.dw), d.lddw * dwe, 0, wc * dwe, wr, ctx->stream), "cudaMemset2DAsync(dw)");
+        return rc != T0B_OK ? rc : finish(ctx, async, what, 0);
+    }
+    const bool teacher = te.logits != 0;
+    const Plan p = make_plan(ctx, d, te.topk, teacher);
+    uint64_t base = 0;
+    int32_t rc = get_scratch(ctx, what, d, p.total, &base);
+    if (rc != T0B_OK) return rc;
+    const float c = 1.4426950408889634f / temperature, inv_t = 1.0f / temperature;
+    cudaStream_t st = ctx->stream;
+    int launched = 0;
+
+    if (teacher) {
+        uint32_t P = 32;
+        while (P < te.topk) P *= 2;
+        const uint32_t ny = std::max(1u, 128u / P);
+        teacher_words_kernel<<<(d.rows + ny - 1) / ny, dim3(P, ny), static_cast<size_t>(P) * ny * 12, st>>>(
+            reinterpret_cast<const uint32_t*>(te.ids), reinterpret_cast<const float*>(te.logits), te.ldk, d.rows, te.topk, d.vocab, inv_t,
+            reinterpret_cast<uint32_t*>(base + p.ids), reinterpret_cast<float*>(base + p.q), reinterpret_cast<float*>(base + p.entropy),
+            reinterpret_cast<uint32_t*>(base + p.live), ctx->status_dev);
+        ++launched;
+    }
+    const uint64_t x = p.copy_x ? base + p.x : d.x, w = p.copy_w ? base + p.w : d.w;
+    if (p.copy_x) {
+        const uint32_t blocks = lin_blocks(ctx, d.rows * (p.ldx / 8));
+        const uint32_t* targets = teacher ? nullptr : reinterpret_cast<const uint32_t*>(te.ids);
+        const uint32_t* live = teacher ? reinterpret_cast<const uint32_t*>(base + p.live) : nullptr;
+        __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(base + p.x);
+        if (d.x_dtype == T0B_OUT_BF16)
+            pack_rows_kernel<<<blocks, 256, 0, st>>>(reinterpret_cast<const __nv_bfloat16*>(d.x), d.ldx, out, static_cast<uint32_t>(p.ldx), d.rows, d.dim, targets, d.vocab, live);
+        else
+            pack_rows_kernel<<<blocks, 256, 0, st>>>(reinterpret_cast<const float*>(d.x), d.ldx, out, static_cast<uint32_t>(p.ldx), d.rows, d.dim, targets, d.vocab, live);
+        ++launched;
+    }
+    if (p.copy_w) {
+        pack_rows_kernel<<<lin_blocks(ctx, p.w_rows * (p.ldw / 8)), 256, 0, st>>>(
+            reinterpret_cast<const __nv_bfloat16*>(d.w), d.ldw, reinterpret_cast<__nv_bfloat16*>(base + p.w), static_cast<uint32_t>(p.ldw),
+            static_cast<uint32_t>(p.w_rows), static_cast<uint32_t>(p.w_cols), nullptr, 0u, nullptr);
+        ++launched;
+    }
+    uint32_t part_shift = 0;
+    while ((1u << part_shift) < p.head.part_cols) ++part_shift;
+    for (uint32_t r0 = 0; r0 < d.rows; r0 += p.piece) {
+        const uint32_t n = std::min(p.piece, d.rows - r0);
+        Targets tg{};
+        tg.ids = reinterpret_cast<const uint32_t*>(teacher ? base + p.ids : te.ids) + static_cast<size_t>(r0) * te.topk;
+        if (teacher) {
+            tg.q = reinterpret_cast<const float*>(base + p.q) + static_cast<size_t>(r0) * te.topk;
+            tg.entropy = reinterpret_cast<const float*>(base + p.entropy) + r0;
+            tg.live = reinterpret_cast<const uint32_t*>(base + p.live) + r0;
+        }
+        tg.z_sel = reinterpret_cast<const float*>(base + p.z_sel) + static_cast<size_t>(r0) * te.topk;
+        tg.n_ids = te.topk;
+        tg.vocab = d.vocab;
+        HeadGemm hg{};
+        hg.plan = p.head;
+        hg.x = x + static_cast<uint64_t>(r0) * p.ldx * 2;
+        hg.w = w;
+        hg.ldx = p.ldx; hg.ldw = p.ldw;
+        hg.rows = n; hg.dim = d.dim; hg.vocab = d.vocab; hg.trans_w = d.trans_w;
+        hg.c = c;
+        hg.part = base + p.part; hg.part_ld = p.part_ld;
+        hg.ids = reinterpret_cast<uint64_t>(tg.ids);
+        hg.z_sel = reinterpret_cast<uint64_t>(tg.z_sel);
+        hg.n_ids = te.topk;
+        hg.u = p.grads ? base + p.u : 0;
+        hg.ldu = p.ldu;
+        rc = head_gemm(ctx, hg);
+        if (rc != T0B_OK) return rc;
+        float2* stats = reinterpret_cast<float2*>(base + p.stats) + r0;
+        join_parts_kernel<<<(n + 31) / 32, 1024, 0, st>>>(reinterpret_cast<const float2*>(base + p.part), p.part_ld, p.parts, n, c, inv_t, tg, stats,
+                                                          d.losses ? reinterpret_cast<float*>(d.losses) + r0 : nullptr,
+                                                          d.lse ? reinterpret_cast<float*>(d.lse) + r0 : nullptr, ctx->status_dev);
+        ++launched;
+        if (!p.grads) continue;
+        // gridDim.y is limited to 65535 rows a launch.
+        for (uint32_t y0 = 0; y0 < n; y0 += 65535u) {
+            const uint32_t ny = std::min(65535u, n - y0);
+            Targets t2 = tg;
+            t2.ids += static_cast<size_t>(y0) * te.topk;
+            if (teacher) { t2.q += static_cast<size_t>(y0) * te.topk; t2.entropy += y0; t2.live += y0; }
+            t2.z_sel += static_cast<size_t>(y0) * te.topk;
+            dz_kernel<<<dim3(static_cast<uint32_t>((p.ldu + kGradCols - 1) / kGradCols), ny), 256, 0, st>>>(
+                reinterpret_cast<__half*>(base + p.u) + y0 * p.ldu, p.ldu, ny, reinterpret_cast<const float2*>(base + p.part) + y0, p.part_ld, part_shift,
+                stats + y0, d.row_weights ? reinterpret_cast<const float*>(d.row_weights) + r0 + y0 : nullptr, d.scale * inv_t, c, t2);
+            ++launched;
+        }
+        rc = check_cuda(ctx, cudaGetLastError(), what);
+        if (rc != T0B_OK) return rc;
+        if (p.dx) {
+            InnerGemm g = dx_gemm(d, p, base + p.u, w, r0, n);
+            g.slabs = base + p.slabs;
+            g.slab_bytes = p.slab_bytes;
+            rc = inner_gemm(ctx, g);
+            if (rc != T0B_OK) return rc;
+        }
+        if (p.dw) {
+            InnerGemm g = dw_gemm(d, p, base + p.u, x, base + p.acc, r0, n);
+            g.slabs = base + p.slabs;
+            g.slab_bytes = p.slab_bytes;
+            rc = inner_gemm(ctx, g);
+            if (rc != T0B_OK) return rc;
+        }
+    }
+    if (p.acc_dw) {
+        round_rows_kernel<<<lin_blocks(ctx, p.w_rows * ((p.w_cols + 7) / 8)), 256, 0, st>>>(
+            reinterpret_cast<const float*>(base + p.acc), static_cast<uint32_t>(p.ld_acc), reinterpret_cast<__nv_bfloat16*>(d.dw), d.lddw,
+            static_cast<uint32_t>(p.w_rows), static_cast<uint32_t>(p.w_cols));
+        ++launched;
+    }
+    return finish(ctx, async, what, launched);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t t0b_linear_loss_scratch_bytes(t0b_ctx* ctx, const t0b_linear_loss* loss, uint32_t topk) {
+    if (!ctx || !loss || loss->rows == 0 || loss->dim == 0 || loss->vocab == 0) return 0;
+    std::lock_guard<std::recursive_mutex> lk(ctx->mu);
+    if (precheck(ctx) != T0B_OK) return 0;
+    return make_plan(ctx, *loss, std::max(1u, topk), topk > 0).total;
+}
+
+int32_t t0b_linear_ce(t0b_ctx* ctx, const t0b_linear_loss* loss, uint64_t targets, int32_t async) {
+    int32_t rc = precheck(ctx);
+    if (rc != T0B_OK) return rc;
+    if (!loss || !targets || targets % 4) return set_error(ctx, T0B_ERR_INVALID, "linear_ce: null or misaligned pointer");
+    std::lock_guard<std::recursive_mutex> lk(ctx->mu);
+    rc = check_desc(ctx, "linear_ce", *loss);
+    if (rc == T0B_OK) rc = check_fits(ctx, "linear_ce", {{"targets", targets, loss->rows * 4ull}});
+    if (rc != T0B_OK) return rc;
+    return run_linear_loss(ctx, "linear_ce", *loss, Teacher{targets, 0, 1, 1}, 1.0f, async);
+}
+
+int32_t t0b_linear_topk_distill(t0b_ctx* ctx, const t0b_linear_loss* loss, uint64_t ids, uint64_t teacher, uint32_t topk, uint64_t ldk,
+                                float temperature, int32_t async) {
+    int32_t rc = precheck(ctx);
+    if (rc != T0B_OK) return rc;
+    if (!loss || !ids || !teacher || ids % 4 || teacher % 4) return set_error(ctx, T0B_ERR_INVALID, "linear_topk_distill: null or misaligned pointer");
+    if (topk == 0 || topk > T0B_MAX_TOPK || ldk < topk)
+        return set_error(ctx, T0B_ERR_INVALID, "linear_topk_distill: topk %u is outside 1..%d, or its pitch %llu is smaller", topk, T0B_MAX_TOPK,
+                         static_cast<unsigned long long>(ldk));
+    if (!(temperature > 0.0f) || !std::isfinite(temperature))
+        return set_error(ctx, T0B_ERR_INVALID, "linear_topk_distill: temperature %g must be positive and finite", temperature);
+    std::lock_guard<std::recursive_mutex> lk(ctx->mu);
+    rc = check_desc(ctx, "linear_topk_distill", *loss);
+    if (rc == T0B_OK && loss->rows > 0)
+        rc = check_fits(ctx, "linear_topk_distill", {{"ids", ids, ((loss->rows - 1ull) * ldk + topk) * 4}, {"teacher", teacher, ((loss->rows - 1ull) * ldk + topk) * 4}});
+    if (rc != T0B_OK) return rc;
+    return run_linear_loss(ctx, "linear_topk_distill", *loss, Teacher{ids, teacher, ldk, topk}, temperature, async);
+}
+
+}  // extern "C"

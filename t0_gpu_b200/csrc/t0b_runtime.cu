@@ -43,6 +43,17 @@ int32_t precheck(t0b_ctx* ctx) {
     return T0B_OK;
 }
 
+int32_t check_fits(t0b_ctx* ctx, const char* what, std::initializer_list<Extent> extents) {
+    for (const Extent& e : extents) {
+        if (!e.ptr) continue;
+        auto it = ctx->live.find(reinterpret_cast<void*>(e.ptr));
+        if (it != ctx->live.end() && e.bytes > it->second)
+            return set_error(ctx, T0B_ERR_INVALID, "%s: %s needs %llu bytes, its buffer has %llu", what, e.name,
+                             static_cast<unsigned long long>(e.bytes), static_cast<unsigned long long>(it->second));
+    }
+    return T0B_OK;
+}
+
 int take_device_status(t0b_ctx* ctx) {
     if (!ctx || !ctx->status_host) return 0;
     volatile int* w = reinterpret_cast<volatile int*>(ctx->status_host);

@@ -9,8 +9,10 @@ from __future__ import annotations
 
 from typing import Optional, Tuple
 
-from ._lib import lib
-from .gpu_context import OUT_F32, GpuBuffer, GpuRuntime
+import ctypes as C
+
+from ._lib import LinearLossC, lib
+from .gpu_context import OUT_BF16, OUT_F32, GpuBuffer, GpuRuntime, _addr
 
 RMSNORM_EPS = 1e-5   # the constant Ignis hard-codes (src/ignis/ops/rmsnorm.rs:18); pass eps explicitly to override
 
@@ -134,6 +136,97 @@ def cross_entropy(rt: GpuRuntime, logits: GpuBuffer, targets: GpuBuffer, batch: 
     loss = float(losses.read_as(np.float32, batch).mean())
     rt.recycle(losses)
     return loss, grad
+
+
+NO_WORD = 0xFFFFFFFF     # a target, or a teacher's word, that is not there
+_ELEM = {OUT_F32: 4, OUT_BF16: 2}
+
+
+def topk_distill(rt: GpuRuntime, logits, ids, teacher, rows: int, cols: int, topk: int, *, temperature: float = 1.0,
+                 scale: Optional[float] = None, row_weights=None, grads: bool = True, logits_dtype: int = OUT_F32,
+                 grad_dtype: int = OUT_F32, ld: Optional[int] = None, ldk: Optional[int] = None, losses=None, dlogits=None):
+    """Distillation from a teacher's top logits, beside `cross_entropy`: logits [rows, cols], ids u32 and teacher f32
+    [rows, topk] (`NO_WORD` = no word).  Returns (losses f32[rows], dlogits): per row the divergence of softmax(z / T) from
+    the softmax of the teacher's logits over its words, and the gradient of scale * sum(row_weights * losses) (default scale
+    1 / rows: the mean), None without `grads`.  Buffers are `GpuBuffer`s or device addresses; outputs that are not given come
+    from the pool, and `dlogits` may be `logits` when the types agree.  Only queues work."""
+    ld, ldk = ld if ld is not None else cols, ldk if ldk is not None else topk
+    losses = losses if losses is not None else rt.alloc(max(rows * 4, 16))
+    if grads and dlogits is None:
+        dlogits = rt.alloc(max(rows * ld * _ELEM.get(grad_dtype, 4), 16))
+    rt._check(lib().t0b_topk_distill(rt.handle, _addr(logits), logits_dtype, _addr(ids), _addr(teacher), _addr(row_weights), _addr(losses),
+                                     _addr(dlogits) if grads else 0, grad_dtype, rows, cols, ld, topk, ldk, temperature,
+                                     scale if scale is not None else 1.0 / max(rows, 1), 1))
+    return losses, dlogits if grads else None
+
+
+def _linear_loss(rt: GpuRuntime, call, x, w, rows, dim, vocab, topk, scale, row_weights, grads, trans_w, x_dtype, w_dtype, dx_dtype,
+                 dw_dtype, ldx, ldw, weight_id, losses, lse, dx, dw, piece_rows, scratch):
+    w_rows, w_cols = (vocab, dim) if trans_w else (dim, vocab)
+    w16 = None
+    if w_dtype == OUT_F32:
+        if ldw is not None and ldw != w_cols:
+            raise ValueError("linear loss: an f32 head is converted as a whole and has no pitch of its own")
+        if weight_id is not None:
+            w = rt.get_or_create_bf16(weight_id, w if isinstance(w, GpuBuffer) else GpuBuffer(rt, w, 0, False), w_rows * w_cols)
+        else:
+            w16 = rt.alloc(max(w_rows * w_cols * 2, 16))
+            rt._check(lib().t0b_cast_f32_to_bf16(rt.handle, _addr(w), w16.gpu_addr(), w_rows * w_cols, 1))
+            w = w16
+    elif w_dtype != OUT_BF16:
+        raise ValueError(f"linear loss: unknown w_dtype {w_dtype}")
+    losses = losses if losses is not None else rt.alloc(max(rows * 4, 16))
+    if grads and dx is None:
+        dx = rt.alloc(max(rows * dim * _ELEM.get(dx_dtype, 4), 16))
+    if grads and dw is None:
+        dw = rt.alloc(max(w_rows * w_cols * _ELEM.get(dw_dtype, 4), 16))
+    d = LinearLossC(x=_addr(x), w=_addr(w), ldx=ldx if ldx is not None else dim, ldw=ldw if ldw is not None else w_cols, row_weights=_addr(row_weights),
+                    losses=_addr(losses), lse=_addr(lse), dx=_addr(dx) if grads else 0, dw=_addr(dw) if grads else 0, lddx=dim, lddw=w_cols,
+                    scratch=_addr(scratch), scratch_bytes=scratch.size() if scratch is not None else 0, rows=rows, dim=dim, vocab=vocab,
+                    trans_w=int(trans_w), piece_rows=piece_rows, x_dtype=x_dtype, dx_dtype=dx_dtype, dw_dtype=dw_dtype,
+                    scale=scale if scale is not None else 1.0 / max(rows, 1))
+    rt._check(call(d))
+    if w16 is not None:
+        rt.recycle(w16)
+    return (losses, dx, dw) if grads else (losses, None, None)
+
+
+def linear_cross_entropy(rt: GpuRuntime, x, w, targets, rows: int, dim: int, vocab: int, *, scale: Optional[float] = None, row_weights=None,
+                         grads: bool = True, trans_w: bool = False, x_dtype: int = OUT_F32, w_dtype: int = OUT_F32, dx_dtype: int = OUT_F32,
+                         dw_dtype: int = OUT_F32, ldx: Optional[int] = None, ldw: Optional[int] = None, weight_id: Optional[int] = None,
+                         losses=None, lse=None, dx=None, dw=None, piece_rows: int = 0, scratch: Optional[GpuBuffer] = None):
+    """`matmul` with the head followed by `cross_entropy`, and both their backwards, without the [rows, vocab] logits: x
+    [rows, dim], w [dim, vocab] (`trans_w`: [vocab, dim]), targets u32[rows] (`NO_WORD`: the row is left out).  Returns
+    (losses f32[rows], dx, dw) with the gradients of scale * sum(row_weights * losses) (default scale 1 / rows), or
+    (losses, None, None) without `grads`.  As in `matmul`, f32 operands are multiplied as bf16 (an f32 head is converted in
+    every call, or once through the runtime's cached copy under `weight_id`) and gradients are f32 unless asked otherwise.  Buffers are
+    `GpuBuffer`s or device addresses; outputs that are not given come from the pool; `lse` (f32[rows], optional) receives
+    log-sum-exp.  Only queues work; inside a captured graph pass `scratch` (`linear_loss_scratch_bytes`)."""
+    return _linear_loss(rt, lambda d: lib().t0b_linear_ce(rt.handle, C.byref(d), _addr(targets), 1), x, w, rows, dim, vocab, 0, scale,
+                        row_weights, grads, trans_w, x_dtype, w_dtype, dx_dtype, dw_dtype, ldx, ldw, weight_id, losses, lse, dx, dw, piece_rows,
+                        scratch)
+
+
+def linear_topk_distill(rt: GpuRuntime, x, w, ids, teacher, rows: int, dim: int, vocab: int, topk: int, *, temperature: float = 1.0,
+                        ldk: Optional[int] = None, scale: Optional[float] = None, row_weights=None, grads: bool = True, trans_w: bool = False,
+                        x_dtype: int = OUT_F32, w_dtype: int = OUT_F32, dx_dtype: int = OUT_F32, dw_dtype: int = OUT_F32,
+                        ldx: Optional[int] = None, ldw: Optional[int] = None, weight_id: Optional[int] = None, losses=None, lse=None, dx=None,
+                        dw=None, piece_rows: int = 0, scratch: Optional[GpuBuffer] = None):
+    """`topk_distill` on the logits x * head, without the logits; arguments and results as for `linear_cross_entropy`."""
+    return _linear_loss(rt, lambda d: lib().t0b_linear_topk_distill(rt.handle, C.byref(d), _addr(ids), _addr(teacher), topk,
+                                                                    ldk if ldk is not None else topk, temperature, 1),
+                        x, w, rows, dim, vocab, topk, scale, row_weights, grads, trans_w, x_dtype, w_dtype, dx_dtype, dw_dtype, ldx, ldw,
+                        weight_id, losses, lse, dx, dw, piece_rows, scratch)
+
+
+def linear_loss_scratch_bytes(rt: GpuRuntime, rows: int, dim: int, vocab: int, *, topk: int = 0, grads: bool = True, trans_w: bool = False,
+                              x_dtype: int = OUT_F32, dx_dtype: int = OUT_F32, dw_dtype: int = OUT_F32, piece_rows: int = 0) -> int:
+    """Bytes of a `scratch` that holds any call of these sizes, whatever the alignment and pitch of x and w."""
+    w_cols = dim if trans_w else vocab
+    d = LinearLossC(x=2 if x_dtype == OUT_BF16 else 4, w=2, ldx=dim, ldw=w_cols, losses=4, dx=256 if grads else 0, dw=256 if grads else 0, lddx=dim,
+                    lddw=w_cols, rows=rows, dim=dim, vocab=vocab, trans_w=int(trans_w), piece_rows=piece_rows, x_dtype=x_dtype,
+                    dx_dtype=dx_dtype, dw_dtype=dw_dtype, scale=1.0)
+    return lib().t0b_linear_loss_scratch_bytes(rt.handle, C.byref(d), topk)
 
 
 def embedding_forward(rt: GpuRuntime, table: GpuBuffer, ids: GpuBuffer, seq_len: int, dim: int, vocab_size: int):

@@ -1,0 +1,326 @@
+"""Vocabulary losses (cross entropy and distillation from hidden states or logits) against their definitions in 64 bits.
+
+Bounds.  u32 = 2^-23 covers one f32 operation of the tensor cores or of ex2.approx (rounded or truncated), u_b = 2^-8 and
+u_h = 2^-11 a rounding to bf16 and fp16.  A logit is a sum of `dim` exact products: |dz| <= dim u32 sum|x w| =: ez.  A
+probability is exp of a difference of such logits times 1 / T, divided by a sum of such: relative error
+  ep = 2 ez / T + (max z - z) / T * 4 u32 + 8 u32,
+and a loss, a sum of differences of logarithms, is off by at most 2 ez / T + (|z - max z| / T + 16) 8 u32.  The gradient of a
+logit, a (p - q), is stored in bf16 after exp went through fp16 (absolute 2^-25 of the part's largest below fp16's normal
+range); dx and dw are sums of those times bf16 operands, plus their f32 summation and the rounding of the result."""
+import math
+
+import numpy as np
+import pytest
+
+import t0_gpu_b200 as t
+from t0_gpu_b200 import OUT_BF16, OUT_F32, T0Error, ops
+
+pytestmark = pytest.mark.gpu
+
+U32, UB, UH = 2.0 ** -23, 2.0 ** -8, 2.0 ** -11
+
+
+@pytest.fixture(scope="module")
+def th():
+    import torch
+
+    return torch
+
+
+@pytest.fixture(scope="module")
+def art(th):
+    """A runtime on a torch stream, so that tensors made by torch are ordered with its launches."""
+    r = t.GpuRuntime()
+    s = th.cuda.Stream()
+    with th.cuda.stream(s):
+        r.set_stream(s.cuda_stream)
+        yield r
+        r.synchronize()
+    r.close()
+
+
+def make_teacher(th, rows, topk, vocab, seed, ragged):
+    g = np.random.default_rng(seed)
+    ids = np.stack([g.choice(vocab, size=min(topk, vocab), replace=False) for _ in range(rows)]).astype(np.int64)
+    if topk > vocab:
+        ids = np.concatenate([ids, np.full((rows, topk - vocab), -1)], 1)
+    logits = g.normal(size=(rows, topk)) * 3
+    if ragged:
+        for r in range(rows):
+            have = r % (topk + 1)
+            ids[r, have:] = -1
+            logits[r, have:] = [np.nan, np.inf, -np.inf][r % 3]
+    return th.tensor(ids.astype(np.int32), device="cuda"), th.tensor(logits.astype(np.float32), device="cuda")
+
+
+def target_rows(th, ids, teacher, temperature, vocab):
+    """q [rows, vocab], sum over words of q log q, live rows -- all in 64 bits."""
+    ids = ids.long()
+    have = (ids >= 0) & (ids < vocab) & ~(th.isneginf(teacher) & (ids >= 0))
+    lq = (teacher.double() / temperature).masked_fill(~have, -math.inf)
+    live = have.any(1)
+    lq = th.where(live[:, None], lq - th.logsumexp(lq, 1, keepdim=True), lq)
+    q = th.zeros((ids.shape[0], vocab), dtype=th.float64, device="cuda")
+    pk = lq.exp()
+    q.scatter_add_(1, ids.clamp(0, vocab - 1), pk.masked_fill(~have, 0.0))
+    ent = (pk * lq.masked_fill(~have, 0.0)).masked_fill(~have, 0.0).sum(1)
+    return q, ent, live
+
+
+def losses_and_dz(th, z, q, ent, live, temperature, row_scale):
+    z = z / temperature
+    top = z.amax(1, keepdim=True)
+    some = live & ~th.isneginf(top[:, 0])
+    top = top.masked_fill(~some[:, None], 0.0)
+    log_s = (z - top).exp().sum(1, keepdim=True).log()
+    lp = (z - top) - log_s                      # not z - logsumexp: beside z = -3e38 that would lose log_s, in 64 bits too
+    lse = top + log_s
+    losses = ent - (q * lp.masked_fill(q == 0, 0.0)).sum(1)
+    p = lp.exp().masked_fill(~some[:, None], 0.0)
+    dz = (p * q.sum(1, keepdim=True) - q) * (row_scale / temperature)[:, None]
+    losses, dz = losses.masked_fill(~some, 0.0), dz.masked_fill(~some[:, None], 0.0)
+    return losses, dz, p, lse[:, 0]
+
+
+def check_linear(th, art, rows, dim, vocab, trans_w, *, topk=0, temperature=1.0, grads=True, x_dtype=OUT_BF16, gdt=OUT_BF16, weights=True, ignore=True,
+                 piece_rows=0, ldx_pad=0, ldw_pad=0, ragged=True, big=1.0, offset=0):
+    g = th.Generator(device="cuda")
+    g.manual_seed(rows * 7919 + dim * 31 + vocab)
+    w_rows, w_cols = (vocab, dim) if trans_w else (dim, vocab)
+    wbuf = (th.randn((w_rows * (w_cols + ldw_pad) + offset,), device="cuda", generator=g) / math.sqrt(dim)).bfloat16()
+    w = wbuf[offset:].view(w_rows, w_cols + ldw_pad)[:, :w_cols]
+    wd = (w if trans_w else w.t()).double()                                     # [vocab, dim]
+    xt = th.bfloat16 if x_dtype == OUT_BF16 else th.float32
+    x = (th.randn((rows, dim + ldx_pad), device="cuda", generator=g) * 2 * big).to(xt)[:, :dim]
+    ldx, ldw = dim + ldx_pad, w_cols + ldw_pad
+    if topk:
+        ids, teacher = make_teacher(th, rows, topk, vocab, rows + topk, ragged)
+        q, ent, live = target_rows(th, ids, teacher, temperature, vocab)
+    else:
+        tgt = th.randint(0, vocab, (rows,), device="cuda", generator=g)
+        x = x.clone() if not ldx_pad else x
+        if ignore:
+            tgt[::3] = -1
+        live = tgt >= 0
+        q = th.zeros((rows, vocab), dtype=th.float64, device="cuda")
+        q[th.arange(rows, device="cuda"), tgt.clamp_min(0)] = live.double()
+        ent = th.zeros(rows, dtype=th.float64, device="cuda")
+        tgt = tgt.to(th.int32)
+    if ignore and grads:
+        x[~live] = math.nan                                                     # a row that is left out may hold anything
+    rw = th.rand(rows, device="cuda", generator=g) * 2 if weights else None
+    scale = 1.0 / rows
+    row_scale = (rw.double() if weights else th.ones(rows, device="cuda", dtype=th.float64)) * scale
+    xd = x.bfloat16().double().masked_fill(~live[:, None], 0.0) if (ignore and grads) else x.bfloat16().double()
+    z = xd @ wd.t()
+    losses_ref, dz, p, lse_ref = losses_and_dz(th, z, q, ent, live, temperature, row_scale)
+    losses, lse = th.full((rows,), 7.0, device="cuda"), th.full((rows,), 7.0, device="cuda")
+    odt = th.bfloat16 if gdt == OUT_BF16 else th.float32
+    dx = th.full((rows + 1, dim), 7.0, device="cuda", dtype=odt)
+    dw = th.full((w_rows + 1, w_cols), 7.0, device="cuda", dtype=odt)
+    kw = dict(grads=grads, trans_w=trans_w, x_dtype=x_dtype, w_dtype=OUT_BF16, dx_dtype=gdt, dw_dtype=gdt, ldx=ldx, ldw=ldw, losses=losses.data_ptr(),
+              lse=lse.data_ptr(), dx=dx.data_ptr() if grads else None, dw=dw.data_ptr() if grads else None, piece_rows=piece_rows,
+              row_weights=rw.data_ptr() if weights else None)
+    if topk:
+        ops.linear_topk_distill(art, x.data_ptr(), w.data_ptr(), ids.data_ptr(), teacher.data_ptr(), rows, dim, vocab, topk, temperature=temperature, **kw)
+    else:
+        ops.linear_cross_entropy(art, x.data_ptr(), w.data_ptr(), tgt.data_ptr(), rows, dim, vocab, **kw)
+    art.synchronize()
+    xa, wa = xd.abs(), wd.abs()
+    ez = (dim * U32) * (xa @ wa.t()).amax(1) / temperature                       # per row
+    down = (z.amax(1, keepdim=True) - z) / temperature
+    reach = (down * (q > 0)).amax(1)
+    tol = 2 * ez + (reach + 16 + lse_ref.abs()) * 8 * U32
+    assert ((losses.double() - losses_ref).abs() <= tol).all(), ((losses.double() - losses_ref).abs() / tol).max()
+    assert (losses[~live] == 0).all()
+    assert ((lse.double() - lse_ref)[live].abs() <= tol[live]).all() and (lse[~live] == 0).all()
+    if not grads:
+        assert (dx == 7).all() and (dw == 7).all()
+        return
+    a = (row_scale / temperature).abs()[:, None] * live[:, None]
+    ep = 2 * ez[:, None] + down * 4 * U32 + 8 * U32
+    edz = UB * dz.abs() + a * (p * (ep + UH + UB * UH) + 2.0 ** -24 * p.amax(1, keepdim=True))
+    full = dz.abs() + edz
+    uo = UB if gdt == OUT_BF16 else U32
+    dx_ref, edx = dz @ wd, edz @ wa + vocab * U32 * (full @ wa)
+    bound = edx + uo * (dx_ref.abs() + edx) + 1e-30
+    err = (dx[:rows].double() - dx_ref).abs()
+    assert (err <= bound).all(), (err / bound).max()
+    dw_ref, edw = dz.t() @ xd, edz.t() @ xa + rows * U32 * (full.t() @ xa)
+    bound = edw + uo * (dw_ref.abs() + edw) + 1e-30
+    got = dw[:w_rows].double() if trans_w else dw[:w_rows].double().t()
+    err = (got - dw_ref).abs()
+    assert (err <= bound).all(), (err / bound).max()
+    assert (dx[rows] == 7).all() and (dw[w_rows] == 7).all()                     # nothing behind the last row
+    assert (dx[:rows][~live] == 0).all()
+
+
+LINEAR_SIZES = [(1, 64, 64), (1, 8, 1), (3, 40, 17), (33, 64, 129), (128, 128, 1000), (130, 200, 513), (257, 96, 2048), (300, 1000, 777), (64, 72, 5001)]
+
+
+@pytest.mark.parametrize("trans_w", [False, True])
+@pytest.mark.parametrize("rows,dim,vocab", LINEAR_SIZES)
+def test_linear_ce(th, art, rows, dim, vocab, trans_w):
+    check_linear(th, art, rows, dim, vocab, trans_w)
+
+
+@pytest.mark.parametrize("trans_w", [False, True])
+@pytest.mark.parametrize("rows,dim,vocab,topk", [(1, 64, 64, 1), (2, 8, 5, 9), (33, 64, 129, 4), (130, 200, 513, 33), (257, 96, 2048, 100), (40, 64, 3001, 1024)])
+def test_linear_topk_distill(th, art, rows, dim, vocab, topk, trans_w):
+    check_linear(th, art, rows, dim, vocab, trans_w, topk=topk, temperature=2.0)
+
+
+@pytest.mark.parametrize("topk", [0, 5])
+@pytest.mark.parametrize("trans_w", [False, True])
+@pytest.mark.parametrize("rows,dim,vocab", [(1, 64, 64), (70, 100, 999), (300, 256, 4000)])
+def test_linear_losses_alone(th, art, rows, dim, vocab, trans_w, topk):
+    check_linear(th, art, rows, dim, vocab, trans_w, topk=topk, grads=False, ignore=False)
+
+
+@pytest.mark.parametrize("trans_w", [False, True])
+@pytest.mark.parametrize("x_dtype,gdt", [(OUT_F32, OUT_F32), (OUT_F32, OUT_BF16), (OUT_BF16, OUT_F32)])
+def test_linear_types(th, art, x_dtype, gdt, trans_w):
+    check_linear(th, art, 65, 136, 777, trans_w, x_dtype=x_dtype, gdt=gdt)
+    check_linear(th, art, 65, 136, 776, trans_w, x_dtype=x_dtype, gdt=gdt, topk=7)
+
+
+@pytest.mark.parametrize("trans_w", [False, True])
+@pytest.mark.parametrize("gdt", [OUT_F32, OUT_BF16])
+@pytest.mark.parametrize("vocab", [640, 601])
+def test_linear_in_pieces_of_rows(th, art, vocab, gdt, trans_w):
+    check_linear(th, art, 300, 128, vocab, trans_w, gdt=gdt, piece_rows=128)
+    check_linear(th, art, 100, 60, vocab, trans_w, gdt=gdt, piece_rows=33, topk=6)
+
+
+@pytest.mark.parametrize("trans_w", [False, True])
+def test_linear_pitches_and_offsets(th, art, trans_w):
+    check_linear(th, art, 50, 64, 320, trans_w, ldx_pad=8, ldw_pad=16)
+    check_linear(th, art, 50, 64, 320, trans_w, ldx_pad=3, ldw_pad=5)
+    check_linear(th, art, 50, 64, 320, trans_w, offset=1)
+    check_linear(th, art, 50, 64, 320, trans_w, grads=False, ignore=False, ldx_pad=1, offset=3)
+
+
+@pytest.mark.parametrize("trans_w", [False, True])
+def test_linear_large_logits(th, art, trans_w):
+    check_linear(th, art, 100, 64, 700, trans_w, big=40.0)
+
+
+# ------------------------------------------------------------------------------------------------ on given logits
+
+def check_logits(th, art, rows, cols, topk, *, dtype=OUT_F32, gdt=None, temperature=1.0, pad=0, offset=0, ragged=True, mask=0, in_place=False, weights=True,
+                 grads=True, ids=None, teacher=None, edit=None):
+    gdt = dtype if gdt is None else gdt
+    dt, odt = (th.bfloat16 if k == OUT_BF16 else th.float32 for k in (dtype, gdt))
+    g = th.Generator(device="cuda")
+    g.manual_seed(rows * 7919 + cols * 31 + topk)
+    ld = cols + pad
+    buf = (th.randn((rows * ld + offset + 64,), device="cuda", generator=g) * 4).to(dt)
+    view = buf[offset:offset + rows * ld].view(rows, ld)
+    if ids is None:
+        ids, teacher = make_teacher(th, rows, topk, cols, rows + topk, ragged)
+    if mask:
+        view[:, cols - mask:cols] = -math.inf
+    if edit:
+        edit(view)
+    q, ent, live = target_rows(th, ids, teacher, temperature, cols)
+    view[~live, :cols] = math.nan if rows % 2 else math.inf                      # rows that are left out may hold anything
+    z = view[:, :cols].double().masked_fill(~live[:, None], 0.0)
+    before = buf.clone()
+    rw = th.rand(rows, device="cuda", generator=g) * 2 if weights else None
+    row_scale = (rw.double() if weights else th.ones(rows, device="cuda", dtype=th.float64)) / rows
+    losses_ref, dz, p, lse = losses_and_dz(th, z, q, ent, live, temperature, row_scale)
+    losses = th.full((rows + 1,), 7.0, device="cuda")
+    out = buf if in_place else th.full((rows * ld + offset + 64,), 7.0, device="cuda", dtype=odt)
+    kept = out.clone()
+    dview = out[offset:offset + rows * ld].view(rows, ld)
+    ops.topk_distill(art, view.data_ptr(), ids.data_ptr(), teacher.data_ptr(), rows, cols, topk, temperature=temperature, logits_dtype=dtype, grad_dtype=gdt,
+                     ld=ld, losses=losses.data_ptr(), dlogits=dview.data_ptr() if grads else None, grads=grads, row_weights=rw.data_ptr() if weights else None)
+    art.synchronize()
+    zmax = z.amax(1, keepdim=True)
+    down = ((zmax - z) / temperature).nan_to_num(0.0, 0.0, 0.0)
+    reach = (down * (q > 0)).amax(1)
+    tol = (reach + 16 + ent.abs()) * 8 * U32
+    got = losses[:rows].double()
+    masked = th.isinf(losses_ref)                                                # a target is masked
+    assert (got[masked] == losses_ref[masked]).all()
+    # A loss within its bound of the largest f32 may round to infinity.
+    fin = ~masked & ~((losses_ref + tol > th.finfo(th.float32).max) & th.isposinf(got))
+    assert ((got - losses_ref).abs()[fin] <= tol[fin]).all(), ((got - losses_ref).abs() / tol)[fin].max()
+    assert losses[rows] == 7
+    if not in_place:
+        assert th.equal(buf.view(th.int16 if dtype == OUT_BF16 else th.int32), before.view(th.int16 if dtype == OUT_BF16 else th.int32))
+    if not grads:
+        assert (out == 7).all()
+        return
+    a = (row_scale / temperature).abs()[:, None] * live[:, None]
+    uo = UB if gdt == OUT_BF16 else U32
+    bound = uo * dz.abs() + a * (p * (down * 4 + 16) + q * (8 + 4 * ent.abs()[:, None])) * U32 * 2 + 1e-37
+    err = (dview[:, :cols].double() - dz).abs()
+    assert (err <= bound).all(), (err / bound).max()
+    assert (dview[:, :cols][~live] == 0).all()
+    if pad:
+        assert th.equal(dview[:, cols:].float().nan_to_num(1e9), kept[offset:offset + rows * ld].view(rows, ld)[:, cols:].float().nan_to_num(1e9))
+    assert th.equal(out[offset + rows * ld:], kept[offset + rows * ld:]) and th.equal(out[:offset], kept[:offset])
+
+
+LOGIT_SIZES = [(1, 1, 1), (1, 7, 3), (5, 33, 4), (3, 1000, 20), (40, 4097, 8), (300, 2050, 16), (2, 32000, 64), (5, 50257, 9), (150, 13000, 5), (3, 150001, 1024)]
+
+
+@pytest.mark.parametrize("dtype", [OUT_F32, OUT_BF16])
+@pytest.mark.parametrize("rows,cols,topk", LOGIT_SIZES)
+def test_topk_distill(th, art, rows, cols, topk, dtype):
+    check_logits(th, art, rows, cols, topk, dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype,gdt", [(OUT_F32, OUT_BF16), (OUT_BF16, OUT_F32)])
+def test_topk_distill_mixed_types(th, art, dtype, gdt):
+    check_logits(th, art, 9, 1001, 6, dtype=dtype, gdt=gdt)
+    check_logits(th, art, 9, 1024, 6, dtype=dtype, gdt=gdt, temperature=3.0)
+
+
+@pytest.mark.parametrize("dtype", [OUT_F32, OUT_BF16])
+@pytest.mark.parametrize("pad,offset", [(0, 0), (5, 0), (8, 1), (3, 3)])
+def test_topk_distill_pitches_offsets_masks_in_place(th, art, dtype, pad, offset):
+    for in_place in (False, True):
+        check_logits(th, art, 7, 2000, 6, dtype=dtype, pad=pad, offset=offset, in_place=in_place, mask=9 if pad else 0, temperature=1.5)
+    check_logits(th, art, 7, 2000, 6, dtype=dtype, pad=pad, offset=offset, grads=False)
+
+
+@pytest.mark.parametrize("dtype", [OUT_F32, OUT_BF16])
+def test_topk_distill_long_rows_are_read_twice(th, art, dtype):
+    cols = 450_000 if dtype == OUT_F32 else 900_001
+    check_logits(th, art, 3, cols, 5, dtype=dtype)
+    check_logits(th, art, 2, cols, 5, dtype=dtype, in_place=True)
+
+
+def test_topk_distill_values_at_the_edge(th, art):
+    """Logits at the type's lowest value, a row of nothing but it, rows of -inf alone, huge differences."""
+    lowest = th.finfo(th.float32).min
+
+    def edit(z):
+        z[0] = lowest
+        z[1, 1:] = lowest
+        z[2] = -math.inf
+        z[3, ::2] = -math.inf
+        z[4, 5] = 3e38
+
+    check_logits(th, art, 6, 500, 3, ragged=False, edit=edit)
+
+
+def test_topk_distill_same_word_twice(th, art):
+    ids = th.tensor([[3, 3, 9, 3], [0, 0, 0, 0], [5, -1, 5, 6]], device="cuda", dtype=th.int32)
+    teacher = th.tensor([[1.0, 0.5, 2.0, -1.0], [1.0, 1.0, 1.0, 1.0], [0.0, math.nan, 2.0, 1.0]], device="cuda")
+    check_logits(th, art, 3, 40, 4, ids=ids, teacher=teacher)
+    rows, dim, vocab = 3, 16, 40
+    x = th.randn((rows, dim), device="cuda").bfloat16()
+    w = th.randn((vocab, dim), device="cuda").bfloat16()
+    z = (x.double() @ w.double().t())
+    q, ent, live = target_rows(th, ids, teacher, 1.0, vocab)
+    losses_ref, dz, p, _ = losses_and_dz(th, z, q, ent, live, 1.0, th.full((rows,), 1.0 / rows, device="cuda", dtype=th.float64))
+    losses, dx = th.empty(rows, device="cuda"), th.empty((rows, dim), device="cuda")
+    ops.linear_topk_distill(art, x.data_ptr(), w.data_ptr(), ids.data_ptr(), teacher.data_ptr(), rows, dim, vocab, 4, trans_w=True, x_dtype=OUT_BF16,
+                            w_dtype=OUT_BF16, losses=losses.data_ptr(), dx=dx.data_ptr())
+    art.synchronize()
+    assert ((losses.double() - losses_ref).abs() <= 1e-4).all()      # |z| < 40: 2 ez = 2 * 16 * 2^-23 * 16 * 16 < 1e-3 / 10
+    edz = UB * dz.abs() + p * (UH + 1e-4) / rows + 1e-8
+    assert ((dx.double() - dz @ w.double()).abs() <= edz @ w.double().abs() + 1e-5).all()
