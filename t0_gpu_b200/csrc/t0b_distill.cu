@@ -3,11 +3,19 @@
 //   p = softmax over the vocabulary of z_v / T                          (the student)
 //   loss = sum_k q_k (log q_k - log p_{id_k})                           (Kullback-Leibler divergence)
 //   d loss / d z_v = (p_v - sum_{k: id_k = v} q_k) / T
-// Loss and gradient come from one read of the logits.  A row is shared by a thread-block cluster of 1 to 8 CTAs; each keeps
-// its slice of the row in shared memory while it gathers the running maximum and sum, the CTAs exchange those two numbers
-// over distributed shared memory, and the gradient is written from the cached slice.  HBM traffic: one read of z, one
-// write of dz.  All statistics are f32.
+// Loss and gradient come from one pass over HBM, which bounds the kernels: one read of z, one write of dz.  Three forms:
+//   rows in registers  a cluster of 1 to 8 CTAs per row; every thread keeps up to sixteen 16-byte groups, all loaded before
+//                      the first is used: maximum; exponentials, which replace the logits, and their sum; -- the CTAs
+//                      exchange (maximum, sum) over distributed shared memory -- gradient = exponential times one factor
+//   streamed rows      long rows, enough of them for every SM: one CTA per row, which L2 serves the second time
+//   any rows           pointers off their 16-byte boundaries
+// Rows in registers keep the exponentials of bf16 logits in 16 bits as fp16, relative to their CTA's maximum (11 significant
+// bits down to 2^-14 of it, at most 2^-25 of it off below), where the gradient is bf16 as well; for an f32 gradient they are
+// computed again instead.  Statistics, losses and the gradient at the teacher's words are f32 throughout.
+
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_pipeline.h>
 
 #include <algorithm>
 #include <atomic>
@@ -20,11 +28,9 @@ using namespace t0b;
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+constexpr int kThreads = 256;         // rows in registers, and the general form
 constexpr uint32_t kNoWord = 0xffffffffu;
 constexpr int kMaxCluster = 8;
-constexpr size_t kCacheMax = 200 * 1024;   // per CTA; a longer slice is read twice instead
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -41,34 +47,50 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Block-wide sum / maximum; every thread receives it.  `red` holds kWarps floats.
-__device__ __forceinline__ float block_sum(float v, float* red) {
-    v = warp_sum(v);
+// Block-wide maxima / sums of two values at once; every thread receives them.  `red` is used by one call only.
+template <int T>
+__device__ __forceinline__ void block_max2(float& a, float& b, float2* red) {
+    a = warp_max(a);
+    b = warp_max(b);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_float2(a, b);
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float t = 0.0f;
+    a = red[0].x;
+    b = red[0].y;
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) t += red[i];
-    return t;
+    for (int i = 1; i < T / 32; ++i) {
+        a = fmaxf(a, red[i].x);
+        b = fmaxf(b, red[i].y);
+    }
 }
-__device__ __forceinline__ float block_max(float v, float* red) {
-    v = warp_max(v);
+template <int T>
+__device__ __forceinline__ void block_sum2(float& a, float& b, float2* red) {
+    a = warp_sum(a);
+    b = warp_sum(b);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_float2(a, b);
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float t = red[0];
+    a = b = 0.0f;
 #pragma unroll
-    for (int i = 1; i < kWarps; ++i) t = fmaxf(t, red[i]);
-    return t;
+    for (int i = 0; i < T / 32; ++i) {
+        a += red[i].x;
+        b += red[i].y;
+    }
 }
-// (m, s) <- the statistics of both halves: s = sum of 2^((z - m) c).  A half without any z above -inf has m = -inf, s = 0.
-__device__ __forceinline__ void join_stats(float& m, float& s, float m2, float s2, float c) {
-    const float mm = fmaxf(m, m2);
-    const float ref = mm == -INFINITY ? 0.0f : mm;
-    s = s * exp2_approx((m - ref) * c) + s2 * exp2_approx((m2 - ref) * c);
-    m = mm;
-}
+
+// exp(z / T) relative to the largest z of a set, as 2^(z c - mc) with c = log2(e) / T and mc = m c rounded: one fused
+// multiply-add whose only rounding is that of the small difference, and references that subtract exactly from one another.
+// Where m c leaves f32's range (logits at the type's lowest value) the difference is taken first.
+struct Ref {
+    float m, mc;
+    bool fused;
+    __device__ __forceinline__ Ref(float m_, float c) : m(m_), mc(m_ * c), fused(fabsf(m_ * c) < 1e37f) {
+        if (m_ == -INFINITY) { m = mc = 0.0f; fused = true; }   // nothing in the set: exponentials 0, not exp(-inf + inf)
+    }
+    __device__ __forceinline__ float arg(float z, float c) const { return fused ? fmaf(z, c, -mc) : (z - m) * c; }
+    // (z - m) / T, as the exponent's counterpart in the loss.
+    __device__ __forceinline__ float log_of(float z, float c, float inv_t) const { return fused ? 0.6931471805599453f * fmaf(z, c, -mc) : (z - m) * inv_t; }
+    // What an exponential relative to this reference is worth relative to `other` (>= this one).
+    __device__ __forceinline__ float to(const Ref& other, float c) const { return exp2_approx(fused && other.fused ? mc - other.mc : (m - other.m) * c); }
+};
 
 // 16 bytes of logits as floats.
 template <typename T> struct Vec;
@@ -130,212 +152,510 @@ struct DistillParams {
     unsigned long long ld, ldk;
     float c, inv_t;          // log2(e) / T and 1 / T
     float scale;             // of the gradient, 1 / T included
-    uint32_t groups_per_cta; // 16-byte groups of one CTA's slice
-    int in_vec, out_vec;     // base pointers allow whole-group accesses
+    uint32_t groups_per_cta; // 16-byte groups of one CTA's slice (rows in registers)
     int* status;
 };
 
-template <typename IN, typename OUT, bool CACHE>
-__global__ void __launch_bounds__(kThreads) topk_distill_kernel(const DistillParams p) {
-    constexpr int N = Vec<IN>::kN;
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float red[kWarps];
-    __shared__ float2 red2[kWarps];
-    __shared__ __align__(16) float2 xch[kMaxCluster];
-    uint4* cache = reinterpret_cast<uint4*>(smem);
-    uint32_t* ids = reinterpret_cast<uint32_t*>(smem + (CACHE ? static_cast<size_t>(p.groups_per_cta) * 16 : 0));
-    float* q = reinterpret_cast<float*>(ids + p.topk);
-    uint32_t nranks, rank;
-    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(nranks));
-    rank = ptx::cluster_ctarank();
-    const uint32_t row = blockIdx.x / nranks;
-    const int tid = threadIdx.x;
-    ptx::cluster_arrive();   // every CTA of the cluster has started once the matching wait returns
-
-    // The teacher's distribution; every CTA of the cluster computes all of it (at most 1024 words).
-    float tmax = -INFINITY;
-    for (uint32_t k = tid; k < p.topk; k += kThreads) {
-        uint32_t id = p.ids[row * p.ldk + k];
-        if (id != kNoWord && id >= p.cols) {
-            if (rank == 0) *reinterpret_cast<volatile int*>(p.status) = kDevBadIndex;   // the word is left out
-            id = kNoWord;
-        }
-        const float t = id == kNoWord ? -INFINITY : p.teacher[row * p.ldk + k];
-        ids[k] = id;
-        q[k] = t;
-        tmax = fmaxf(tmax, t);
-    }
-    tmax = block_max(tmax, red);
-    const float tref = tmax == -INFINITY ? 0.0f : tmax;
-    float tsum = 0.0f;
-    for (uint32_t k = tid; k < p.topk; k += kThreads) tsum += ids[k] == kNoWord ? 0.0f : expf((q[k] - tref) * p.inv_t);
-    tsum = block_sum(tsum, red);
-    const float tlog = logf(tsum);
-    bool live = tsum > 0.0f || tsum != tsum;
-    const IN* zr = static_cast<const IN*>(p.logits) + row * p.ld;
-    float cross = 0.0f;   // rank 0: sum of q (log q - z / T) over this thread's words, z relative to the row's maximum later
-    float qsum = 0.0f;
-    const bool want_loss = rank == 0 && p.losses;
-    constexpr int kOwn = 1024 / kThreads;   // words per thread at most
-    float z_own[kOwn];
+// v <- 2^(v c - mc), the exponentials relative to `r`.
+template <int N>
+__device__ __forceinline__ void exp_group(float (&v)[N], const Ref& r, float c) {
+    if (r.fused) {
 #pragma unroll
-    for (int i = 0; i < kOwn; ++i) {
-        const uint32_t k = tid + i * kThreads;
-        z_own[i] = 0.0f;
-        if (live && k < p.topk) {
-            const float lq = (q[k] - tref) * p.inv_t - tlog;
-            const float qk = ids[k] == kNoWord ? 0.0f : expf(lq);
-            if (ids[k] != kNoWord) z_own[i] = to_float(zr[ids[k]]);   // before anything is written: dlogits may be the logits
-            if (qk != 0.0f) cross += qk * lq;
-            q[k] = qk;
-        }
-    }
-
-    // This CTA's slice in 16-byte groups, counted from the 16-byte boundary at or before the row.
-    const unsigned long long e0 = row * p.ld;
-    const unsigned long long g0 = e0 / N;
-    const uint32_t ngroups = static_cast<uint32_t>((e0 + p.cols - 1) / N - g0 + 1);
-    const uint32_t lo = min(rank * p.groups_per_cta, ngroups), hi = min(lo + p.groups_per_cta, ngroups);
-    const IN* zg = static_cast<const IN*>(p.logits) + g0 * N;
-    const int lead = static_cast<int>(e0 - g0 * N);   // elements of group 0 that belong to the row before
-    // Group g holds columns g * N - lead ...; read it whole, or element by element at the row's ends.
-    auto load_group = [&](uint32_t g) -> uint4 {
-        const long long col = static_cast<long long>(g) * N - lead;
-        if (p.in_vec && col >= 0 && col + N <= p.cols) return __ldcs(reinterpret_cast<const uint4*>(zg) + g);
-        float v[N];
+        for (int e = 0; e < N; ++e) v[e] = exp2_approx(fmaf(v[e], c, -r.mc));
+    } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = (col + i >= 0 && col + i < p.cols) ? to_float(zr[col + i]) : -INFINITY;
-        return Vec<IN>::pack(v);
-    };
-    float m = -INFINITY, s = 0.0f;
-    if (live) {
-        constexpr int U = 4;   // loads in flight per thread
-        for (uint32_t g = lo + tid; g < hi; g += U * kThreads) {
-            uint4 raw[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (g + u * kThreads < hi) raw[u] = load_group(g + u * kThreads);
-            float lm = m;
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (g + u * kThreads < hi) {
-                    if (CACHE) cache[g + u * kThreads - lo] = raw[u];
-                    float v[N];
-                    Vec<IN>::unpack(raw[u], v);
-#pragma unroll
-                    for (int i = 0; i < N; ++i) lm = fmaxf(lm, v[i]);
-                }
-            const float ref = lm == -INFINITY ? 0.0f : lm;
-            if (lm > m) s *= exp2_approx((m - ref) * p.c);
-            m = lm;
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (g + u * kThreads < hi) {
-                    float v[N];
-                    Vec<IN>::unpack(raw[u], v);
-#pragma unroll
-                    for (int i = 0; i < N; ++i) s += exp2_approx((v[i] - ref) * p.c);
-                }
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-            join_stats(m, s, m2, s2, p.c);
-        }
-        if ((tid & 31) == 0) red2[tid >> 5] = make_float2(m, s);
-        __syncthreads();
-        m = red2[0].x;
-        s = red2[0].y;
-#pragma unroll
-        for (int i = 1; i < kWarps; ++i) join_stats(m, s, red2[i].x, red2[i].y, p.c);
-    }
-    // Exchange over the cluster: every CTA gets every (m, s) and joins them in rank order, so all hold the same bits.
-    ptx::cluster_wait();
-    if (tid < static_cast<int>(nranks)) {
-        const uint32_t dst = ptx::mapa(ptx::smem_u32(&xch[rank]), static_cast<uint32_t>(tid));
-        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(dst), "f"(m), "f"(s) : "memory");
-    }
-    ptx::cluster_arrive();
-    ptx::cluster_wait();
-    m = xch[0].x;
-    s = xch[0].y;
-    for (uint32_t r = 1; r < nranks; ++r) join_stats(m, s, xch[r].x, xch[r].y, p.c);
-    if (m == -INFINITY && s == 0.0f) live = false;   // every logit is -inf: the row has no distribution
-
-    if (want_loss) {
-        const float lse = logf(s);
-#pragma unroll
-        for (int i = 0; i < kOwn; ++i) {
-            const uint32_t k = tid + i * kThreads;
-            if (live && k < p.topk && q[k] != 0.0f) {
-                cross -= q[k] * ((z_own[i] - m) * p.inv_t);
-                qsum += q[k];
-            }
-        }
-        cross = block_sum(cross, red);
-        qsum = block_sum(qsum, red);
-        if (tid == 0) p.losses[row] = live ? cross + qsum * lse : 0.0f;
-    }
-    if (!p.dlogits) return;
-    OUT* dr = static_cast<OUT*>(p.dlogits) + e0;
-    OUT* dg = static_cast<OUT*>(p.dlogits) + g0 * N;
-    const float a = live ? p.scale * (p.weights ? p.weights[row] : 1.0f) : 0.0f;
-    const float inv = a / s;
-    for (uint32_t g = lo + tid; g < hi; g += kThreads) {
-        const long long col = static_cast<long long>(g) * N - lead;
-        float v[N];
-        if (live) {
-            Vec<IN>::unpack(CACHE ? cache[g - lo] : load_group(g), v);
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = exp2_approx((v[i] - m) * p.c) * inv;
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = 0.0f;
-        }
-        if (p.out_vec && col >= 0 && col + N <= p.cols) {
-            store_group(dg + static_cast<size_t>(g) * N, v);
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (col + i >= 0 && col + i < p.cols) store_as(dr + col + i, v[i]);
-        }
-    }
-    if (!live) return;
-    // The teacher's words of this slice, after their neighbours: one thread per distinct word writes p - (its q).
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kOwn; ++i) {
-        const uint32_t k = tid + i * kThreads;
-        if (k >= p.topk) break;
-        const uint32_t id = ids[k];
-        const uint32_t g = (id + lead) / N;
-        if (id == kNoWord || g < lo || g >= hi) continue;
-        bool first = true;
-        for (uint32_t j = 0; j < k; ++j) first = first && ids[j] != id;
-        if (!first) continue;
-        float qk = q[k];
-        for (uint32_t j = k + 1; j < p.topk; ++j)
-            if (ids[j] == id) qk += q[j];
-        store_as(dr + id, a * (exp2_approx((z_own[i] - m) * p.c) / s - qk));
+        for (int e = 0; e < N; ++e) v[e] = exp2_approx((v[e] - r.m) * c);
     }
 }
 
-// Dynamic shared memory above 48 KB has to be asked for once per kernel and device.
-template <typename IN, typename OUT, bool CACHE>
-int32_t launch_distill(t0b_ctx* ctx, const DistillParams& p, uint32_t rows, uint32_t nranks, size_t smem) {
-    auto kfn = topk_distill_kernel<IN, OUT, CACHE>;
-    static std::atomic<bool> configured[64];
-    std::atomic<bool>& done = configured[ctx->device & 63];
-    if (!done.load(std::memory_order_acquire)) {
-        const int32_t rc = check_cuda(ctx, cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kCacheMax + 8 * 1024 + 16)),
-                                      "cudaFuncSetAttribute(topk_distill)");
-        if (rc != T0B_OK) return rc;
-        done.store(true, std::memory_order_release);
+// What the exponentials are kept as between the passes: f32 logits f32, bf16 logits fp16.
+template <typename T> struct Kept;
+template <> struct Kept<float> {
+    static __device__ __forceinline__ uint4 pack(const float (&e)[4]) { return Vec<float>::pack(e); }
+    static __device__ __forceinline__ void unpack(const uint4& q, float (&e)[4]) { Vec<float>::unpack(q, e); }
+};
+template <> struct Kept<__nv_bfloat16> {
+    static __device__ __forceinline__ uint4 pack(const float (&e)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 h = __floats2half2_rn(e[2 * i], e[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
     }
+    static __device__ __forceinline__ void unpack(const uint4& q, float (&e)[8]) {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            e[2 * i] = f.x;
+            e[2 * i + 1] = f.y;
+        }
+    }
+};
+
+// Maximum of a group, NaN left out (it shows in the sum).
+__device__ __forceinline__ float group_max(const uint4& q, const float*) {
+    return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
+}
+__device__ __forceinline__ float group_max(const uint4& q, const __nv_bfloat16*) {
+    auto h = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+    const __nv_bfloat162 m = __hmax2(__hmax2(h(q.x), h(q.y)), __hmax2(h(q.z), h(q.w)));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+
+// The teacher's side of a row in one CTA: each thread owns the words tid, tid + T, ... (at most 1024 in all).
+template <int T>
+struct Words {
+    static constexpr int kOwn = T0B_MAX_TOPK / T;
+    uint32_t id[kOwn];
+    float t[kOwn], z[kOwn];   // t: the teacher's logit, then q
+    float tmax;
+
+    // Warps beyond the last word skip all of it.
+    static __device__ __forceinline__ bool mine(const DistillParams& p, int i) { return i * T + (threadIdx.x & ~31u) < p.topk; }
+
+    template <typename IN>
+    __device__ __forceinline__ void load(const DistillParams& p, uint32_t row, const IN* zr, bool report) {
+        tmax = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            id[i] = kNoWord;
+            t[i] = z[i] = 0.0f;
+            const uint32_t k = threadIdx.x + i * T;
+            if (mine(p, i) && k < p.topk) {
+                id[i] = p.ids[row * p.ldk + k];
+                t[i] = p.teacher[row * p.ldk + k];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+            if (mine(p, i)) {
+                if (id[i] != kNoWord && id[i] >= p.cols) {
+                    if (report) *reinterpret_cast<volatile int*>(p.status) = kDevBadIndex;   // the word is left out
+                    id[i] = kNoWord;
+                }
+                if (id[i] != kNoWord) {
+                    z[i] = to_float(zr[id[i]]);   // before anything is written: dlogits may be the logits
+                    tmax = fmaxf(tmax, t[i]);
+                }
+            }
+    }
+    // Sum of exp((t - max) / T) over this thread's words.
+    __device__ __forceinline__ float sum(const DistillParams& p, float tref) const {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+            if (mine(p, i) && id[i] != kNoWord) s += expf((t[i] - tref) * p.inv_t);
+        return s;
+    }
+    // t becomes q; ids and q go to shared memory; returns sum q log q and sum q over this thread's words.
+    __device__ __forceinline__ float2 probs(const DistillParams& p, float tref, float tsum, bool live, uint32_t* sh_ids, float* sh_q) {
+        float cross = 0.0f, qsum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+            if (mine(p, i)) {
+                const uint32_t k = threadIdx.x + i * T;
+                const float lq = (t[i] - tref) * p.inv_t - logf(tsum);
+                const float qk = (live && id[i] != kNoWord) ? expf(lq) : 0.0f;
+                if (qk != 0.0f) {
+                    cross += qk * lq;
+                    qsum += qk;
+                }
+                t[i] = qk;
+                if (k < p.topk) {
+                    sh_ids[k] = id[i];
+                    sh_q[k] = qk;
+                }
+            }
+        return make_float2(cross, qsum);
+    }
+    // - sum q (z - m) / T over this thread's words.
+    __device__ __forceinline__ float cross(const DistillParams& p, const Ref& all) const {
+        float c = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+            if (mine(p, i) && t[i] != 0.0f) c -= t[i] * all.log_of(z[i], p.c, p.inv_t);
+        return c;
+    }
+    // The gradient at the words of columns [c_lo, c_hi): one thread per distinct word writes a (p - its q).
+    template <typename OUT>
+    __device__ __forceinline__ void gradient(const DistillParams& p, const Ref& all, float a, float total, long long c_lo, long long c_hi,
+                                             const uint32_t* sh_ids, const float* sh_q, OUT* dr) const {
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+            if (mine(p, i) && id[i] != kNoWord && id[i] >= c_lo && id[i] < c_hi) {
+                const uint32_t k = threadIdx.x + i * T;
+                bool first = true;
+#pragma unroll 8
+                for (uint32_t j = 0; j < k; ++j) first = first && sh_ids[j] != id[i];
+                if (!first) continue;
+                float qk = t[i];
+#pragma unroll 8
+                for (uint32_t j = k + 1; j < p.topk; ++j)
+                    if (sh_ids[j] == id[i]) qk += sh_q[j];
+                store_as(dr + id[i], a * (exp2_approx(all.arg(z[i], p.c)) / total - qk));
+            }
+    }
+};
+
+struct RowStats { float m, total; };
+
+// Every CTA of the cluster gets every CTA's (m, s) and joins them in rank order, so all hold the same bits.  `between` runs
+// while the exchange is under way.
+template <typename F>
+__device__ __forceinline__ RowStats exchange(float m, float s, float c, uint32_t nranks, uint32_t rank, float2* xch, F&& between) {
+    if (nranks == 1) {
+        between();
+        return {m, s};
+    }
+    ptx::cluster_wait();   // every CTA has started
+    if (threadIdx.x < nranks) {
+        const uint32_t dst = ptx::mapa(ptx::smem_u32(&xch[rank]), threadIdx.x);
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(dst), "f"(m), "f"(s) : "memory");
+    }
+    ptx::cluster_arrive();
+    between();
+    ptx::cluster_wait();
+    RowStats st{xch[0].x, 0.0f};
+    for (uint32_t r = 1; r < nranks; ++r) st.m = fmaxf(st.m, xch[r].x);
+    const Ref all(st.m, c);
+    for (uint32_t r = 0; r < nranks; ++r) st.total += xch[r].x == -INFINITY ? xch[r].y : xch[r].y * Ref(xch[r].x, c).to(all, c);
+    return st;
+}
+
+// Where a row's whole 16-byte groups are: `front` columns before the first, `groups` of them, `back` columns behind the last.
+template <typename IN>
+struct RowSpan {
+    unsigned long long e0, g_first;
+    uint32_t front, groups, back;
+    __device__ __forceinline__ RowSpan(const DistillParams& p, uint32_t row) {
+        constexpr int N = Vec<IN>::kN;
+        e0 = row * p.ld;
+        g_first = (e0 + N - 1) / N;
+        const unsigned long long g_end = (e0 + p.cols) / N;
+        groups = g_end > g_first ? static_cast<uint32_t>(g_end - g_first) : 0;
+        front = min(p.cols, static_cast<uint32_t>(g_first * N - e0));   // a row within one or two groups may have no whole one
+        back = p.cols - front - groups * N;
+    }
+    __device__ __forceinline__ const uint4* at(const DistillParams& p) const {
+        return reinterpret_cast<const uint4*>(static_cast<const IN*>(p.logits) + g_first * Vec<IN>::kN);
+    }
+};
+
+// The columns of one of the row's ends as a group, filled up with -inf.
+template <typename IN>
+__device__ __forceinline__ uint4 edge_group(const DistillParams& p, const RowSpan<IN>& span, bool at_back) {
+    constexpr int N = Vec<IN>::kN;
+    const IN* z = static_cast<const IN*>(p.logits) + span.e0 + (at_back ? p.cols - span.back : 0);
+    const uint32_t count = at_back ? span.back : span.front;
+    float v[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = e < count ? to_float(z[e]) : -INFINITY;
+    return Vec<IN>::pack(v);
+}
+
+// Rows of more than 64 KB, at least one for every SM: one CTA per row, two an SM.  The row is streamed twice, for the
+// statistics and for the gradient; the second time L2 still has most of it (two rows an SM under way are 76 MB of a
+// 128000-word bf16 batch).  Each thread's 16-byte groups arrive in batches through its own slots of a ring in shared memory,
+// asked for two batches ahead and through both passes, so loads do not stop at the barriers between them.
+// 4096 x 128000 bf16 with gradient: 430 us (4.9 TB/s; 510 us with clusters and the row in shared memory, 640 us with the row
+// in registers); 2048 x 50257 f32, losses alone: 71 us (5.8 TB/s).
+constexpr int kStreamThreads = 512, kRingBatch = 4, kRingBatches = 3;
+template <typename IN, typename OUT>
+__global__ void __launch_bounds__(kStreamThreads, 2) topk_distill_stream_kernel(const DistillParams p) {
+    constexpr int N = Vec<IN>::kN, T = kStreamThreads, B = kRingBatch, S = kRingBatches;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float2 red_max[T / 32], red_sum[T / 32], red_loss[T / 32];
+    uint4* ring = reinterpret_cast<uint4*>(smem);        // slot j of thread t: ring[j * T + t]
+    uint32_t* ids = reinterpret_cast<uint32_t*>(smem + static_cast<size_t>(B) * S * T * 16);
+    float* q = reinterpret_cast<float*>(ids + p.topk);
+    const uint32_t row = blockIdx.x, tid = threadIdx.x;
+    const RowSpan<IN> span(p, row);
+    const IN* zr = static_cast<const IN*>(p.logits) + span.e0;
+    const uint4* zg = span.at(p);
+    const uint32_t batches = (span.groups + T * B - 1) / (T * B);
+    const uint32_t total = p.dlogits ? 2 * batches : batches;
+    // Batch n of the stream (the second pass repeats the first) goes to ring batch n % S; always one group of copies, empty
+    // or not, so that "all but the last S - 1 groups" is the batch in turn.
+    auto ask = [&](uint32_t n) {
+        if (n < total) {
+            const uint32_t first = (n < batches ? n : n - batches) * (B * T) + tid;
+            const uint32_t slot = (n % S) * B;
+#pragma unroll
+            for (int u = 0; u < B; ++u)
+                if (first + u * T < span.groups) __pipeline_memcpy_async(ring + (slot + u) * T + tid, zg + first + u * T, 16);
+        }
+        __pipeline_commit();
+    };
+#pragma unroll
+    for (int n = 0; n < S - 1; ++n) ask(n);
+    Words<T> words;
+    words.load(p, row, zr, true);
+
+    // This thread's running maximum and sum.
+    const IN* kind = nullptr;
+    float m = -INFINITY, s = 0.0f;
+    Ref cur(m, p.c);
+    auto add = [&](const uint4 (&raw)[B], const bool (&have)[B]) {
+        float lm = m;
+#pragma unroll
+        for (int u = 0; u < B; ++u)
+            if (have[u]) lm = fmaxf(lm, group_max(raw[u], kind));
+        if (lm > m) {
+            const Ref next(lm, p.c);
+            if (m != -INFINITY) s *= cur.to(next, p.c);
+            m = lm;
+            cur = next;
+        }
+#pragma unroll
+        for (int u = 0; u < B; ++u)
+            if (have[u]) {
+                float v[N];
+                Vec<IN>::unpack(raw[u], v);
+                exp_group(v, cur, p.c);
+#pragma unroll
+                for (int e = 0; e < N; e += 4) s += (v[e] + v[e + 1]) + (v[e + 2] + v[e + 3]);
+            }
+    };
+    for (uint32_t n = 0; n < batches; ++n) {
+        ask(n + S - 1);
+        __pipeline_wait_prior(S - 1);   // a thread reads only what it asked for itself
+        const uint32_t first = n * (B * T) + tid, slot = (n % S) * B;
+        uint4 raw[B];
+        bool have[B];
+#pragma unroll
+        for (int u = 0; u < B; ++u) {
+            have[u] = first + u * T < span.groups;
+            raw[u] = have[u] ? ring[(slot + u) * T + tid] : make_uint4(0, 0, 0, 0);
+        }
+        add(raw, have);
+    }
+    // The columns outside whole groups, at most N - 1 at each end: one thread each.
+    if (tid < 2) {
+        uint4 raw[B];
+        const bool have[B] = {true, false, false, false};
+        raw[0] = edge_group<IN>(p, span, tid != 0);
+        add(raw, have);
+    }
+    float mall = m;
+    block_max2<T>(mall, words.tmax, red_max);
+    const Ref all(mall, p.c);
+    if (m != -INFINITY) s *= cur.to(all, p.c);
+    const float tref = words.tmax == -INFINITY ? 0.0f : words.tmax;
+    float tsum = words.sum(p, tref);
+    block_sum2<T>(s, tsum, red_sum);
+    bool live = tsum > 0.0f || tsum != tsum;
+    float2 cq = words.probs(p, tref, tsum, live, ids, q);
+    if (mall == -INFINITY && s == 0.0f) live = false;   // every logit is -inf: the row has no distribution
+    if (p.losses) {
+        if (live) cq.x += words.cross(p, all);
+        block_sum2<T>(cq.x, cq.y, red_loss);
+        if (tid == 0) p.losses[row] = live ? fmaf(cq.y, logf(s), cq.x) : 0.0f;
+    }
+    if (!p.dlogits) return;
+    OUT* dr = static_cast<OUT*>(p.dlogits) + span.e0;
+    OUT* dg = static_cast<OUT*>(p.dlogits) + span.g_first * N;
+    const float a = live ? p.scale * (p.weights ? p.weights[row] : 1.0f) : 0.0f;
+    const float inv = a / s;
+    auto gradient = [&](const uint4& g, float (&v)[N]) {
+        Vec<IN>::unpack(g, v);
+        if (live) exp_group(v, all, p.c);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = live ? v[e] * inv : 0.0f;
+    };
+    // The columns outside whole groups first: with dlogits in the place of the logits they are read here once more.
+    if (tid < 2) {
+        float v[N];
+        gradient(edge_group<IN>(p, span, tid != 0), v);
+        const uint32_t col = tid == 0 ? 0 : p.cols - span.back, count = tid == 0 ? span.front : span.back;
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (e < count) store_as(dr + col + e, v[e]);
+    }
+    // In place, too, a thread reads and writes its own groups only.
+    for (uint32_t n = 0; n < batches; ++n) {
+        ask(n + batches + S - 1);
+        __pipeline_wait_prior(S - 1);
+        const uint32_t first = n * (B * T) + tid, slot = ((n + batches) % S) * B;
+#pragma unroll
+        for (int u = 0; u < B; ++u)
+            if (first + u * T < span.groups) {
+                float v[N];
+                gradient(ring[(slot + u) * T + tid], v);
+                store_group(dg + static_cast<size_t>(first + u * T) * N, v);
+            }
+    }
+    __syncthreads();   // the words after their neighbours
+    if (live) words.gradient(p, all, a, s, 0, p.cols, ids, q, dr);
+}
+
+// The fast form: base pointers on 16-byte boundaries (any pitch).  A row's whole
+// 16-byte groups are divided among the cluster's threads, G to each at most, and the partial groups at its two ends go to
+// one thread each (an extra group that only their warps look at).
+template <typename IN, typename OUT, int G>
+__global__ void __launch_bounds__(kThreads, G == 16 ? 2 : (G == 8 ? 3 : 4)) topk_distill_kernel(const DistillParams p) {
+    constexpr int N = Vec<IN>::kN;
+    constexpr bool kKeepExp = !(sizeof(IN) == 2 && sizeof(OUT) == 4);
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float2 red_max[kThreads / 32], red_sum[kThreads / 32], red_loss[kThreads / 32];
+    __shared__ __align__(16) float2 xch[kMaxCluster];
+    uint32_t* ids = reinterpret_cast<uint32_t*>(smem);
+    float* q = reinterpret_cast<float*>(ids + p.topk);
+    uint32_t nranks;
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(nranks));
+    const uint32_t rank = ptx::cluster_ctarank();
+    const uint32_t row = blockIdx.x / nranks;
+    const uint32_t tid = threadIdx.x;
+    if (nranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;");
+
+    const RowSpan<IN> span(p, row);
+    const uint32_t lo = min(rank * p.groups_per_cta, span.groups), n_own = min(p.groups_per_cta, span.groups - lo);
+    const IN* zr = static_cast<const IN*>(p.logits) + span.e0;
+    const uint4* zg = span.at(p) + lo;
+    const bool at_back = tid != 0;
+    const bool has_edge = (tid == 0 && rank == 0 && span.front > 0) || (tid == 32 && rank == nranks - 1 && span.back > 0);
+
+    uint4 raw[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+        if (tid + i * kThreads < n_own) raw[i] = __ldcs(zg + tid + i * kThreads);
+    uint4 edge = make_uint4(0, 0, 0, 0);
+    if (has_edge) edge = edge_group<IN>(p, span, at_back);
+    Words<kThreads> words;
+    words.load(p, row, zr, rank == 0);
+
+    // Maximum of the slice (and of the teacher's logits), over the CTA.
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+        if (tid + i * kThreads < n_own) m = fmaxf(m, group_max(raw[i], static_cast<const IN*>(nullptr)));
+    if (has_edge) m = fmaxf(m, group_max(edge, static_cast<const IN*>(nullptr)));
+    block_max2<kThreads>(m, words.tmax, red_max);
+    // Exponentials relative to it, and their sum.
+    const Ref own(m, p.c);
+    const bool nothing = m == -INFINITY;   // in this slice
+    float s = 0.0f;
+    auto exponentials = [&](uint4& g, bool fused) {
+        float v[N];
+        Vec<IN>::unpack(g, v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = exp2_approx(fused ? fmaf(v[e], p.c, -own.mc) : (v[e] - own.m) * p.c);
+#pragma unroll
+        for (int e = 0; e < N; e += 4) s += (v[e] + v[e + 1]) + (v[e + 2] + v[e + 3]);
+        if (kKeepExp) g = Kept<IN>::pack(v);
+    };
+    if (own.fused) {
+#pragma unroll
+        for (int i = 0; i < G; ++i)
+            if (tid + i * kThreads < n_own) exponentials(raw[i], true);
+    } else {
+#pragma unroll
+        for (int i = 0; i < G; ++i)
+            if (tid + i * kThreads < n_own) exponentials(raw[i], false);
+    }
+    if (has_edge) exponentials(edge, own.fused);
+    const float tref = words.tmax == -INFINITY ? 0.0f : words.tmax;
+    float tsum = words.sum(p, tref);
+    block_sum2<kThreads>(s, tsum, red_sum);
+    bool live = tsum > 0.0f || tsum != tsum;
+    float2 cq;
+    const RowStats st = exchange(m, s, p.c, nranks, rank, xch, [&] { cq = words.probs(p, tref, tsum, live, ids, q); });
+    const Ref all(st.m, p.c);
+    if (st.m == -INFINITY && st.total == 0.0f) live = false;   // every logit is -inf: the row has no distribution
+    if (rank == 0 && p.losses) {
+        if (live) cq.x += words.cross(p, all);
+        block_sum2<kThreads>(cq.x, cq.y, red_loss);
+        if (tid == 0) p.losses[row] = live ? fmaf(cq.y, logf(st.total), cq.x) : 0.0f;
+    }
+    if (!p.dlogits) return;
+    OUT* dr = static_cast<OUT*>(p.dlogits) + span.e0;
+    OUT* dg = static_cast<OUT*>(p.dlogits) + (span.g_first + lo) * N;
+    const float a = live ? p.scale * (p.weights ? p.weights[row] : 1.0f) : 0.0f;
+    const float inv = a / st.total;
+    const float f = kKeepExp ? (nothing ? 0.0f : own.to(all, p.c) * inv) : inv;
+    auto gradient = [&](const uint4& g, float (&v)[N]) {
+        if (kKeepExp) {
+            Kept<IN>::unpack(g, v);
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = live ? v[e] * f : 0.0f;
+        } else {
+            Vec<IN>::unpack(g, v);
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = live ? exp2_approx(all.arg(v[e], p.c)) * f : 0.0f;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+        if (tid + i * kThreads < n_own) {
+            float v[N];
+            gradient(raw[i], v);
+            store_group(dg + static_cast<size_t>(tid + i * kThreads) * N, v);
+        }
+    if (has_edge) {
+        float v[N];
+        gradient(edge, v);
+        const uint32_t col = at_back ? p.cols - span.back : 0, count = at_back ? span.back : span.front;
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (e < count) store_as(dr + col + e, v[e]);
+    }
+    if (!live) return;
+    __syncthreads();   // the words after their neighbours
+    const long long c_lo = (rank == 0 ? 0 : static_cast<long long>(span.front) + static_cast<long long>(lo) * N);
+    const long long c_hi = (rank == nranks - 1 ? p.cols : static_cast<long long>(span.front) + static_cast<long long>(lo + n_own) * N);
+    words.gradient(p, all, a, st.total, c_lo, c_hi, ids, q, dr);
+}
+
+// The general form, one CTA per row: base pointers off their 16-byte boundaries, or rows longer than a cluster's registers.
+// Every pass reads the row by element again (from L2, where it fits).
+template <typename IN, typename OUT>
+__global__ void __launch_bounds__(kThreads) topk_distill_any_kernel(const DistillParams p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float2 red_max[kThreads / 32], red_sum[kThreads / 32], red_loss[kThreads / 32];
+    uint32_t* ids = reinterpret_cast<uint32_t*>(smem);
+    float* q = reinterpret_cast<float*>(ids + p.topk);
+    const uint32_t row = blockIdx.x, tid = threadIdx.x;
+    const IN* zr = static_cast<const IN*>(p.logits) + row * p.ld;
+    Words<kThreads> words;
+    words.load(p, row, zr, true);
+    float m = -INFINITY;
+#pragma unroll 8
+    for (uint32_t i = tid; i < p.cols; i += kThreads) m = fmaxf(m, to_float(zr[i]));
+    block_max2<kThreads>(m, words.tmax, red_max);
+    const Ref all(m, p.c);
+    float s = 0.0f;
+#pragma unroll 8
+    for (uint32_t i = tid; i < p.cols; i += kThreads) s += exp2_approx(all.arg(to_float(zr[i]), p.c));
+    const float tref = words.tmax == -INFINITY ? 0.0f : words.tmax;
+    float tsum = words.sum(p, tref);
+    block_sum2<kThreads>(s, tsum, red_sum);
+    bool live = tsum > 0.0f || tsum != tsum;
+    float2 cq = words.probs(p, tref, tsum, live, ids, q);
+    if (m == -INFINITY && s == 0.0f) live = false;
+    if (p.losses) {
+        if (live) cq.x += words.cross(p, all);
+        block_sum2<kThreads>(cq.x, cq.y, red_loss);
+        if (tid == 0) p.losses[row] = live ? fmaf(cq.y, logf(s), cq.x) : 0.0f;
+    }
+    if (!p.dlogits) return;
+    OUT* dr = static_cast<OUT*>(p.dlogits) + row * p.ld;
+    const float a = live ? p.scale * (p.weights ? p.weights[row] : 1.0f) : 0.0f;
+    const float inv = a / s;
+#pragma unroll 4
+    for (uint32_t i = tid; i < p.cols; i += kThreads) store_as(dr + i, live ? exp2_approx(all.arg(to_float(zr[i]), p.c)) * inv : 0.0f);
+    if (!live) return;
+    __syncthreads();
+    words.gradient(p, all, a, s, 0, p.cols, ids, q, dr);
+}
+
+template <typename IN, typename OUT, int G>
+int32_t launch_distill(t0b_ctx* ctx, const DistillParams& p, uint32_t rows, uint32_t nranks) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(rows * nranks);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = p.topk * 8ull;
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -344,7 +664,45 @@ int32_t launch_distill(t0b_ctx* ctx, const DistillParams& p, uint32_t rows, uint
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return check_cuda(ctx, cudaLaunchKernelEx(&cfg, kfn, p), "cudaLaunchKernelEx(topk_distill)");
+    return check_cuda(ctx, cudaLaunchKernelEx(&cfg, topk_distill_kernel<IN, OUT, G>, p), "cudaLaunchKernelEx(topk_distill)");
+}
+
+template <typename IN, typename OUT>
+int32_t launch_stream(t0b_ctx* ctx, const DistillParams& p, uint32_t rows) {
+    auto kfn = topk_distill_stream_kernel<IN, OUT>;
+    constexpr size_t kRing = static_cast<size_t>(kRingBatch) * kRingBatches * kStreamThreads * 16;
+    static std::atomic<bool> configured[64];
+    std::atomic<bool>& done = configured[ctx->device & 63];
+    if (!done.load(std::memory_order_acquire)) {   // dynamic shared memory above 48 KB has to be asked for
+        const int32_t rc = check_cuda(ctx, cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kRing + T0B_MAX_TOPK * 8)), "cudaFuncSetAttribute(topk_distill)");
+        if (rc != T0B_OK) return rc;
+        done.store(true, std::memory_order_release);
+    }
+    kfn<<<rows, kStreamThreads, kRing + p.topk * 8ull, ctx->stream>>>(p);
+    return check_cuda(ctx, cudaGetLastError(), "topk_distill launch");
+}
+
+template <typename IN, typename OUT>
+int32_t run_distill(t0b_ctx* ctx, DistillParams p, uint32_t rows) {
+    constexpr uint32_t N = Vec<IN>::kN;
+    const uint32_t groups = p.cols / N + 1;
+    const bool aligned = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && reinterpret_cast<uintptr_t>(p.dlogits) % std::min<size_t>(16, N * sizeof(OUT)) == 0;
+    if (!aligned) {
+        topk_distill_any_kernel<IN, OUT><<<rows, kThreads, p.topk * 8ull, ctx->stream>>>(p);
+        return check_cuda(ctx, cudaGetLastError(), "topk_distill launch");
+    }
+    // Rows that one CTA's registers hold stay there.  Longer ones are streamed when there is one for every SM (1001 x 32003
+    // f32: 63 us against 69 us for clusters of two); with fewer rows clusters of CTAs share them: enough that a thread's
+    // groups fit its registers, and more while SMs would idle and every thread still has two groups (24 x 32000 f32: 5.6 us).
+    if (groups > kThreads * 16 && (rows >= static_cast<uint32_t>(ctx->num_sms) || groups > kMaxCluster * kThreads * 16)) return launch_stream<IN, OUT>(ctx, p, rows);
+    uint32_t nranks = 1;
+    while (groups > nranks * kThreads * 16) nranks *= 2;
+    while (nranks < kMaxCluster && static_cast<uint64_t>(rows) * nranks < static_cast<uint64_t>(ctx->num_sms) && groups >= nranks * kThreads * 4) nranks *= 2;
+    p.groups_per_cta = (groups + nranks - 1) / nranks;
+    if (p.groups_per_cta <= 2 * kThreads) return launch_distill<IN, OUT, 2>(ctx, p, rows, nranks);
+    if (p.groups_per_cta <= 4 * kThreads) return launch_distill<IN, OUT, 4>(ctx, p, rows, nranks);
+    if (p.groups_per_cta <= 8 * kThreads) return launch_distill<IN, OUT, 8>(ctx, p, rows, nranks);
+    return launch_distill<IN, OUT, 16>(ctx, p, rows, nranks);
 }
 
 }  // namespace
@@ -375,7 +733,6 @@ int32_t t0b_topk_distill(t0b_ctx* ctx, uint64_t logits, int32_t logits_dtype, ui
                                           {"losses", losses, rows * 4ull}, {"row_weights", row_weights, rows * 4ull}});
     if (rc != T0B_OK) return rc;
 
-    const uint32_t n = static_cast<uint32_t>(16 / ie);
     DistillParams p{};
     p.logits = reinterpret_cast<const void*>(logits);
     p.dlogits = reinterpret_cast<void*>(dlogits);
@@ -387,27 +744,9 @@ int32_t t0b_topk_distill(t0b_ctx* ctx, uint64_t logits, int32_t logits_dtype, ui
     p.inv_t = 1.0f / temperature;
     p.c = 1.4426950408889634f / temperature;
     p.scale = scale / temperature;
-    p.in_vec = logits % 16 == 0;
-    p.out_vec = dlogits % std::min<size_t>(16, n * oe) == 0;
     p.status = ctx->status_dev;
-    // CTAs per row: enough that four slices fit an SM (their loads and stores overlap each other), and more while few rows
-    // would leave SMs idle and the slices stay worth a CTA.
-    const size_t groups = (static_cast<size_t>(cols) + n - 1) / n + 1;   // one more where rows start off a 16-byte boundary
-    uint32_t nranks = 1;
-    while (nranks < kMaxCluster && groups * 16 / nranks > 48 * 1024) nranks *= 2;
-    while (nranks < kMaxCluster && static_cast<uint64_t>(rows) * nranks < static_cast<uint64_t>(ctx->num_sms) && groups * 16 / nranks >= 8 * 1024) nranks *= 2;
-    if (static_cast<uint64_t>(rows) * nranks > 0x7fffffffull) return set_error(ctx, T0B_ERR_INVALID, "topk_distill: %u rows are too many", rows);
-    p.groups_per_cta = static_cast<uint32_t>((groups + nranks - 1) / nranks);
-    const bool cached = p.groups_per_cta * 16ull <= kCacheMax;
-    const size_t smem = (cached ? p.groups_per_cta * 16ull : 0) + topk * 8ull;
-    const bool in16 = ie == 2, out16 = oe == 2;
-    if (in16) {
-        if (out16) rc = cached ? launch_distill<__nv_bfloat16, __nv_bfloat16, true>(ctx, p, rows, nranks, smem) : launch_distill<__nv_bfloat16, __nv_bfloat16, false>(ctx, p, rows, nranks, smem);
-        else rc = cached ? launch_distill<__nv_bfloat16, float, true>(ctx, p, rows, nranks, smem) : launch_distill<__nv_bfloat16, float, false>(ctx, p, rows, nranks, smem);
-    } else {
-        if (out16) rc = cached ? launch_distill<float, __nv_bfloat16, true>(ctx, p, rows, nranks, smem) : launch_distill<float, __nv_bfloat16, false>(ctx, p, rows, nranks, smem);
-        else rc = cached ? launch_distill<float, float, true>(ctx, p, rows, nranks, smem) : launch_distill<float, float, false>(ctx, p, rows, nranks, smem);
-    }
+    if (ie == 2) rc = oe == 2 ? run_distill<__nv_bfloat16, __nv_bfloat16>(ctx, p, rows) : run_distill<__nv_bfloat16, float>(ctx, p, rows);
+    else rc = oe == 2 ? run_distill<float, __nv_bfloat16>(ctx, p, rows) : run_distill<float, float>(ctx, p, rows);
     if (rc != T0B_OK) return rc;
     return finish(ctx, async, "topk_distill");
 }

@@ -255,6 +255,8 @@ def check_logits(th, art, rows, cols, topk, *, dtype=OUT_F32, gdt=None, temperat
     a = (row_scale / temperature).abs()[:, None] * live[:, None]
     uo = UB if gdt == OUT_BF16 else U32
     bound = uo * dz.abs() + a * (p * (down * 4 + 16) + q * (8 + 4 * ent.abs()[:, None])) * U32 * 2 + 1e-37
+    if dtype == gdt == OUT_BF16:      # exponentials kept in fp16 between the passes, relative to the largest of their slice
+        bound += a * (1 + uo) * (p * UH + 2.0 ** -24 * p.amax(1, keepdim=True))
     err = (dview[:, :cols].double() - dz).abs()
     assert (err <= bound).all(), (err / bound).max()
     assert (dview[:, :cols][~live] == 0).all()
