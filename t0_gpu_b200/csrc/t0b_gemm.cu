@@ -450,7 +450,7 @@ GemmCall call_of(const InnerGemm& d) {
     g.trans_a = d.trans_a; g.trans_b = d.trans_b; g.a = d.a; g.b = d.b;
     g.c_dst[0] = d.c; g.n_dst = 1; g.m = d.m; g.n = d.n; g.k = d.k; g.lda = d.lda; g.ldb = d.ldb; g.ldc = d.ldc;
     g.out_bf16 = d.out_bf16; g.accumulate = d.accumulate; g.workspace = d.slabs; g.workspace_bytes = d.slab_bytes;
-    g.no_auto_split = d.accumulate || d.no_split;
+    g.no_auto_split = d.accumulate;
     return g;
 }
 
@@ -465,7 +465,7 @@ size_t inner_gemm_slab_bytes(t0b_ctx* ctx, const InnerGemm& d) {
     const GemmCall g = call_of(d);
     t0b_gemm_config cfg;
     const char* source = "";
-    if (g.accumulate || choose_config(ctx, g, &cfg, &source) != T0B_OK) return 0;
+    if (d.head_grad || g.accumulate || choose_config(ctx, g, &cfg, &source) != T0B_OK) return 0;
     t0b_gemm_plan plan;
     const PlanInput pin{g.m, g.n, g.k, g.trans_a, g.trans_b, g.lda, g.ldb, g.a, g.b, ctx->num_sms};
     resolve_plan(&cfg, pin, &plan);
@@ -473,20 +473,52 @@ size_t inner_gemm_slab_bytes(t0b_ctx* ctx, const InnerGemm& d) {
     return static_cast<size_t>(plan.split_k) * g.m * g.n * 4;
 }
 
+// A tile for the head's gradient product: a huge output, a contraction over the rows of a batch, no split.  The cost model of
+// t0b_gemm is made for long contractions; here a wave costs what its stores or its operands from L2 cost, whichever is more.
+// Cycles measured at 32000 x 1024 x 128, 50257 x 1000 x 777 and 4096 x 32000 x 1024 (m, n, rows): with 128 rows 128x256 tiles
+// take 19.6 us against 25.2 for 256x512; with 777 rows 122 us against 101 for 256x256 and 96 for 256x512.
+static t0b_gemm_config head_grad_config(t0b_ctx* ctx, const GemmCall& g) {
+    struct Cand { const char* name; uint32_t bm, bn, cg; double kb_cycles, epi, floor; };
+    static const Cand cands[] = {{"b200_256x512", 256, 512, 2, 1165.0, 10500.0, 0.0}, {"b200_256x256", 256, 256, 2, 830.0, 0.0, 6500.0},
+                                 {"b200_128x256", 128, 256, 1, 1000.0, 0.0, 4900.0},  {"b200_128x128", 128, 128, 1, 700.0, 0.0, 3000.0}};
+    const double kb = (g.k + 63) / 64;
+    const Cand* best = nullptr;
+    double best_cost = 1e300;
+    for (const Cand& c : cands) {
+        const uint64_t tiles = static_cast<uint64_t>((g.m + c.bm - 1) / c.bm) * ((g.n + c.bn - 1) / c.bn), clusters = static_cast<uint64_t>(ctx->num_sms) / c.cg;
+        const double cost = static_cast<double>((tiles + clusters - 1) / clusters) * std::max(kb * c.kb_cycles + c.epi, c.floor);
+        if (cost < best_cost) {
+            best_cost = cost;
+            best = &c;
+        }
+    }
+    t0b_gemm_config cfg{};
+    t0b_config_preset(best->name, &cfg);
+    cfg.swap_grid = g.m >= g.n ? 1 : 0;
+    return cfg;
+}
+
 int32_t inner_gemm(t0b_ctx* ctx, const InnerGemm& d) {
     GemmCall g = call_of(d);
     // The caller's slabs were sized for the config of that moment; a table entry that appeared since may want more.  The
     // context's own workspace is never used here: it may be freed by a later call while a captured graph still holds it.
-    if (inner_gemm_slab_bytes(ctx, d) > d.slab_bytes) g.no_auto_split = true;
+    t0b_gemm_config cfg;
+    if (d.head_grad) {
+        cfg = head_grad_config(ctx, g);
+        g.cfg = &cfg;
+    } else if (inner_gemm_slab_bytes(ctx, d) > d.slab_bytes) {
+        g.no_auto_split = true;
+    }
     return run_gemm(ctx, g);
 }
 
 HeadPlan head_plan(t0b_ctx* ctx, uint32_t rows, uint32_t vocab, uint32_t dim) {
-    // The three tiles of the softmax epilogue by the cost model of the plain product (cycles per 64-deep K block and the
-    // epilogue that bounds a tile with a short contraction): a CTA pair shares each head column block between 256 rows; one
-    // CTA takes 128 rows, in 256 or 128 columns, whichever fills the last wave better.
+    // The three tiles of the softmax epilogue by waves and cycles per 64-deep K block, or per epilogue where that is more: a CTA
+    // pair shares each block of head columns between 256 rows; a single CTA takes 128 rows, in 256 or 128 columns, and needs
+    // 1.5 times the operand bytes from L2 for the same products (777 x 1000 -> 50257: 129 us against the pair's 101 us, although
+    // the pair's last rows are padding; 16 x 1024 -> 32000: 18.7 us against 22.1 us).
     struct Cand { uint32_t bm, bn, cg; double kb_cycles, epi_cycles; };
-    static const Cand cands[] = {{256, 256, 2, 780.0, 4000.0}, {128, 256, 1, 760.0, 4000.0}, {128, 128, 1, 700.0, 2200.0}};
+    static const Cand cands[] = {{256, 256, 2, 800.0, 5000.0}, {128, 256, 1, 900.0, 5000.0}, {128, 128, 1, 700.0, 2800.0}};
     const double kb = (dim + 63) / 64;
     HeadPlan best{};
     double best_cost = 1e300;

@@ -130,7 +130,7 @@ struct InnerGemm {
     uint64_t lda, ldb, ldc;
     int out_bf16;
     bool accumulate;   // C += A*B, f32
-    bool no_split;
+    bool head_grad;    // the head's gradient: its own choice of tile, never split
     uint64_t slabs;
     size_t slab_bytes;
 };

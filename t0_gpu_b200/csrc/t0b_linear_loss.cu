@@ -46,39 +46,152 @@ __device__ __forceinline__ void join_stats(float& m, float& s, float m2, float s
     m = mm;
 }
 
+// --------------------------------------------------------------------------------------------------- rows as operands
+__device__ __forceinline__ uint4 pack_bf16x8(const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+        w[e] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Columns c ... c + 7 of a row of `cols` elements as bf16, zeros behind its end.
+template <typename IN>
+__device__ __forceinline__ uint4 operand_group(const IN* row, uint32_t c, uint32_t cols, bool vec) {
+    const IN* src = row + c;
+    if constexpr (sizeof(IN) == 2) {
+        if (vec && c + 8 <= cols) return *reinterpret_cast<const uint4*>(src);
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t a = c + 2 * e < cols ? *reinterpret_cast<const uint16_t*>(src + 2 * e) : 0u;
+            const uint32_t b = c + 2 * e + 1 < cols ? *reinterpret_cast<const uint16_t*>(src + 2 * e + 1) : 0u;
+            w[e] = a | (b << 16);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+        float v[8];
+        if (vec && c + 8 <= cols) {
+            const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? static_cast<float>(src[e]) : 0.0f;
+        }
+        return pack_bf16x8(v);
+    }
+}
+template <typename IN>
+__device__ __forceinline__ bool rows_vec(const IN* in, unsigned long long ld) {
+    return (reinterpret_cast<uintptr_t>(in) & 15) == 0 && ld % (16 / sizeof(IN)) == 0;
+}
+
+// out[r, c] = bf16(in[r, c]), rows of `cols` elements at a pitch of whole 16 bytes; a row without a target is written as zeros,
+// whatever it holds (its hidden state may be anything, and 0 * NaN would reach the head's gradient).
+template <typename IN>
+__global__ void __launch_bounds__(256) pack_rows_kernel(const IN* in, unsigned long long ld, __nv_bfloat16* out, uint32_t ld_out, uint32_t rows,
+                                                        uint32_t cols, const uint32_t* targets, uint32_t vocab) {
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
+    const uint32_t per_row = ld_out / 8;
+    const unsigned long long total = static_cast<unsigned long long>(rows) * per_row;
+    const bool vec = rows_vec(in, ld);
+    for (unsigned long long i = blockIdx.x * 256ull + threadIdx.x; i < total; i += gridDim.x * 256ull) {
+        const uint32_t r = static_cast<uint32_t>(i / per_row), c = static_cast<uint32_t>(i % per_row) * 8;
+        const uint4 o = targets[r] < vocab ? operand_group(in + r * ld, c, cols, vec) : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(out + static_cast<unsigned long long>(r) * ld_out + c) = o;
+    }
+}
+
+// The same copy of a bf16 matrix whose rows start off 16-byte boundaries (a head with an odd vocabulary, [dim, vocab]): a warp
+// reads whole 16-byte chunks of the source, a lane shifts its chunk and its neighbour's into the 16 bytes it writes.  Chunks
+// that reach over the matrix' ends are read by element.  2048 x 50257: 206 MB each way, bound by HBM.
+__global__ void __launch_bounds__(256) pack_shifted_kernel(const __nv_bfloat16* in, unsigned long long ld, __nv_bfloat16* out, uint32_t ld_out,
+                                                           uint32_t rows, uint32_t cols) {
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t per_row = ld_out / 8, warps_per_row = (per_row + 31) / 32;
+    const unsigned long long total = static_cast<unsigned long long>(rows) * warps_per_row;
+    const uint64_t begin = reinterpret_cast<uint64_t>(in), end = begin + ((rows - 1ull) * ld + cols) * 2;
+    for (unsigned long long i = blockIdx.x * 8ull + (threadIdx.x >> 5); i < total; i += gridDim.x * 8ull) {
+        const uint32_t r = static_cast<uint32_t>(i / warps_per_row);
+        const uint32_t c = (static_cast<uint32_t>(i % warps_per_row) * 32 + lane) * 8;
+        const uint64_t at = begin + (r * ld + c) * 2, chunk = at & ~15ull;
+        const uint32_t shift = static_cast<uint32_t>(at & 15);
+        auto load = [&](uint64_t addr) {
+            return addr >= begin && addr + 16 <= end ? __ldcs(reinterpret_cast<const uint4*>(addr)) : make_uint4(0, 0, 0, 0);
+        };
+        const uint4 a = load(chunk);
+        uint4 b;
+        b.x = __shfl_down_sync(0xffffffffu, a.x, 1);
+        b.y = __shfl_down_sync(0xffffffffu, a.y, 1);
+        b.z = __shfl_down_sync(0xffffffffu, a.z, 1);
+        b.w = __shfl_down_sync(0xffffffffu, a.w, 1);
+        if (c >= ld_out) continue;
+        if (lane == 31) b = load(chunk + 16);
+        uint4 o;
+        if (chunk < begin || chunk + (shift ? 32 : 16) > end || c + 8 > cols) {
+            o = operand_group(in + r * ld, c, cols, false);
+        } else {
+            uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int e = 0; e < 6; ++e) w[e] = (shift & 8) ? w[e + 2] : w[e];
+#pragma unroll
+            for (int e = 0; e < 5; ++e) w[e] = (shift & 4) ? w[e + 1] : w[e];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = __funnelshift_r(w[e], w[e + 1], (shift & 2) * 8);
+            o = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        *reinterpret_cast<uint4*>(out + static_cast<unsigned long long>(r) * ld_out + c) = o;
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ the teacher's words
 // One row per threadIdx.y, one word per threadIdx.x (P = a power of two >= topk): q = softmax(t / T) over the words that are
 // there, entropy = sum q log q, and the words in ascending order of id (what the head's epilogue searches).  A word named
-// more than once keeps its first place with the sum of its q; the other places get q = -1.
-__global__ void __launch_bounds__(1024) teacher_words_kernel(const uint32_t* __restrict__ ids, const float* __restrict__ teacher,
-                                                             unsigned long long ldk, uint32_t rows, uint32_t topk, uint32_t vocab,
-                                                             float inv_t, uint32_t* __restrict__ out_ids, float* __restrict__ out_q,
-                                                             float* __restrict__ entropy, uint32_t* __restrict__ live, int* status) {
+// more than once keeps its first place with the sum of its q; the other places get q = -1.  Then the row's hidden state is
+// copied as pack_rows_kernel does it (x_out null: no copy is needed).
+template <typename IN>
+__global__ void __launch_bounds__(1024) teacher_words_kernel(const uint32_t* ids, const float* teacher, unsigned long long ldk, uint32_t rows,
+                                                             uint32_t topk, uint32_t vocab, float inv_t, uint32_t* out_ids, float* out_q,
+                                                             float* entropy, uint32_t* live, int* status, const IN* x, unsigned long long ldx,
+                                                             __nv_bfloat16* x_out, uint32_t ldx_out, uint32_t dim) {
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
     extern __shared__ __align__(16) uint8_t smem[];
-    const uint32_t P = blockDim.x, x = threadIdx.x, y = threadIdx.y;
+    const uint32_t P = blockDim.x, k = threadIdx.x, y = threadIdx.y;
     unsigned long long* key = reinterpret_cast<unsigned long long*>(smem) + static_cast<size_t>(y) * P;
     float* val = reinterpret_cast<float*>(smem + static_cast<size_t>(blockDim.y) * P * 8) + static_cast<size_t>(y) * P;
     const uint32_t row = blockIdx.x * blockDim.y + y;
-    const bool in = row < rows && x < topk;
+    const bool in = row < rows && k < topk;
     uint32_t id = kNoWord;
     float t = -INFINITY;
     if (in) {
-        id = ids[row * ldk + x];
+        id = ids[row * ldk + k];
+        t = teacher[row * ldk + k];
         if (id != kNoWord && id >= vocab) {
             *reinterpret_cast<volatile int*>(status) = kDevBadIndex;   // the word is left out
             id = kNoWord;
         }
-        if (id != kNoWord) t = teacher[row * ldk + x];
+        if (id == kNoWord) t = -INFINITY;
     }
+    // Over the row: within its warps by shuffles (P >= 32), then over the warps.
     auto reduce = [&](float v, bool is_max) -> float {
-        __syncthreads();
-        val[x] = v;
-        __syncthreads();
-        for (uint32_t o = P >> 1; o > 0; o >>= 1) {
-            if (x < o) val[x] = is_max ? fmaxf(val[x], val[x + o]) : val[x] + val[x + o];
-            __syncthreads();
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const float u = __shfl_xor_sync(0xffffffffu, v, o);
+            v = is_max ? fmaxf(v, u) : v + u;
         }
-        return val[0];
+        if (P == 32) return v;
+        __syncthreads();
+        if ((k & 31) == 0) val[k >> 5] = v;
+        __syncthreads();
+        v = val[0];
+        for (uint32_t i = 1; i < P / 32; ++i) v = is_max ? fmaxf(v, val[i]) : v + val[i];
+        return v;
     };
     const float mx = reduce(t, true);
     const float ref = mx == -INFINITY ? 0.0f : mx;
@@ -89,91 +202,50 @@ __global__ void __launch_bounds__(1024) teacher_words_kernel(const uint32_t* __r
     const float q = (some && id != kNoWord) ? e / sum : 0.0f;
     const float ent = reduce(q != 0.0f ? q * lq : 0.0f, false);
     __syncthreads();
-    key[x] = (static_cast<unsigned long long>(some ? id : kNoWord) << 32) | x;
-    val[x] = q;
+    key[k] = (static_cast<unsigned long long>(some ? id : kNoWord) << 32) | k;
+    val[k] = q;
     __syncthreads();
     for (uint32_t size = 2; size <= P; size <<= 1)
         for (uint32_t stride = size >> 1; stride > 0; stride >>= 1) {
-            const uint32_t other = x ^ stride;
-            if (other > x) {
-                const unsigned long long a = key[x], b = key[other];
-                if ((a > b) == ((x & size) == 0)) {
-                    key[x] = b;
+            const uint32_t other = k ^ stride;
+            if (other > k) {
+                const unsigned long long a = key[k], b = key[other];
+                if ((a > b) == ((k & size) == 0)) {
+                    key[k] = b;
                     key[other] = a;
                 }
             }
-            __syncthreads();
+            if (stride >= 32) __syncthreads();   // partners in one warp: the warp's own order is enough
+            else __syncwarp();
+            if (stride == 1) __syncthreads();
         }
     if (in) {
-        const uint32_t my = static_cast<uint32_t>(key[x] >> 32);
-        float qs = val[static_cast<uint32_t>(key[x])];
+        const uint32_t my = static_cast<uint32_t>(key[k] >> 32);
+        float qs = val[static_cast<uint32_t>(key[k])];
         if (my != kNoWord) {
-            if (x > 0 && static_cast<uint32_t>(key[x - 1] >> 32) == my) qs = -1.0f;
+            if (k > 0 && static_cast<uint32_t>(key[k - 1] >> 32) == my) qs = -1.0f;
             else
-                for (uint32_t i = x + 1; i < P && static_cast<uint32_t>(key[i] >> 32) == my; ++i) qs += val[static_cast<uint32_t>(key[i])];
+                for (uint32_t i = k + 1; i < P && static_cast<uint32_t>(key[i] >> 32) == my; ++i) qs += val[static_cast<uint32_t>(key[i])];
         }
-        out_ids[static_cast<size_t>(row) * topk + x] = my;
-        out_q[static_cast<size_t>(row) * topk + x] = qs;
-        if (x == 0) {
+        out_ids[static_cast<size_t>(row) * topk + k] = my;
+        out_q[static_cast<size_t>(row) * topk + k] = qs;
+        if (k == 0) {
             entropy[row] = some ? ent : 0.0f;
             live[row] = some ? 1u : 0u;
         }
     }
-}
-
-// --------------------------------------------------------------------------------------------------- rows as operands
-// out[r, c] = bf16(in[r, c]), rows of `cols` elements at a pitch of whole 16 bytes; a row that has no target is written as
-// zeros, whatever it holds (its hidden state may be anything, and 0 * NaN would reach the head's gradient).
-template <typename IN>
-__global__ void __launch_bounds__(256) pack_rows_kernel(const IN* __restrict__ in, unsigned long long ld, __nv_bfloat16* __restrict__ out,
-                                                        uint32_t ld_out, uint32_t rows, uint32_t cols, const uint32_t* __restrict__ targets,
-                                                        uint32_t vocab, const uint32_t* __restrict__ live) {
-    const uint32_t per_row = ld_out / 8;
-    const unsigned long long total = static_cast<unsigned long long>(rows) * per_row;
-    const bool vec = (reinterpret_cast<uintptr_t>(in) & 15) == 0 && ld % (16 / sizeof(IN)) == 0;
-    for (unsigned long long i = blockIdx.x * 256ull + threadIdx.x; i < total; i += gridDim.x * 256ull) {
-        const uint32_t r = static_cast<uint32_t>(i / per_row), c = static_cast<uint32_t>(i % per_row) * 8;
-        const bool on = targets ? targets[r] < vocab : (live ? live[r] != 0 : true);
-        uint4 o = make_uint4(0, 0, 0, 0);
-        if (on) {
-            const IN* src = in + r * ld + c;
-            if constexpr (sizeof(IN) == 2) {
-                if (vec && c + 8 <= cols) o = *reinterpret_cast<const uint4*>(src);
-                else {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t a = c + 2 * e < cols ? *reinterpret_cast<const uint16_t*>(src + 2 * e) : 0u;
-                        const uint32_t b = c + 2 * e + 1 < cols ? *reinterpret_cast<const uint16_t*>(src + 2 * e + 1) : 0u;
-                        w[e] = a | (b << 16);
-                    }
-                    o = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-            } else {
-                float v[8];
-                if (vec && c + 8 <= cols) {
-                    const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
-                    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? static_cast<float>(src[e]) : 0.0f;
-                }
-                uint32_t w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-                    w[e] = *reinterpret_cast<const uint32_t*>(&h);
-                }
-                o = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        }
-        *reinterpret_cast<uint4*>(out + static_cast<unsigned long long>(r) * ld_out + c) = o;
+    if (x_out && row < rows) {
+        const bool vec = rows_vec(x, ldx);
+        for (uint32_t c = k * 8; c < ldx_out; c += P * 8)
+            *reinterpret_cast<uint4*>(x_out + static_cast<unsigned long long>(row) * ldx_out + c) =
+                some ? operand_group(x + row * ldx, c, dim, vec) : make_uint4(0, 0, 0, 0);
     }
 }
 
 // out[r, c] = bf16(acc[r, c]): the head's gradient summed in f32 over several pieces, rounded once.
-__global__ void __launch_bounds__(256) round_rows_kernel(const float* __restrict__ acc, uint32_t ld_acc, __nv_bfloat16* __restrict__ out,
+__global__ void __launch_bounds__(256) round_rows_kernel(const float* acc, uint32_t ld_acc, __nv_bfloat16* out,
                                                          unsigned long long ld, uint32_t rows, uint32_t cols) {
+    ptx::grid_dependency_wait();
     const uint32_t per_row = (cols + 7) / 8;
     const unsigned long long total = static_cast<unsigned long long>(rows) * per_row;
     const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && ld % 8 == 0;
@@ -184,13 +256,7 @@ __global__ void __launch_bounds__(256) round_rows_kernel(const float* __restrict
         const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
         __nv_bfloat16* dst = out + r * ld + c;
         if (vec && c + 8 <= cols) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-                w[e] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-            *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(dst) = pack_bf16x8(v);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -213,10 +279,12 @@ __device__ __forceinline__ bool row_live(const Targets& t, uint32_t row) { retur
 
 // One block per 32 rows: warps walk the parts (a warp's load is 32 neighbouring rows of one part), the warps' results meet in
 // shared memory, then warp i finishes row i: stats[row] = (max z, sum of exp), the loss and log-sum-exp.
-__global__ void __launch_bounds__(1024) join_parts_kernel(const float2* __restrict__ part, unsigned long long part_ld, uint32_t parts, uint32_t rows,
-                                                          float c, float inv_t, Targets tg, float2* __restrict__ stats,
-                                                          float* __restrict__ losses, float* __restrict__ lse_out, int* status) {
+__global__ void __launch_bounds__(1024) join_parts_kernel(const float2* part, unsigned long long part_ld, uint32_t parts, uint32_t rows,
+                                                          float c, float inv_t, Targets tg, float2* stats,
+                                                          float* losses, float* lse_out, int* status) {
     __shared__ float2 sh[32][33];
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t row = blockIdx.x * 32 + lane;
     float m = -INFINITY, s = 0.0f;
@@ -269,9 +337,11 @@ __global__ void __launch_bounds__(1024) join_parts_kernel(const float2* __restri
 // words of the targets are written last, from their f32 logit.  Bound by HBM: 2 bytes in, 2 bytes out per element.
 constexpr int kGradVecs = 4;
 constexpr uint32_t kGradCols = 256 * 8 * kGradVecs;
-__global__ void __launch_bounds__(256) dz_kernel(__half* __restrict__ u, unsigned long long ldu, uint32_t rows, const float2* __restrict__ part,
-                                                 unsigned long long part_ld, uint32_t part_shift, const float2* __restrict__ stats,
-                                                 const float* __restrict__ weights, float scale, float c, Targets tg) {
+__global__ void __launch_bounds__(256) dz_kernel(__half* u, unsigned long long ldu, uint32_t rows, const float2* part,
+                                                 unsigned long long part_ld, uint32_t part_shift, const float2* stats,
+                                                 const float* weights, float scale, float c, Targets tg) {
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
     const uint32_t row = blockIdx.y;
     const uint32_t c0 = blockIdx.x * kGradCols;
     __half* ur = u + row * ldu;
@@ -315,6 +385,23 @@ __global__ void __launch_bounds__(256) dz_kernel(__half* __restrict__ u, unsigne
         if (q < 0.0f) continue;
         gr[id] = __float2bfloat16_rn(a * (exp2_approx((tg.z_sel[at] - st.x) * c) * inv - q));
     }
+}
+
+// Programmatic launch: a kernel's blocks may be placed while the one before drains; every kernel here waits for it before it
+// touches memory.
+template <typename... P, typename... A>
+void launch(t0b_ctx* ctx, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ctx->pdl ? 1 : 0;
+    cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);   // an error stays with the runtime until finish() asks
 }
 
 uint64_t align256(uint64_t x) { return (x + 255) & ~255ull; }
@@ -363,7 +450,7 @@ InnerGemm dw_gemm(const t0b_linear_loss& d, const Plan& p, uint64_t u, uint64_t 
     g.ldc = p.acc_dw ? p.ld_acc : d.lddw;
     g.out_bf16 = !p.acc_dw && d.dw_dtype == T0B_OUT_BF16;
     g.accumulate = r0 > 0;
-    g.no_split = p.pieces > 1;
+    g.head_grad = true;
     return g;
 }
 
@@ -414,7 +501,6 @@ Plan make_plan(t0b_ctx* ctx, const t0b_linear_loss& d, uint32_t n_ids, bool teac
         const uint32_t n = std::min(p.piece, d.rows - r0);
         if (r0 > 0 && n == p.piece) continue;   // like the first
         if (p.dx) p.slab_bytes = std::max<uint64_t>(p.slab_bytes, inner_gemm_slab_bytes(ctx, dx_gemm(d, p, 256, 256, r0, n)));
-        if (p.dw) p.slab_bytes = std::max<uint64_t>(p.slab_bytes, inner_gemm_slab_bytes(ctx, dw_gemm(d, p, 256, 256, 256, r0, n)));
     }
     p.slabs = take(p.slab_bytes);
     p.total = std::max<uint64_t>(off, 256);
@@ -494,35 +580,36 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
     int32_t rc = get_scratch(ctx, what, d, p.total, &base);
     if (rc != T0B_OK) return rc;
     const float c = 1.4426950408889634f / temperature, inv_t = 1.0f / temperature;
-    cudaStream_t st = ctx->stream;
     int launched = 0;
 
+    const uint64_t x = p.copy_x ? base + p.x : d.x, w = p.copy_w ? base + p.w : d.w;
+    __nv_bfloat16* x_out = reinterpret_cast<__nv_bfloat16*>(p.copy_x ? base + p.x : 0);
+    const bool x16 = d.x_dtype == T0B_OUT_BF16;
+    const __nv_bfloat16* xb = reinterpret_cast<const __nv_bfloat16*>(d.x);
+    const float* xf = reinterpret_cast<const float*>(d.x);
     if (teacher) {
         uint32_t P = 32;
         while (P < te.topk) P *= 2;
         const uint32_t ny = std::max(1u, 128u / P);
-        teacher_words_kernel<<<(d.rows + ny - 1) / ny, dim3(P, ny), static_cast<size_t>(P) * ny * 12, st>>>(
-            reinterpret_cast<const uint32_t*>(te.ids), reinterpret_cast<const float*>(te.logits), te.ldk, d.rows, te.topk, d.vocab, inv_t,
-            reinterpret_cast<uint32_t*>(base + p.ids), reinterpret_cast<float*>(base + p.q), reinterpret_cast<float*>(base + p.entropy),
-            reinterpret_cast<uint32_t*>(base + p.live), ctx->status_dev);
+        auto words = [&](auto kernel, auto* xp) {
+            launch(ctx, kernel, dim3((d.rows + ny - 1) / ny), dim3(P, ny), static_cast<size_t>(P) * ny * 12, reinterpret_cast<const uint32_t*>(te.ids),
+                   reinterpret_cast<const float*>(te.logits), te.ldk, d.rows, te.topk, d.vocab, inv_t, reinterpret_cast<uint32_t*>(base + p.ids),
+                   reinterpret_cast<float*>(base + p.q), reinterpret_cast<float*>(base + p.entropy), reinterpret_cast<uint32_t*>(base + p.live),
+                   ctx->status_dev, xp, d.ldx, x_out, static_cast<uint32_t>(p.ldx), d.dim);
+        };
+        if (x16) words(teacher_words_kernel<__nv_bfloat16>, xb);
+        else words(teacher_words_kernel<float>, xf);
         ++launched;
-    }
-    const uint64_t x = p.copy_x ? base + p.x : d.x, w = p.copy_w ? base + p.w : d.w;
-    if (p.copy_x) {
+    } else if (p.copy_x) {
         const uint32_t blocks = lin_blocks(ctx, d.rows * (p.ldx / 8));
-        const uint32_t* targets = teacher ? nullptr : reinterpret_cast<const uint32_t*>(te.ids);
-        const uint32_t* live = teacher ? reinterpret_cast<const uint32_t*>(base + p.live) : nullptr;
-        __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(base + p.x);
-        if (d.x_dtype == T0B_OUT_BF16)
-            pack_rows_kernel<<<blocks, 256, 0, st>>>(reinterpret_cast<const __nv_bfloat16*>(d.x), d.ldx, out, static_cast<uint32_t>(p.ldx), d.rows, d.dim, targets, d.vocab, live);
-        else
-            pack_rows_kernel<<<blocks, 256, 0, st>>>(reinterpret_cast<const float*>(d.x), d.ldx, out, static_cast<uint32_t>(p.ldx), d.rows, d.dim, targets, d.vocab, live);
+        const uint32_t* targets = reinterpret_cast<const uint32_t*>(te.ids);
+        if (x16) launch(ctx, pack_rows_kernel<__nv_bfloat16>, blocks, 256, 0, xb, d.ldx, x_out, static_cast<uint32_t>(p.ldx), d.rows, d.dim, targets, d.vocab);
+        else launch(ctx, pack_rows_kernel<float>, blocks, 256, 0, xf, d.ldx, x_out, static_cast<uint32_t>(p.ldx), d.rows, d.dim, targets, d.vocab);
         ++launched;
     }
     if (p.copy_w) {
-        pack_rows_kernel<<<lin_blocks(ctx, p.w_rows * (p.ldw / 8)), 256, 0, st>>>(
-            reinterpret_cast<const __nv_bfloat16*>(d.w), d.ldw, reinterpret_cast<__nv_bfloat16*>(base + p.w), static_cast<uint32_t>(p.ldw),
-            static_cast<uint32_t>(p.w_rows), static_cast<uint32_t>(p.w_cols), nullptr, 0u, nullptr);
+        launch(ctx, pack_shifted_kernel, lin_blocks(ctx, p.w_rows * ((p.ldw / 8 + 31) / 32 * 32)), 256, 0, reinterpret_cast<const __nv_bfloat16*>(d.w), d.ldw,
+               reinterpret_cast<__nv_bfloat16*>(base + p.w), static_cast<uint32_t>(p.ldw), static_cast<uint32_t>(p.w_rows), static_cast<uint32_t>(p.w_cols));
         ++launched;
     }
     uint32_t part_shift = 0;
@@ -555,9 +642,8 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
         rc = head_gemm(ctx, hg);
         if (rc != T0B_OK) return rc;
         float2* stats = reinterpret_cast<float2*>(base + p.stats) + r0;
-        join_parts_kernel<<<(n + 31) / 32, 1024, 0, st>>>(reinterpret_cast<const float2*>(base + p.part), p.part_ld, p.parts, n, c, inv_t, tg, stats,
-                                                          d.losses ? reinterpret_cast<float*>(d.losses) + r0 : nullptr,
-                                                          d.lse ? reinterpret_cast<float*>(d.lse) + r0 : nullptr, ctx->status_dev);
+        launch(ctx, join_parts_kernel, (n + 31) / 32, 1024, 0, reinterpret_cast<const float2*>(base + p.part), p.part_ld, p.parts, n, c, inv_t, tg, stats,
+               d.losses ? reinterpret_cast<float*>(d.losses) + r0 : nullptr, d.lse ? reinterpret_cast<float*>(d.lse) + r0 : nullptr, ctx->status_dev);
         ++launched;
         if (!p.grads) continue;
         // gridDim.y is limited to 65535 rows a launch.
@@ -567,7 +653,7 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
             t2.ids += static_cast<size_t>(y0) * te.topk;
             if (teacher) { t2.q += static_cast<size_t>(y0) * te.topk; t2.entropy += y0; t2.live += y0; }
             t2.z_sel += static_cast<size_t>(y0) * te.topk;
-            dz_kernel<<<dim3(static_cast<uint32_t>((p.ldu + kGradCols - 1) / kGradCols), ny), 256, 0, st>>>(
+            launch(ctx, dz_kernel, dim3(static_cast<uint32_t>((p.ldu + kGradCols - 1) / kGradCols), ny), 256, 0,
                 reinterpret_cast<__half*>(base + p.u) + y0 * p.ldu, p.ldu, ny, reinterpret_cast<const float2*>(base + p.part) + y0, p.part_ld, part_shift,
                 stats + y0, d.row_weights ? reinterpret_cast<const float*>(d.row_weights) + r0 + y0 : nullptr, d.scale * inv_t, c, t2);
             ++launched;
@@ -590,7 +676,7 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
         }
     }
     if (p.acc_dw) {
-        round_rows_kernel<<<lin_blocks(ctx, p.w_rows * ((p.w_cols + 7) / 8)), 256, 0, st>>>(
+        launch(ctx, round_rows_kernel, lin_blocks(ctx, p.w_rows * ((p.w_cols + 7) / 8)), 256, 0,
             reinterpret_cast<const float*>(base + p.acc), static_cast<uint32_t>(p.ld_acc), reinterpret_cast<__nv_bfloat16*>(d.dw), d.lddw,
             static_cast<uint32_t>(p.w_rows), static_cast<uint32_t>(p.w_cols));
         ++launched;
