@@ -72,7 +72,8 @@ struct HeadParams {
     float2* part;            // [parts][part_ld]
     long long part_ld;       // rows, padded
     float c;                 // log2(e) / T: exp(v / T) = 2^(c v)
-    const uint32_t* ids;     // [rows][n_ids], ascending within a row; entries >= N are never met
+    const uint32_t* ids;     // [..][n_ids], ascending within a row; entries >= N are never met
+    const uint32_t* row_of;  // which row of `ids` a row of the product is; null: the same
     int n_ids;
     float* z_sel;            // [rows][n_ids]: z of those columns
     int store_u;
@@ -103,6 +104,10 @@ struct GemmParams {
     unsigned long long* trace;   // timeline build only: [CTA][16] stamps of this launch (null = no stamps)
 #endif
     int accumulate;         // 1: C += the product (f32 output, one destination, no split-K)
+    // Rows counted on the device: M (dyn_k = 0) or K (dyn_k = 1) is at most *dyn_rows - dyn_off, and the launch was sized for
+    // the most there can be.  K comes as whole blocks of zero rows behind the last (one at least).
+    const int* dyn_rows;
+    int dyn_off, dyn_k;
     HeadParams head;        // HEAD kernels only
     int cluster_sk;         // > 1: split-K inside a thread-block cluster of that many CTAs (one per K range): the partial
                             // tiles stay in shared memory and are summed over distributed shared memory; 0 = slabs
@@ -158,13 +163,16 @@ struct WorkItem {
     int m0, n0, split, kb_begin, kb_end;
 };
 
-__device__ __forceinline__ WorkItem decode_work(const GemmParams& p, int w, int bm, int bn) {
-    const int num_tiles = p.tiles_m * p.tiles_n;
+// The extents of the product as this launch sees them (GemmParams, or less where rows are counted on the device).
+struct Extents { int M, tiles_m, kb_total, num_work; };
+
+__device__ __forceinline__ WorkItem decode_work(const GemmParams& p, const Extents& x, int w, int bm, int bn) {
+    const int num_tiles = x.tiles_m * p.tiles_n;
     // Cluster split-K: the CTAs of a cluster (consecutive work items) are the K ranges of one tile.
     const int split = p.cluster_sk > 1 ? w % p.cluster_sk : w / num_tiles;
     const int tile = p.cluster_sk > 1 ? w / p.cluster_sk : w - split * num_tiles;
-    int major_cnt = p.raster_along_n ? p.tiles_n : p.tiles_m;   // dimension that is grouped
-    int minor_cnt = p.raster_along_n ? p.tiles_m : p.tiles_n;
+    int major_cnt = p.raster_along_n ? p.tiles_n : x.tiles_m;   // dimension that is grouped
+    int minor_cnt = p.raster_along_n ? x.tiles_m : p.tiles_n;
     const int per_group = p.group * minor_cnt;
     const int g = tile / per_group;
     const int first = g * p.group;
@@ -177,7 +185,7 @@ __device__ __forceinline__ WorkItem decode_work(const GemmParams& p, int w, int 
     wi.n0 = (p.raster_along_n ? major : minor) * bn;
     wi.split = split;
     wi.kb_begin = split * p.kb_per_split;
-    wi.kb_end = min(p.kb_total, wi.kb_begin + p.kb_per_split);
+    wi.kb_end = min(x.kb_total, wi.kb_begin + p.kb_per_split);
     return wi;
 }
 
@@ -504,13 +512,13 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
     // Cluster split-K (single-CTA tiles only): the CTAs of the cluster are the K ranges of one tile.
     const bool csk = (CG == 1 && MT == 1) && p.cluster_sk > 1;
     const WaitCtl ctl{abort_flag, p.status, p.wait_limit_ns};
-    const int num_work = p.tiles_m * p.tiles_n * p.split_k;
+    Extents ext{p.M, p.tiles_m, p.kb_total, p.tiles_m * p.tiles_n * p.split_k};
     const int cluster_id = blockIdx.x / CG;
     const int num_clusters = gridDim.x / CG;
     // The first work item is decoded here, before the dependency wait: the parameter reads and the divisions of the
     // decode (half a microsecond on a cold SM, measured with globaltimer stamps) then overlap the previous kernel's
     // tail.  The empty asm pins the values in front of the wait.
-    const WorkItem first_wi = decode_work(p, cluster_id < num_work ? cluster_id : 0, BM, BNT);
+    WorkItem first_wi = decode_work(p, ext, cluster_id < ext.num_work ? cluster_id : 0, BM, BNT);
     asm volatile("" ::"r"(first_wi.m0), "r"(first_wi.n0), "r"(first_wi.kb_begin), "r"(first_wi.kb_end), "r"(first_wi.split));
     if (threadIdx.x == 0) T0B_STAMP(1);
     // Programmatic dependent launch: everything above (barriers, TMEM, descriptor prefetch) may run while the previous
@@ -518,6 +526,19 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
     ptx::grid_dependency_wait();
     if (threadIdx.x == 0) T0B_STAMP(2);
     ptx::grid_launch_dependents();   // the next GEMM's CTAs may take over SMs as this grid's CTAs exit
+    if (p.dyn_rows != nullptr) {
+        const int n = max(0, min(*p.dyn_rows - p.dyn_off, p.dyn_k ? p.K : p.M));
+        if (p.dyn_k) {
+            ext.kb_total = max(1, (n + kBk - 1) / kBk);
+            if (n == 0 && p.accumulate) ext.num_work = 0;   // nothing to add
+        } else {
+            ext.M = n;
+            ext.tiles_m = (n + BM - 1) / BM;
+            ext.num_work = ext.tiles_m * p.tiles_n * p.split_k;
+        }
+        if (cluster_id < ext.num_work) first_wi = decode_work(p, ext, cluster_id, BM, BNT);
+    }
+    const int num_work = ext.num_work;
 
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer
@@ -526,7 +547,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
             uint32_t ph = 0;
             bool ok = true;
             for (int w = cluster_id; w < num_work && ok; w += num_clusters) {
-                const WorkItem wi = (w == cluster_id) ? first_wi : decode_work(p, w, BM, BNT);
+                const WorkItem wi = (w == cluster_id) ? first_wi : decode_work(p, ext, w, BM, BNT);
                 const int m0_cta = wi.m0 + static_cast<int>(cta_rank) * kBmCta;
                 const int n0_cta = wi.n0 + static_cast<int>(cta_rank) * T::kBnCta;
                 for (int kb = wi.kb_begin; kb < wi.kb_end; ++kb) {
@@ -592,7 +613,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
             uint32_t slot_ph[2] = {0u, 0u};    // phase of each accumulator slot
             bool ok = true;
             for (int w = cluster_id; w < num_work && ok; w += num_clusters) {
-                const WorkItem wi = (w == cluster_id) ? first_wi : decode_work(p, w, BM, BNT);
+                const WorkItem wi = (w == cluster_id) ? first_wi : decode_work(p, ext, w, BM, BNT);
                 if constexpr (MT == 1) {
                     if (!bounded_wait(tempty_bar(acc), slot_ph[acc] ^ 1u, ctl, DEV_TIMEOUT_TMEM_EMPTY)) { ok = false; break; }
                     ptx::tc_fence_after();
@@ -690,7 +711,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
         if (tma_out && lane == 0) ptx::prefetch_tmap(&tmap_c);
         const uint32_t stage = ctrl + T::kCtrlBytes + static_cast<uint32_t>(warp - 2) * 4096u;
         for (int w = cluster_id; w < num_work; w += num_clusters) {
-            const WorkItem wi = (w == cluster_id) ? first_wi : decode_work(p, w, BM, BNT);
+            const WorkItem wi = (w == cluster_id) ? first_wi : decode_work(p, ext, w, BM, BNT);
             if (!bounded_wait_warp(tfull_bar(slot), slot_phase, ctl, DEV_TIMEOUT_TMEM_FULL, lane, p.wait_hint_ns)) break;
             if (warp == 2 && lane == 0) T0B_STAMP(6);
             ptx::tc_fence_after();
@@ -715,14 +736,16 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                 }
                 const int col0 = n_base + c_begin * 32;
                 const int ncols = p.N - col0;
-                if (row0 < p.M && ncols > 0) {   // warp-uniform
+                if (row0 < ext.M && ncols > 0) {   // warp-uniform
                     float v[W];
 #pragma unroll
                     for (int j = 0; j < W; ++j) v[j] = (j < ncols) ? __uint_as_float(raw[j]) : -INFINITY;
                     const HeadParams& hp = p.head;
                     if (hp.n_ids > 0) {
                         // The columns this row asks for: ids ascend, so the ones of this part are consecutive.
-                        const uint32_t* rid = hp.ids + static_cast<long long>(row < p.M ? row : 0) * hp.n_ids;
+                        long long r_ids = row < ext.M ? row : 0;
+                        if (hp.row_of) r_ids = hp.row_of[r_ids];
+                        const uint32_t* rid = hp.ids + r_ids * hp.n_ids;
                         int at = 0;
                         if (hp.n_ids > 1) {
                             int hi = hp.n_ids;
@@ -733,7 +756,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                             }
                         }
                         uint32_t j = at < hp.n_ids ? rid[at] - static_cast<uint32_t>(col0) : 0xffffffffu;
-                        bool hit = row < p.M && j < static_cast<uint32_t>(W);
+                        bool hit = row < ext.M && j < static_cast<uint32_t>(W);
                         while (__any_sync(0xffffffffu, hit)) {
                             const float z = pick_reg<W>(v, j);
                             if (hit) {
@@ -758,7 +781,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                         v[j] = exp2_approx((v[j] - ref) * hp.c);
                         sm[j & 3] += v[j];
                     }
-                    if (row < p.M) hp.part[static_cast<long long>(col0 / W) * hp.part_ld + row] = make_float2(m, (sm[0] + sm[1]) + (sm[2] + sm[3]));
+                    if (row < ext.M) hp.part[static_cast<long long>(col0 / W) * hp.part_ld + row] = make_float2(m, (sm[0] + sm[1]) + (sm[2] + sm[3]));
                     if (hp.store_u) {
 #pragma unroll
                         for (int c = 0; c < kChunks; ++c) {
@@ -812,7 +835,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                                      "r"(raw[4 * j + 1]), "r"(raw[4 * j + 2]), "r"(raw[4 * j + 3])
                                      : "memory");
                 } else if (tma_out && out16) {
-                    if (row0 < p.M && ncols > 0) {   // warp-uniform
+                    if (row0 < ext.M && ncols > 0) {   // warp-uniform
                         float v[32];
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
@@ -838,7 +861,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                 } else if (staged && out16) {
                     const int half = c & 1;
                     if (half == 0) __syncwarp();   // the previous pair's reads of the staging tile are done
-                    if (row0 < p.M && ncols > 0) {   // warp-uniform
+                    if (row0 < ext.M && ncols > 0) {   // warp-uniform
                         float v[32];
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
@@ -855,13 +878,13 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                     if (half == 1) {
                         __syncwarp();
                         const int cbase = col0 - 32;
-                        if (row0 < p.M && cbase < p.N) {
+                        if (row0 < ext.M && cbase < p.N) {
                             for (int d = 0; d < p.n_dst; ++d)
-                                flush_pair_bf16(stage, lane, static_cast<__nv_bfloat16*>(p.c_dst[d]), ld_out, row0, cbase, p.M, p.N);
+                                flush_pair_bf16(stage, lane, static_cast<__nv_bfloat16*>(p.c_dst[d]), ld_out, row0, cbase, ext.M, p.N);
                         }
                     }
                 } else if (staged) {
-                    if (row0 < p.M && ncols > 0) {   // warp-uniform
+                    if (row0 < ext.M && ncols > 0) {   // warp-uniform
                         float v[32];
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
@@ -897,13 +920,13 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                         __syncwarp();
                         if (to_slab) {
                             flush_chunk_f32(stage, lane, p.partial + static_cast<long long>(wi.split) * p.slab_stride, ld_out,
-                                            row0, col0, p.M, p.N);
+                                            row0, col0, ext.M, p.N);
                         } else {
                             for (int d = 0; d < p.n_dst; ++d)
-                                flush_chunk_f32(stage, lane, static_cast<float*>(p.c_dst[d]), ld_out, row0, col0, p.M, p.N, p.accumulate != 0);
+                                flush_chunk_f32(stage, lane, static_cast<float*>(p.c_dst[d]), ld_out, row0, col0, ext.M, p.N, p.accumulate != 0);
                         }
                     }
-                } else if (row < p.M && ncols > 0) {
+                } else if (row < ext.M && ncols > 0) {
                     float v[32];
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
@@ -951,7 +974,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
         ptx::cluster_arrive();
         ptx::cluster_wait();
         if (threadIdx.x == 64) T0B_STAMP(13);
-        if (warp >= 2 && !*abort_flag) {
+        if (warp >= 2 && !*abort_flag && cluster_id < num_work) {
             const int sk = p.cluster_sk;
             const WorkItem& wi = first_wi;   // a cluster split-K CTA has exactly one work item (CG == 1: cluster_id == blockIdx.x)
             const int rows_per = kBmCta / sk;
@@ -976,7 +999,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                         acc[2] = acc[2] + part[sidx].z; acc[3] = acc[3] + part[sidx].w;
                     }
                 const int row = wi.m0 + rl, col = wi.n0 + pc * 4;
-                if (row >= p.M || col >= p.N) continue;
+                if (row >= ext.M || col >= p.N) continue;
                 if (p.epi.n > 0) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)

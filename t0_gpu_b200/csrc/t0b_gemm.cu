@@ -83,6 +83,8 @@ struct GemmCall {
     uint32_t force_split;   // for slabs_only: the exact number of slabs the caller expects
     bool no_auto_split;     // an automatically chosen config keeps the whole contraction in one tile (fixed summation order)
     bool accumulate;        // C += A*B (f32 output, one destination, never split)
+    const int* dyn_rows;    // rows counted on the device (GemmParams)
+    int dyn_off, dyn_k;
 };
 
 // Expand the public single-op epilogue code into a chain (EPI_BIAS_RELU = bias add, then ReLU).
@@ -365,6 +367,7 @@ int32_t run_gemm(t0b_ctx* ctx, const GemmCall& g) {
         p.b_mn_major = g.trans_b ? 0 : 1;     // B stored [K,N]: N contiguous
         p.out_bf16 = g.out_bf16;
         p.accumulate = g.accumulate ? 1 : 0;
+        p.dyn_rows = g.dyn_rows; p.dyn_off = g.dyn_off; p.dyn_k = g.dyn_k;
         p.raster_along_n = cfg.swap_grid ? 0 : 1;
         {
             p.group = raster_group(ctx, plan.bm, plan.bn, plan.cta_group, cfg.swap_grid != 0);
@@ -451,6 +454,7 @@ GemmCall call_of(const InnerGemm& d) {
     g.c_dst[0] = d.c; g.n_dst = 1; g.m = d.m; g.n = d.n; g.k = d.k; g.lda = d.lda; g.ldb = d.ldb; g.ldc = d.ldc;
     g.out_bf16 = d.out_bf16; g.accumulate = d.accumulate; g.workspace = d.slabs; g.workspace_bytes = d.slab_bytes;
     g.no_auto_split = d.accumulate;
+    g.dyn_rows = reinterpret_cast<const int*>(d.dyn_rows); g.dyn_off = d.dyn_off; g.dyn_k = d.dyn_k;
     return g;
 }
 
@@ -569,6 +573,9 @@ int32_t head_gemm(t0b_ctx* ctx, const HeadGemm& d) {
     p.head.part_ld = static_cast<long long>(d.part_ld);
     p.head.c = d.c;
     p.head.ids = reinterpret_cast<const uint32_t*>(d.ids);
+    p.head.row_of = reinterpret_cast<const uint32_t*>(d.row_of);
+    p.dyn_rows = reinterpret_cast<const int*>(d.dyn_rows);
+    p.dyn_off = d.dyn_off;
     p.head.n_ids = static_cast<int>(d.n_ids);
     p.head.z_sel = reinterpret_cast<float*>(d.z_sel);
     p.head.store_u = d.u ? 1 : 0;

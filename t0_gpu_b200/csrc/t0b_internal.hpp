@@ -133,6 +133,8 @@ struct InnerGemm {
     bool head_grad;    // the head's gradient: its own choice of tile, never split
     uint64_t slabs;
     size_t slab_bytes;
+    uint64_t dyn_rows;   // device int, or 0: m (dyn_k: k) is at most *dyn_rows - dyn_off
+    int dyn_off, dyn_k;
 };
 size_t inner_gemm_slab_bytes(t0b_ctx* ctx, const InnerGemm& d);
 int32_t inner_gemm(t0b_ctx* ctx, const InnerGemm& d);
@@ -150,6 +152,9 @@ struct HeadGemm {
     uint64_t part, part_ld;      // float2 [ceil(vocab / part_cols)][part_ld]
     uint64_t ids, z_sel;         // u32 / f32 [rows][n_ids]
     uint32_t n_ids;
+    uint64_t row_of;             // u32[rows]: the row of ids that belongs to a row of x; 0 = the same
+    uint64_t dyn_rows;           // device int, or 0: rows is at most *dyn_rows - dyn_off
+    int dyn_off;
     uint64_t u, ldu;             // fp16 [rows][ldu], ldu a multiple of 8; 0 = statistics alone
 };
 int32_t head_gemm(t0b_ctx* ctx, const HeadGemm& d);

@@ -265,15 +265,105 @@ __global__ void __launch_bounds__(256) round_rows_kernel(const float* acc, uint3
     }
 }
 
+// ------------------------------------------------------------------------------------------------ rows with a target
+// Which rows have a target, in order: row_of[i] = the i-th of them, place_of[r] = its place or kNoWord, count = how many.  The
+// products then run over those rows alone, and count stays on the device.  One block: thread t looks at the rows
+// [t * per, (t + 1) * per).  Rows that are left out get their losses here.
+__global__ void __launch_bounds__(1024) live_rows_kernel(const uint32_t* targets, const uint32_t* live, uint32_t vocab, uint32_t rows, uint32_t* row_of,
+                                                         uint32_t* place_of, int* count, float* losses, float* lse, int* status) {
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
+    __shared__ uint32_t warp_sums[32];
+    const uint32_t per = (rows + 1023) / 1024, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t lo = min(rows, threadIdx.x * per), hi = min(rows, lo + per);
+    uint32_t mine = 0;
+    for (uint32_t r = lo; r < hi; ++r) mine += live ? (live[r] != 0) : (targets[r] < vocab);
+    uint32_t upto = mine;   // inclusive sum over the warp
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) warp_sums[warp] = upto;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+    for (uint32_t w = 0; w < 32; ++w) {
+        if (w < warp) before += warp_sums[w];
+        all += warp_sums[w];
+    }
+    uint32_t at = before + upto - mine;
+    for (uint32_t r = lo; r < hi; ++r) {
+        const bool on = live ? (live[r] != 0) : (targets[r] < vocab);
+        if (on) row_of[at] = r;
+        else {
+            if (losses) losses[r] = 0.0f;
+            if (lse) lse[r] = 0.0f;
+            if (!live && targets[r] != kNoWord) *reinterpret_cast<volatile int*>(status) = kDevBadIndex;
+        }
+        place_of[r] = on ? at++ : kNoWord;
+    }
+    if (threadIdx.x == 0) *count = static_cast<int>(all);
+}
+
+// The rows with a target, gathered as bf16 operand rows, and 64 rows of zeros behind the last: the head's gradient contracts
+// whole 64-row blocks, counted from the start of a piece.
+template <typename IN>
+__global__ void __launch_bounds__(256) gather_rows_kernel(const IN* in, unsigned long long ld, __nv_bfloat16* out, uint32_t ld_out, uint32_t rows,
+                                                          uint32_t cols, const uint32_t* row_of, const int* count) {
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
+    const uint32_t per_row = ld_out / 8, n = static_cast<uint32_t>(*count), padded = min(rows, n + 64);
+    const unsigned long long total = static_cast<unsigned long long>(padded) * per_row;
+    const bool vec = rows_vec(in, ld);
+    for (unsigned long long i = blockIdx.x * 256ull + threadIdx.x; i < total; i += gridDim.x * 256ull) {
+        const uint32_t r = static_cast<uint32_t>(i / per_row), c = static_cast<uint32_t>(i % per_row) * 8;
+        const uint4 o = r < n ? operand_group(in + row_of[r] * ld, c, cols, vec) : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(out + static_cast<unsigned long long>(r) * ld_out + c) = o;
+    }
+}
+
+// dx[r, :] = the gathered gradient at the row's place, or zeros.  T: the gradient's type, moved as it is.
+template <typename T>
+__global__ void __launch_bounds__(256) spread_rows_kernel(const T* in, uint32_t ld_in, T* out, unsigned long long ld, uint32_t rows, uint32_t cols,
+                                                          const uint32_t* place_of) {
+    ptx::grid_dependency_wait();
+    constexpr uint32_t N = 16 / sizeof(T);
+    const uint32_t per_row = (cols + N - 1) / N;
+    const unsigned long long total = static_cast<unsigned long long>(rows) * per_row;
+    const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && ld % N == 0;
+    for (unsigned long long i = blockIdx.x * 256ull + threadIdx.x; i < total; i += gridDim.x * 256ull) {
+        const uint32_t r = static_cast<uint32_t>(i / per_row), c = static_cast<uint32_t>(i % per_row) * N;
+        const uint32_t at = place_of[r];
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (at != kNoWord) v = *reinterpret_cast<const uint4*>(in + static_cast<unsigned long long>(at) * ld_in + c);   // pitch: whole 16 bytes
+        T* dst = out + r * ld + c;
+        if (vec && c + N <= cols) {
+            *reinterpret_cast<uint4*>(dst) = v;
+        } else {
+            const T* e = reinterpret_cast<const T*>(&v);
+            for (uint32_t j = 0; j < N && c + j < cols; ++j) dst[j] = e[j];
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------- joining the parts
 // What the join and the gradient pass know about the targets of a row.
 struct Targets {
-    const uint32_t* ids;      // [rows][n_ids]
+    const uint32_t* ids;      // [rows][n_ids], by row of the call like q, entropy and live
     const float* q;           // [rows][n_ids], null: cross entropy (one word, q = 1)
     const float* entropy;     // [rows], with q
     const uint32_t* live;     // [rows], with q
-    const float* z_sel;       // [rows][n_ids]
+    const float* z_sel;       // [rows of the piece][n_ids]
     uint32_t n_ids, vocab;
+    // Products over the rows with a target alone: row i of a piece is row row_of[row0 + i] of the call, and the piece has
+    // count - row0 of them.  Null: row i is row row0 + i.
+    const uint32_t* row_of;
+    const int* count;
+    uint32_t row0;
+    __device__ __forceinline__ uint32_t rows_here(uint32_t most) const {
+        return row_of ? static_cast<uint32_t>(max(0, min(static_cast<int>(most), *count - static_cast<int>(row0)))) : most;
+    }
+    __device__ __forceinline__ uint32_t row(uint32_t i) const { return row_of ? row_of[row0 + i] : row0 + i; }
 };
 __device__ __forceinline__ bool row_live(const Targets& t, uint32_t row) { return t.q ? t.live[row] != 0 : t.ids[row] < t.vocab; }
 
@@ -286,21 +376,24 @@ __global__ void __launch_bounds__(1024) join_parts_kernel(const float2* part, un
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t row = blockIdx.x * 32 + lane;
+    rows = tg.rows_here(rows);
+    if (blockIdx.x * 32 >= rows) return;
+    const uint32_t at = blockIdx.x * 32 + lane;
     float m = -INFINITY, s = 0.0f;
-    if (row < rows) {
+    if (at < rows) {
         for (uint32_t i = warp; i < parts; i += 128) {
             float2 v[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = i + 32 * u < parts ? part[(i + 32 * u) * part_ld + row] : make_float2(-INFINITY, 0.0f);
+            for (int u = 0; u < 4; ++u) v[u] = i + 32 * u < parts ? part[(i + 32 * u) * part_ld + at] : make_float2(-INFINITY, 0.0f);
 #pragma unroll
             for (int u = 0; u < 4; ++u) join_stats(m, s, v[u].x, v[u].y, c);
         }
     }
     sh[warp][lane] = make_float2(m, s);
     __syncthreads();
-    const uint32_t r = blockIdx.x * 32 + warp;
-    if (r >= rows) return;
+    const uint32_t i = blockIdx.x * 32 + warp;   // the row of the piece, and r of the call
+    if (i >= rows) return;
+    const uint32_t r = tg.row(i);
     m = sh[lane][warp].x;
     s = sh[lane][warp].y;
 #pragma unroll
@@ -313,19 +406,20 @@ __global__ void __launch_bounds__(1024) join_parts_kernel(const float2* part, un
     const float log_s = logf(s);
     float cross = 0.0f;
     if (live) {
+        const float* z = tg.z_sel + static_cast<size_t>(i) * tg.n_ids;
         if (tg.q) {
             for (uint32_t k = lane; k < tg.n_ids; k += 32) {
                 const float q = tg.q[static_cast<size_t>(r) * tg.n_ids + k];
                 if (tg.ids[static_cast<size_t>(r) * tg.n_ids + k] == kNoWord || q == 0.0f || q < 0.0f) continue;
-                cross += q * (log_s - (tg.z_sel[static_cast<size_t>(r) * tg.n_ids + k] - m) * inv_t);
+                cross += q * (log_s - (z[k] - m) * inv_t);
             }
             cross = warp_sum(cross) + tg.entropy[r];
         } else {
-            cross = log_s - (tg.z_sel[r] - m) * inv_t;
+            cross = log_s - (z[0] - m) * inv_t;
         }
     }
     if (lane == 0) {
-        stats[r] = make_float2(m, s);
+        stats[i] = make_float2(m, s);
         if (losses) losses[r] = live ? cross : 0.0f;
         if (lse_out) lse_out[r] = live ? m * inv_t + log_s : 0.0f;
         if (!tg.q && tg.ids[r] >= tg.vocab && tg.ids[r] != kNoWord) *reinterpret_cast<volatile int*>(status) = kDevBadIndex;
@@ -337,55 +431,65 @@ __global__ void __launch_bounds__(1024) join_parts_kernel(const float2* part, un
 // words of the targets are written last, from their f32 logit.  Bound by HBM: 2 bytes in, 2 bytes out per element.
 constexpr int kGradVecs = 4;
 constexpr uint32_t kGradCols = 256 * 8 * kGradVecs;
-__global__ void __launch_bounds__(256) dz_kernel(__half* u, unsigned long long ldu, uint32_t rows, const float2* part,
+__global__ void __launch_bounds__(256) dz_kernel(__half* u, unsigned long long ldu, uint32_t rows, uint32_t y0, const float2* part,
                                                  unsigned long long part_ld, uint32_t part_shift, const float2* stats,
                                                  const float* weights, float scale, float c, Targets tg) {
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
-    const uint32_t row = blockIdx.y;
+    const uint32_t i = y0 + blockIdx.y;          // the row of the piece, and r of the call
     const uint32_t c0 = blockIdx.x * kGradCols;
-    __half* ur = u + row * ldu;
+    const uint32_t n = tg.rows_here(rows);
+    const bool behind = i >= n;                  // zeros up to a whole 64-row block: the head's gradient reads it
+    if (behind && i >= max(64u, (n + 63) / 64 * 64)) return;
+    const uint32_t r = behind ? 0 : tg.row(i);
+    __half* ur = u + i * ldu;
     __nv_bfloat16* gr = reinterpret_cast<__nv_bfloat16*>(ur);
-    const float2 st = stats[row];
-    const bool live = row_live(tg, row) && !(st.x == -INFINITY && st.y == 0.0f);
-    const float a = live ? scale * (weights ? weights[row] : 1.0f) : 0.0f;
+    const float2 st = behind ? make_float2(0.0f, 1.0f) : stats[i];
+    const bool live = !behind && row_live(tg, r) && !(st.x == -INFINITY && st.y == 0.0f);
+    const float a = live ? scale * (weights ? weights[r] : 1.0f) : 0.0f;
     const float inv = 1.0f / st.y;
     uint4 raw[kGradVecs];
+    float top[kGradVecs];
 #pragma unroll
-    for (int i = 0; i < kGradVecs; ++i) {
-        const uint32_t col = c0 + (i * 256 + threadIdx.x) * 8;
-        if (live && col < ldu) raw[i] = *reinterpret_cast<const uint4*>(ur + col);
+    for (int v = 0; v < kGradVecs; ++v) {
+        const uint32_t col = c0 + (v * 256 + threadIdx.x) * 8;
+        if (live && col < ldu) {
+            raw[v] = __ldcs(reinterpret_cast<const uint4*>(ur + col));
+            top[v] = part[(col >> part_shift) * part_ld + i].x;
+        }
     }
 #pragma unroll
-    for (int i = 0; i < kGradVecs; ++i) {
-        const uint32_t col = c0 + (i * 256 + threadIdx.x) * 8;
+    for (int v = 0; v < kGradVecs; ++v) {
+        const uint32_t col = c0 + (v * 256 + threadIdx.x) * 8;
         if (col >= ldu) continue;
         uint4 o = make_uint4(0, 0, 0, 0);
         if (live) {
-            const float f = a * (exp2_approx((part[(col >> part_shift) * part_ld + row].x - st.x) * c) * inv);
-            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-            uint32_t g[4];
+            const float f = a * (exp2_approx((top[v] - st.x) * c) * inv);
+            const uint32_t w[4] = {raw[v].x, raw[v].y, raw[v].z, raw[v].w};
+            float g[8];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-                const __nv_bfloat162 h = __floats2bfloat162_rn(v.x * f, v.y * f);
-                g[e] = *reinterpret_cast<const uint32_t*>(&h);
+                const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+                g[2 * e] = t.x * f;
+                g[2 * e + 1] = t.y * f;
             }
-            o = make_uint4(g[0], g[1], g[2], g[3]);
+            o = pack_bf16x8(g);
         }
         *reinterpret_cast<uint4*>(gr + col) = o;
     }
     if (!live) return;
     __syncthreads();
+    const float* z = tg.z_sel + static_cast<size_t>(i) * tg.n_ids;
     for (uint32_t k = threadIdx.x; k < tg.n_ids; k += 256) {
-        const size_t at = static_cast<size_t>(row) * tg.n_ids + k;
+        const size_t at = static_cast<size_t>(r) * tg.n_ids + k;
         const uint32_t id = tg.ids[at];
         if (id - c0 >= kGradCols || id >= tg.vocab) continue;
         const float q = tg.q ? tg.q[at] : 1.0f;
         if (q < 0.0f) continue;
-        gr[id] = __float2bfloat16_rn(a * (exp2_approx((tg.z_sel[at] - st.x) * c) * inv - q));
+        gr[id] = __float2bfloat16_rn(a * (exp2_approx((z[k] - st.x) * c) * inv - q));
     }
 }
+
 
 // Programmatic launch: a kernel's blocks may be placed while the one before drains; every kernel here waits for it before it
 // touches memory.
@@ -416,6 +520,9 @@ struct Plan {
     uint64_t part_ld;
     uint64_t ldu;
     bool copy_x, copy_w;
+    bool gather;                       // the products run over the rows with a target alone
+    uint64_t ld_dxg;
+    uint64_t row_of, place_of, count, dxg;
     uint64_t ldx, ldw;                 // pitches of the operands as the products read them
     uint64_t w_rows, w_cols;
     bool acc_dw;                       // bf16 gradient of the head over several pieces: summed in f32 in the scratch
@@ -426,20 +533,24 @@ struct Plan {
 
 bool tma_ok(uint64_t ptr, uint64_t ld) { return ptr % 16 == 0 && ld % 8 == 0; }
 
-InnerGemm dx_gemm(const t0b_linear_loss& d, const Plan& p, uint64_t u, uint64_t w, uint32_t r0, uint32_t n) {
+InnerGemm dx_gemm(const t0b_linear_loss& d, const Plan& p, uint64_t u, uint64_t w, uint64_t base, uint32_t r0, uint32_t n) {
     InnerGemm g{};
+    const uint64_t out = p.gather ? base + p.dxg : d.dx, ld = p.gather ? p.ld_dxg : d.lddx;
+    if (p.gather) { g.dyn_rows = base + p.count; g.dyn_off = static_cast<int>(r0); }
     g.trans_a = 0;
     g.trans_b = d.trans_w ? 0 : 1;
     g.a = u; g.b = w;
-    g.c = d.dx + static_cast<uint64_t>(r0) * d.lddx * (d.dx_dtype == T0B_OUT_BF16 ? 2 : 4);
+    g.c = out + static_cast<uint64_t>(r0) * ld * (d.dx_dtype == T0B_OUT_BF16 ? 2 : 4);
     g.m = n; g.n = d.dim; g.k = d.vocab;
-    g.lda = p.ldu; g.ldb = p.ldw; g.ldc = d.lddx;
+    g.lda = p.ldu; g.ldb = p.ldw; g.ldc = ld;
     g.out_bf16 = d.dx_dtype == T0B_OUT_BF16;
     return g;
 }
 
-InnerGemm dw_gemm(const t0b_linear_loss& d, const Plan& p, uint64_t u, uint64_t x, uint64_t acc, uint32_t r0, uint32_t n) {
+InnerGemm dw_gemm(const t0b_linear_loss& d, const Plan& p, uint64_t u, uint64_t x, uint64_t base, uint32_t r0, uint32_t n) {
     InnerGemm g{};
+    const uint64_t acc = base + p.acc;
+    if (p.gather) { g.dyn_rows = base + p.count; g.dyn_off = static_cast<int>(r0); g.dyn_k = 1; }
     const uint64_t xr = x + static_cast<uint64_t>(r0) * p.ldx * 2;
     g.trans_a = 1;
     g.trans_b = 0;
@@ -472,7 +583,9 @@ Plan make_plan(t0b_ctx* ctx, const t0b_linear_loss& d, uint32_t n_ids, bool teac
     p.head = head_plan(ctx, p.piece, d.vocab, d.dim);
     p.parts = (d.vocab + p.head.part_cols - 1) / p.head.part_cols;
     p.part_ld = (p.piece + 31ull) / 32 * 32;
-    p.copy_x = p.grads || d.x_dtype != T0B_OUT_BF16 || !tma_ok(d.x, d.ldx);
+    // Up to a tile of rows costs the same with and without the rows that are left out.
+    p.gather = d.rows > 256;
+    p.copy_x = p.gather || p.grads || d.x_dtype != T0B_OUT_BF16 || !tma_ok(d.x, d.ldx);
     p.ldx = p.copy_x ? round8(d.dim) : d.ldx;
     p.w_rows = d.trans_w ? d.vocab : d.dim;
     p.w_cols = d.trans_w ? d.dim : d.vocab;
@@ -493,6 +606,13 @@ Plan make_plan(t0b_ctx* ctx, const t0b_linear_loss& d, uint32_t n_ids, bool teac
     }
     if (p.copy_x) p.x = take(rows * p.ldx * 2);
     if (p.copy_w) p.w = take(p.w_rows * p.ldw * 2);
+    if (p.gather) {
+        p.row_of = take(rows * 4);
+        p.place_of = take(rows * 4);
+        p.count = take(4);
+        p.ld_dxg = round8(d.dim);
+        if (p.dx) p.dxg = take(rows * p.ld_dxg * (d.dx_dtype == T0B_OUT_BF16 ? 2 : 4));
+    }
     p.part = take(p.parts * p.part_ld * 8);
     if (p.grads) p.u = take(p.piece * p.ldu * 2);
     if (p.acc_dw) p.acc = take(p.w_rows * p.ld_acc * 4);
@@ -500,7 +620,7 @@ Plan make_plan(t0b_ctx* ctx, const t0b_linear_loss& d, uint32_t n_ids, bool teac
     for (uint32_t r0 = 0; p.grads && r0 < d.rows; r0 += p.piece) {
         const uint32_t n = std::min(p.piece, d.rows - r0);
         if (r0 > 0 && n == p.piece) continue;   // like the first
-        if (p.dx) p.slab_bytes = std::max<uint64_t>(p.slab_bytes, inner_gemm_slab_bytes(ctx, dx_gemm(d, p, 256, 256, r0, n)));
+        if (p.dx) p.slab_bytes = std::max<uint64_t>(p.slab_bytes, inner_gemm_slab_bytes(ctx, dx_gemm(d, p, 256, 256, 256, r0, n)));
     }
     p.slabs = take(p.slab_bytes);
     p.total = std::max<uint64_t>(off, 256);
@@ -583,7 +703,13 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
     int launched = 0;
 
     const uint64_t x = p.copy_x ? base + p.x : d.x, w = p.copy_w ? base + p.w : d.w;
-    __nv_bfloat16* x_out = reinterpret_cast<__nv_bfloat16*>(p.copy_x ? base + p.x : 0);
+    __nv_bfloat16* xg = reinterpret_cast<__nv_bfloat16*>(base + p.x);
+    __nv_bfloat16* x_out = p.copy_x && !p.gather ? xg : nullptr;
+    uint32_t* row_of = p.gather ? reinterpret_cast<uint32_t*>(base + p.row_of) : nullptr;
+    uint32_t* place_of = reinterpret_cast<uint32_t*>(base + p.place_of);
+    int* count = p.gather ? reinterpret_cast<int*>(base + p.count) : nullptr;
+    float* losses = reinterpret_cast<float*>(d.losses);
+    float* lse = reinterpret_cast<float*>(d.lse);
     const bool x16 = d.x_dtype == T0B_OUT_BF16;
     const __nv_bfloat16* xb = reinterpret_cast<const __nv_bfloat16*>(d.x);
     const float* xf = reinterpret_cast<const float*>(d.x);
@@ -600,12 +726,20 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
         if (x16) words(teacher_words_kernel<__nv_bfloat16>, xb);
         else words(teacher_words_kernel<float>, xf);
         ++launched;
-    } else if (p.copy_x) {
+    } else if (x_out) {
         const uint32_t blocks = lin_blocks(ctx, d.rows * (p.ldx / 8));
         const uint32_t* targets = reinterpret_cast<const uint32_t*>(te.ids);
         if (x16) launch(ctx, pack_rows_kernel<__nv_bfloat16>, blocks, 256, 0, xb, d.ldx, x_out, static_cast<uint32_t>(p.ldx), d.rows, d.dim, targets, d.vocab);
         else launch(ctx, pack_rows_kernel<float>, blocks, 256, 0, xf, d.ldx, x_out, static_cast<uint32_t>(p.ldx), d.rows, d.dim, targets, d.vocab);
         ++launched;
+    }
+    if (p.gather) {
+        launch(ctx, live_rows_kernel, 1, 1024, 0, teacher ? nullptr : reinterpret_cast<const uint32_t*>(te.ids),
+               teacher ? reinterpret_cast<const uint32_t*>(base + p.live) : nullptr, d.vocab, d.rows, row_of, place_of, count, losses, lse, ctx->status_dev);
+        const uint32_t blocks = lin_blocks(ctx, d.rows * (p.ldx / 8));
+        if (x16) launch(ctx, gather_rows_kernel<__nv_bfloat16>, blocks, 256, 0, xb, d.ldx, xg, static_cast<uint32_t>(p.ldx), d.rows, d.dim, row_of, count);
+        else launch(ctx, gather_rows_kernel<float>, blocks, 256, 0, xf, d.ldx, xg, static_cast<uint32_t>(p.ldx), d.rows, d.dim, row_of, count);
+        launched += 2;
     }
     if (p.copy_w) {
         launch(ctx, pack_shifted_kernel, lin_blocks(ctx, p.w_rows * ((p.ldw / 8 + 31) / 32 * 32)), 256, 0, reinterpret_cast<const __nv_bfloat16*>(d.w), d.ldw,
@@ -617,15 +751,18 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
     for (uint32_t r0 = 0; r0 < d.rows; r0 += p.piece) {
         const uint32_t n = std::min(p.piece, d.rows - r0);
         Targets tg{};
-        tg.ids = reinterpret_cast<const uint32_t*>(teacher ? base + p.ids : te.ids) + static_cast<size_t>(r0) * te.topk;
+        tg.ids = reinterpret_cast<const uint32_t*>(teacher ? base + p.ids : te.ids);
         if (teacher) {
-            tg.q = reinterpret_cast<const float*>(base + p.q) + static_cast<size_t>(r0) * te.topk;
-            tg.entropy = reinterpret_cast<const float*>(base + p.entropy) + r0;
-            tg.live = reinterpret_cast<const uint32_t*>(base + p.live) + r0;
+            tg.q = reinterpret_cast<const float*>(base + p.q);
+            tg.entropy = reinterpret_cast<const float*>(base + p.entropy);
+            tg.live = reinterpret_cast<const uint32_t*>(base + p.live);
         }
-        tg.z_sel = reinterpret_cast<const float*>(base + p.z_sel) + static_cast<size_t>(r0) * te.topk;
+        tg.z_sel = reinterpret_cast<const float*>(base + p.z_sel);
         tg.n_ids = te.topk;
         tg.vocab = d.vocab;
+        tg.row_of = row_of;
+        tg.count = count;
+        tg.row0 = r0;
         HeadGemm hg{};
         hg.plan = p.head;
         hg.x = x + static_cast<uint64_t>(r0) * p.ldx * 2;
@@ -634,46 +771,54 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
         hg.rows = n; hg.dim = d.dim; hg.vocab = d.vocab; hg.trans_w = d.trans_w;
         hg.c = c;
         hg.part = base + p.part; hg.part_ld = p.part_ld;
-        hg.ids = reinterpret_cast<uint64_t>(tg.ids);
+        hg.ids = reinterpret_cast<uint64_t>(tg.ids) + (row_of ? 0 : static_cast<uint64_t>(r0) * te.topk * 4);
+        hg.row_of = row_of ? reinterpret_cast<uint64_t>(row_of + r0) : 0;
+        hg.dyn_rows = reinterpret_cast<uint64_t>(count);
+        hg.dyn_off = static_cast<int>(r0);
         hg.z_sel = reinterpret_cast<uint64_t>(tg.z_sel);
         hg.n_ids = te.topk;
         hg.u = p.grads ? base + p.u : 0;
         hg.ldu = p.ldu;
         rc = head_gemm(ctx, hg);
         if (rc != T0B_OK) return rc;
-        float2* stats = reinterpret_cast<float2*>(base + p.stats) + r0;
+        float2* stats = reinterpret_cast<float2*>(base + p.stats);
         launch(ctx, join_parts_kernel, (n + 31) / 32, 1024, 0, reinterpret_cast<const float2*>(base + p.part), p.part_ld, p.parts, n, c, inv_t, tg, stats,
-               d.losses ? reinterpret_cast<float*>(d.losses) + r0 : nullptr, d.lse ? reinterpret_cast<float*>(d.lse) + r0 : nullptr, ctx->status_dev);
+               losses, lse, ctx->status_dev);
         ++launched;
         if (!p.grads) continue;
-        // gridDim.y is limited to 65535 rows a launch.
-        for (uint32_t y0 = 0; y0 < n; y0 += 65535u) {
-            const uint32_t ny = std::min(65535u, n - y0);
-            Targets t2 = tg;
-            t2.ids += static_cast<size_t>(y0) * te.topk;
-            if (teacher) { t2.q += static_cast<size_t>(y0) * te.topk; t2.entropy += y0; t2.live += y0; }
-            t2.z_sel += static_cast<size_t>(y0) * te.topk;
-            launch(ctx, dz_kernel, dim3(static_cast<uint32_t>((p.ldu + kGradCols - 1) / kGradCols), ny), 256, 0,
-                reinterpret_cast<__half*>(base + p.u) + y0 * p.ldu, p.ldu, ny, reinterpret_cast<const float2*>(base + p.part) + y0, p.part_ld, part_shift,
-                stats + y0, d.row_weights ? reinterpret_cast<const float*>(d.row_weights) + r0 + y0 : nullptr, d.scale * inv_t, c, t2);
+        for (uint32_t y0 = 0; y0 < n; y0 += 65535u) {   // gridDim.y is limited to 65535
+            launch(ctx, dz_kernel, dim3(static_cast<uint32_t>((p.ldu + kGradCols - 1) / kGradCols), std::min(65535u, n - y0)), 256, 0,
+                   reinterpret_cast<__half*>(base + p.u), p.ldu, n, y0, reinterpret_cast<const float2*>(base + p.part), p.part_ld, part_shift, stats,
+                   reinterpret_cast<const float*>(d.row_weights), d.scale * inv_t, c, tg);
             ++launched;
         }
         rc = check_cuda(ctx, cudaGetLastError(), what);
         if (rc != T0B_OK) return rc;
         if (p.dx) {
-            InnerGemm g = dx_gemm(d, p, base + p.u, w, r0, n);
+            InnerGemm g = dx_gemm(d, p, base + p.u, w, base, r0, n);
             g.slabs = base + p.slabs;
             g.slab_bytes = p.slab_bytes;
             rc = inner_gemm(ctx, g);
             if (rc != T0B_OK) return rc;
         }
         if (p.dw) {
-            InnerGemm g = dw_gemm(d, p, base + p.u, x, base + p.acc, r0, n);
+            InnerGemm g = dw_gemm(d, p, base + p.u, x, base, r0, n);
             g.slabs = base + p.slabs;
             g.slab_bytes = p.slab_bytes;
             rc = inner_gemm(ctx, g);
             if (rc != T0B_OK) return rc;
         }
+    }
+    if (p.gather && p.dx) {
+        const bool dx16 = d.dx_dtype == T0B_OUT_BF16;
+        const uint32_t blocks = lin_blocks(ctx, d.rows * (p.ld_dxg / (dx16 ? 8 : 4)));
+        if (dx16)
+            launch(ctx, spread_rows_kernel<uint16_t>, blocks, 256, 0, reinterpret_cast<const uint16_t*>(base + p.dxg), static_cast<uint32_t>(p.ld_dxg),
+                   reinterpret_cast<uint16_t*>(d.dx), d.lddx, d.rows, d.dim, place_of);
+        else
+            launch(ctx, spread_rows_kernel<float>, blocks, 256, 0, reinterpret_cast<const float*>(base + p.dxg), static_cast<uint32_t>(p.ld_dxg),
+                   reinterpret_cast<float*>(d.dx), d.lddx, d.rows, d.dim, place_of);
+        ++launched;
     }
     if (p.acc_dw) {
         launch(ctx, round_rows_kernel, lin_blocks(ctx, p.w_rows * ((p.w_cols + 7) / 8)), 256, 0,

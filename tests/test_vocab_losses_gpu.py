@@ -83,7 +83,7 @@ def losses_and_dz(th, z, q, ent, live, temperature, row_scale):
 
 
 def check_linear(th, art, rows, dim, vocab, trans_w, *, topk=0, temperature=1.0, grads=True, x_dtype=OUT_BF16, gdt=OUT_BF16, weights=True, ignore=True,
-                 piece_rows=0, ldx_pad=0, ldw_pad=0, ragged=True, big=1.0, offset=0):
+                 piece_rows=0, ldx_pad=0, ldw_pad=0, ragged=True, big=1.0, offset=0, keep=None):
     g = th.Generator(device="cuda")
     g.manual_seed(rows * 7919 + dim * 31 + vocab)
     w_rows, w_cols = (vocab, dim) if trans_w else (dim, vocab)
@@ -93,25 +93,30 @@ def check_linear(th, art, rows, dim, vocab, trans_w, *, topk=0, temperature=1.0,
     xt = th.bfloat16 if x_dtype == OUT_BF16 else th.float32
     x = (th.randn((rows, dim + ldx_pad), device="cuda", generator=g) * 2 * big).to(xt)[:, :dim]
     ldx, ldw = dim + ldx_pad, w_cols + ldw_pad
+    keep = None if keep is None else th.tensor([r in keep for r in range(rows)], device="cuda")
     if topk:
         ids, teacher = make_teacher(th, rows, topk, vocab, rows + topk, ragged)
+        if keep is not None:
+            ids[~keep] = -1
         q, ent, live = target_rows(th, ids, teacher, temperature, vocab)
     else:
         tgt = th.randint(0, vocab, (rows,), device="cuda", generator=g)
         x = x.clone() if not ldx_pad else x
         if ignore:
             tgt[::3] = -1
+        if keep is not None:
+            tgt[~keep] = -1
         live = tgt >= 0
         q = th.zeros((rows, vocab), dtype=th.float64, device="cuda")
         q[th.arange(rows, device="cuda"), tgt.clamp_min(0)] = live.double()
         ent = th.zeros(rows, dtype=th.float64, device="cuda")
         tgt = tgt.to(th.int32)
-    if ignore and grads:
+    if (ignore or keep is not None) and (grads or rows > 256):
         x[~live] = math.nan                                                     # a row that is left out may hold anything
     rw = th.rand(rows, device="cuda", generator=g) * 2 if weights else None
     scale = 1.0 / rows
     row_scale = (rw.double() if weights else th.ones(rows, device="cuda", dtype=th.float64)) * scale
-    xd = x.bfloat16().double().masked_fill(~live[:, None], 0.0) if (ignore and grads) else x.bfloat16().double()
+    xd = x.bfloat16().double().masked_fill(~live[:, None], 0.0)
     z = xd @ wd.t()
     losses_ref, dz, p, lse_ref = losses_and_dz(th, z, q, ent, live, temperature, row_scale)
     losses, lse = th.full((rows,), 7.0, device="cuda"), th.full((rows,), 7.0, device="cuda")
@@ -190,6 +195,16 @@ def test_linear_types(th, art, x_dtype, gdt, trans_w):
 def test_linear_in_pieces_of_rows(th, art, vocab, gdt, trans_w):
     check_linear(th, art, 300, 128, vocab, trans_w, gdt=gdt, piece_rows=128)
     check_linear(th, art, 100, 60, vocab, trans_w, gdt=gdt, piece_rows=33, topk=6)
+
+
+@pytest.mark.parametrize("trans_w", [False, True])
+@pytest.mark.parametrize("keep", [[], [699], [5, 64, 300], list(range(64)), list(range(600, 665)), list(range(700))])
+def test_linear_rows_left_out(th, art, keep, trans_w):
+    """Products run over the rows with a target alone once there is more than a tile of rows: none, one, whole 64-row blocks."""
+    for piece_rows in (0, 33, 256):
+        check_linear(th, art, 700, 72, 200, trans_w, keep=keep, piece_rows=piece_rows, ignore=len(keep) < 700)
+        check_linear(th, art, 700, 64, 136, trans_w, keep=keep, piece_rows=piece_rows, topk=3, gdt=OUT_F32, ragged=False)
+    check_linear(th, art, 700, 72, 200, trans_w, keep=keep, grads=False)
 
 
 @pytest.mark.parametrize("trans_w", [False, True])
