@@ -68,6 +68,10 @@ constexpr int kMaxDst = 8;
 // gradient follows, u = exp((z - max) / T) in fp16 through the third tensor map.  u lies in [0, 1] with at least one 1 in
 // every part, so fp16 keeps 11 significant bits of everything above 2^-14 of the part's largest exponential and is off by
 // at most 2^-25 of it below; bf16 would lose three bits on the probabilities that carry the gradient.
+// The tensor core's own sums drop what falls below the accumulator's last bit, at every 16 products; over a long contraction
+// that is a bias.  So a row's logit is summed in pieces of 1024 products, in alternating accumulators, and the pieces are
+// added in the epilogue's registers, behind the next piece's products.
+constexpr int kHeadSumKb = 16;
 struct HeadParams {
     float2* part;            // [parts][part_ld]
     long long part_ld;       // rows, padded
@@ -618,7 +622,20 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                     if (!bounded_wait(tempty_bar(acc), slot_ph[acc] ^ 1u, ctl, DEV_TIMEOUT_TMEM_EMPTY)) { ok = false; break; }
                     ptx::tc_fence_after();
                 }
+                int kb_acc = wi.kb_begin;   // first K block of the sum that the accumulator holds
                 for (int kb = wi.kb_begin; kb < wi.kb_end; ++kb) {
+                    if constexpr (HEAD != 0) {
+                        if (kb - kb_acc == kHeadSumKb) {
+                            // Hand the partial sum over and go on in the other slot (HeadParams).
+                            if constexpr (CG == 1) ptx::mma_commit(tfull_bar(acc));
+                            else ptx::mma_commit_pair(tfull_bar(acc), 0x3);
+                            slot_ph[acc] ^= 1u;
+                            acc ^= 1;
+                            if (!bounded_wait(tempty_bar(acc), slot_ph[acc] ^ 1u, ctl, DEV_TIMEOUT_TMEM_EMPTY)) { ok = false; break; }
+                            ptx::tc_fence_after();
+                            kb_acc = kb;
+                        }
+                    }
                     if (!bounded_wait(full_bar(s), ph, ctl, DEV_TIMEOUT_FULL)) { ok = false; break; }
                     if (w == cluster_id && kb == wi.kb_begin) {
                         T0B_STAMP(4);
@@ -629,7 +646,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                     const uint32_t b_addr = a_addr + T::kATileBytes;
 #pragma unroll
                     for (int k = 0; k < kBk / kUmmaK; ++k) {
-                        const uint32_t acc_flag = (kb > wi.kb_begin || k > 0) ? 1u : 0u;
+                        const uint32_t acc_flag = (kb > kb_acc || k > 0) ? 1u : 0u;
                         if constexpr (ND == 1) {
                             // One A slice, two B slices: the second MMA takes A from the collector.
                             const uint64_t adesc = make_smem_desc(a_addr + k * a_kstep, a_lbo, a_sbo);
@@ -723,23 +740,50 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                 // Softmax epilogue: the warp's columns come into registers in one go (the accumulator is free again at
                 // once), so the maximum is known before the first exponential and nothing is rescaled.
                 constexpr int W = T::kPartCols;
-                uint32_t raw[W];
+                float v[W];
+                bool summed = true;   // warp-uniform
+                for (int kb = wi.kb_begin; kb < wi.kb_end; kb += kHeadSumKb) {
+                    if (kb > wi.kb_begin) {
+                        if (!bounded_wait_warp(tfull_bar(slot), slot_phase, ctl, DEV_TIMEOUT_TMEM_FULL, lane, p.wait_hint_ns)) {
+                            summed = false;
+                            break;
+                        }
+                        ptx::tc_fence_after();
+                    }
+                    const uint32_t t_cols = tmem_base + static_cast<uint32_t>(slot * BN + c_begin * 32) + (static_cast<uint32_t>(q * 32) << 16);
+                    if (kb == wi.kb_begin) {
+                        uint32_t(*raw)[32] = reinterpret_cast<uint32_t(*)[32]>(v);
 #pragma unroll
-                for (int c = 0; c < kChunks; ++c) ptx::tmem_ld_32x32(t_row + (c_begin + c) * 32, *reinterpret_cast<uint32_t(*)[32]>(raw + 32 * c));
+                        for (int c = 0; c < kChunks; ++c) ptx::tmem_ld_32x32(t_cols + c * 32, raw[c]);
 #pragma unroll
-                for (int c = 0; c < kChunks; ++c) ptx::tmem_ld_wait_regs(*reinterpret_cast<uint32_t(*)[32]>(raw + 32 * c));
-                ptx::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    if constexpr (CG == 1) ptx::mbar_arrive(tempty_bar(slot));
-                    else ptx::mbar_arrive_cluster(ptx::mapa(tempty_bar(slot), 0));
+                        for (int c = 0; c < kChunks; ++c) ptx::tmem_ld_wait_regs(raw[c]);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < W / 16; ++c) {
+                            uint32_t more[16];
+                            ptx::tmem_ld_32x16(t_cols + c * 16, more);
+                            ptx::tmem_ld_wait_regs16(more);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) v[16 * c + j] += __uint_as_float(more[j]);
+                        }
+                    }
+                    ptx::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if constexpr (CG == 1) ptx::mbar_arrive(tempty_bar(slot));
+                        else ptx::mbar_arrive_cluster(ptx::mapa(tempty_bar(slot), 0));
+                    }
+                    slot ^= 1;
+                    if (slot == 0) slot_phase ^= 1u;
                 }
+                if (!summed) break;
                 const int col0 = n_base + c_begin * 32;
                 const int ncols = p.N - col0;
                 if (row0 < ext.M && ncols > 0) {   // warp-uniform
-                    float v[W];
+                    if (ncols < W) {
 #pragma unroll
-                    for (int j = 0; j < W; ++j) v[j] = (j < ncols) ? __uint_as_float(raw[j]) : -INFINITY;
+                        for (int j = 0; j < W; ++j) v[j] = (j < ncols) ? v[j] : -INFINITY;
+                    }
                     const HeadParams& hp = p.head;
                     if (hp.n_ids > 0) {
                         // The columns this row asks for: ids ascend, so the ones of this part are consecutive.
@@ -798,8 +842,6 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                         }
                     }
                 }
-                slot ^= 1;
-                if (slot == 0) slot_phase ^= 1u;
                 continue;
             }
             // The TMEM read of chunk c+1 is in flight while chunk c is transposed and stored.

@@ -695,7 +695,12 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
         return rc != T0B_OK ? rc : finish(ctx, async, what, 0);
     }
     const bool teacher = te.logits != 0;
-    const Plan p = make_plan(ctx, d, te.topk, teacher);
+    Plan p = make_plan(ctx, d, te.topk, teacher);
+    if (d.scratch && d.scratch_bytes < p.total && d.scratch_bytes >= p.slabs) {
+        // Sized before a t0b_tune that wants more slabs: the product that does not fit them is not split.
+        p.slab_bytes = d.scratch_bytes - p.slabs;
+        p.total = d.scratch_bytes;
+    }
     uint64_t base = 0;
     int32_t rc = get_scratch(ctx, what, d, p.total, &base);
     if (rc != T0B_OK) return rc;

@@ -23,9 +23,10 @@ from __future__ import annotations
 from dataclasses import dataclass, field
 from typing import List, Optional
 
+import ctypes as C
 import os
 
-from ._lib import lib
+from ._lib import LinearLossC, lib
 from .gpu_context import OUT_BF16, OUT_F32, GpuRuntime
 
 
@@ -112,9 +113,12 @@ class MlpTrainer:
     """One data-parallel replica.  `rows` is this rank's share of the batch, `rows_total` the global batch."""
 
     def __init__(self, rt: GpuRuntime, cfg: MlpConfig, rows: int, rows_total: Optional[int] = None, group=None,
-                 seed: int = 100, shard_optimizer: bool = False, autotune: bool = True, local_only: bool = False):
+                 seed: int = 100, shard_optimizer: bool = False, autotune: bool = True, local_only: bool = False,
+                 keep_logits: bool = True):
         """local_only: a single-rank replica even while a process group is up (no gradient exchange) -- the one-rank
-        side of a data-parallel equivalence check."""
+        side of a data-parallel equivalence check.
+        keep_logits=False: the output layer, its loss and both their gradients in one `t0b_linear_ce` call, without the
+        [rows, n_classes] f32 logits (the same step up to rounding; for class counts whose logits do not fit)."""
         import torch
         import torch.distributed as dist
 
@@ -181,8 +185,10 @@ class MlpTrainer:
         self.x16 = torch.empty((B, cfg.d_in), dtype=bf16, device=self.dev)
         self.z = [torch.empty((B, h), dtype=f32, device=self.dev) for h in cfg.hidden]        # Linear outputs
         self.h16 = [torch.empty((B, h), dtype=bf16, device=self.dev) for h in cfg.hidden]     # bf16 layer outputs
-        self.logits = torch.empty((B, cfg.n_classes), dtype=f32, device=self.dev)
-        self.dlogits16 = torch.empty((B, cfg.n_classes), dtype=bf16, device=self.dev)
+        self.keep_logits = keep_logits
+        if keep_logits:
+            self.logits = torch.empty((B, cfg.n_classes), dtype=f32, device=self.dev)
+            self.dlogits16 = torch.empty((B, cfg.n_classes), dtype=bf16, device=self.dev)
         self.losses = torch.empty(B, dtype=f32, device=self.dev)
         self.dh = torch.empty((B, max(cfg.hidden)), dtype=f32, device=self.dev)
         self.dz16 = torch.empty((B, max(cfg.hidden)), dtype=bf16, device=self.dev)
@@ -193,6 +199,14 @@ class MlpTrainer:
         self._updates = {}
         if autotune:
             self._tune_gemms()
+        if not keep_logits:
+            k_out, V = dims[-1]
+            self._head = LinearLossC(x=self.h16[-1].data_ptr(), w=self.w16[nl - 1].data_ptr(), ldx=k_out, ldw=V, losses=self.losses.data_ptr(),
+                                     dx=self.dh.data_ptr(), dw=self.dw[nl - 1].data_ptr(), lddx=k_out, lddw=V, rows=B, dim=k_out, vocab=V,
+                                     x_dtype=OUT_BF16, dx_dtype=OUT_F32, dw_dtype=OUT_F32, scale=1.0 / float(self.rows_total))
+            nbytes = self.L.t0b_linear_loss_scratch_bytes(rt.handle, C.byref(self._head), 0)
+            self._head_scratch = torch.empty(nbytes, dtype=torch.uint8, device=self.dev)
+            self._head.scratch, self._head.scratch_bytes = self._head_scratch.data_ptr(), nbytes
 
     def _tune_gemms(self):
         """Measure the tile candidates for every GEMM shape of the step once (the reference's `auto_gemm` does the same
@@ -206,8 +220,9 @@ class MlpTrainer:
             shapes.add((B, k, n, False, True))           # dX
             k = n
         V = cfg.n_classes
-        shapes.add((B, V, k, False, False))
-        shapes.add((k // len(self._layer_units[-1]), V, B, True, False))
+        if self.keep_logits:
+            shapes.add((B, V, k, False, False))
+            shapes.add((k // len(self._layer_units[-1]), V, B, True, False))
         shapes.add((B, k, V, False, True))
         done = self.rt.__dict__.setdefault("_mlp_tuned_shapes", set())   # a second trainer on this runtime measures nothing twice
         for shape in sorted(shapes - done):
@@ -250,25 +265,17 @@ class MlpTrainer:
             self._ck(L.t0b_rmsnorm_silu_fwd(h, self.z[l].data_ptr(), self.gamma[l].data_ptr(), self.h16[l].data_ptr(), 0, B, n,
                                             cfg.eps, 1))
             inp, k = self.h16[l], n
-        V = cfg.n_classes
         self._wait_layer(nh)
-        self._gemm(inp, self.w16[nh], self.logits, B, V, k, False, False, k, V)
-        _nvtx_pop()
-        # loss and its gradient, stored directly as the bf16 operand of the two GEMMs that follow
-        _nvtx_push("t0b.mlp.loss")
-        self._ck(L.t0b_softmax_ce_bf16(h, self.logits.data_ptr(), targets.data_ptr(), self.losses.data_ptr(),
-                                       self.dlogits16.data_ptr(), B, V, V, scale, 1))
-        _nvtx_pop()
-        # backward
-        _nvtx_push("t0b.mlp.backward")
-        # dW_out[k, V] = h_last^T [k, B] * dlogits [B, V]: A stored [B, k] read transposed
-        ids = self._layer_units[nh]
-        per = k // len(ids)                     # rows of dW_out per panel = columns of h_last
-        for pnl, u in enumerate(ids):
-            self._gemm(inp[:, pnl * per:], self.dlogits16, self.dw[nh][pnl * per:], per, V, B, True, False, k, V)
-            self._start_reduce(u)
-        # dh_last[B, k] = dlogits [B, V] * W_out^T: B operand stored [k, V] = [N_gemm, K_gemm]
-        self._gemm(self.dlogits16, self.w16[nh], self.dh, B, k, V, False, True, V, V)
+        if self.keep_logits:
+            self._output_layer(inp, targets, k, scale)
+        else:
+            _nvtx_pop()
+            _nvtx_push("t0b.mlp.output")
+            self._ck(L.t0b_linear_ce(h, C.byref(self._head), targets.data_ptr(), 1))
+            for u in self._layer_units[nh]:
+                self._start_reduce(u)
+            _nvtx_pop()
+            _nvtx_push("t0b.mlp.backward")
         for l in range(nh - 1, -1, -1):
             n = cfg.hidden[l]
             k = cfg.hidden[l - 1] if l > 0 else cfg.d_in
@@ -287,6 +294,28 @@ class MlpTrainer:
         _nvtx_push("t0b.mlp.grad_exchange_wait")
         self._finish_reduce()
         _nvtx_pop()
+
+    def _output_layer(self, inp, targets, k, scale):
+        """Logits, loss and the output layer's gradients through the [rows, n_classes] buffers."""
+        cfg, B, L, h = self.cfg, self.rows, self.L, self.rt.handle
+        nh, V = len(cfg.hidden), cfg.n_classes
+        self._gemm(inp, self.w16[nh], self.logits, B, V, k, False, False, k, V)
+        _nvtx_pop()
+        # loss and its gradient, stored directly as the bf16 operand of the two GEMMs that follow
+        _nvtx_push("t0b.mlp.loss")
+        self._ck(L.t0b_softmax_ce_bf16(h, self.logits.data_ptr(), targets.data_ptr(), self.losses.data_ptr(),
+                                       self.dlogits16.data_ptr(), B, V, V, scale, 1))
+        _nvtx_pop()
+        # backward
+        _nvtx_push("t0b.mlp.backward")
+        # dW_out[k, V] = h_last^T [k, B] * dlogits [B, V]: A stored [B, k] read transposed
+        ids = self._layer_units[nh]
+        per = k // len(ids)                     # rows of dW_out per panel = columns of h_last
+        for pnl, u in enumerate(ids):
+            self._gemm(inp[:, pnl * per:], self.dlogits16, self.dw[nh][pnl * per:], per, V, B, True, False, k, V)
+            self._start_reduce(u)
+        # dh_last[B, k] = dlogits [B, V] * W_out^T: B operand stored [k, V] = [N_gemm, K_gemm]
+        self._gemm(self.dlogits16, self.w16[nh], self.dh, B, k, V, False, True, V, V)
 
     def _start_reduce(self, unit: int):
         """Start the exchange of one unit's gradient: all-reduce (replicated optimizer) or reduce-scatter (sharded)."""

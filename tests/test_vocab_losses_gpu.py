@@ -341,3 +341,294 @@ def test_topk_distill_same_word_twice(th, art):
     assert ((losses.double() - losses_ref).abs() <= 1e-4).all()      # |z| < 40: 2 ez = 2 * 16 * 2^-23 * 16 * 16 < 1e-3 / 10
     edz = UB * dz.abs() + p * (UH + 1e-4) / rows + 1e-8
     assert ((dx.double() - dz @ w.double()).abs() <= edz @ w.double().abs() + 1e-5).all()
+
+
+# ------------------------------------------------------------------------------------------- in a user's program
+
+@pytest.mark.parametrize("rows,d,V", [(64, 256, 1000), (300, 128, 2048)])
+def test_mlp_step_without_logits(th, rows, d, V):
+    """MlpTrainer(keep_logits=False): the step of the trainer that keeps them, up to the roundings of the logits' gradient."""
+    from t0_gpu_b200.mlp import MlpConfig, MlpTrainer
+
+    rt = t.GpuRuntime()
+    cfg = MlpConfig(d_in=d, hidden=[d, d], n_classes=V)
+    g = th.Generator(device="cuda")
+    g.manual_seed(5)
+    s = th.cuda.Stream()
+    with th.cuda.stream(s):
+        x = th.randn((rows, d), device="cuda", generator=g)
+        targets = th.randint(0, V, (rows,), device="cuda", generator=g).to(th.int32)
+        a = MlpTrainer(rt, cfg, rows, seed=3, autotune=False)
+        b = MlpTrainer(rt, cfg, rows, seed=3, autotune=False, keep_logits=False)
+        a.forward_backward(x, targets)
+        b.forward_backward(x, targets)
+        rt.synchronize()
+        h, w, dz = a.h16[-1].double(), a.w16[-1].double(), a.dlogits16.double()
+        # |z| <= sum |h w|; a loss is a difference of logarithms of sums of exponentials of such (bounds at the top of this file)
+        ez = d * U32 * (h.abs() @ w.abs()).amax(1)
+        assert ((a.losses - b.losses).abs() <= 4 * ez + 64 * U32 * (1 + a.losses.abs())).all()
+        # dz: rounded to bf16 on both sides, and through fp16 on one, of exponentials that differ by the logits' error
+        p = th.softmax(a.logits.double(), 1)
+        e = 2 * UB * dz.abs() + (p * (UH + 4 * ez[:, None] + 2.0 ** -18) + 2.0 ** -24) / rows
+        bound = h.abs().t() @ e + rows * U32 * (h.abs().t() @ dz.abs())
+        assert ((a.dw[-1] - b.dw[-1]).double().abs() <= bound).all()
+        for _ in range(3):
+            b.step(x, targets)
+        assert math.isfinite(b.mean_loss()) and not hasattr(b, "logits")
+    rt.synchronize()
+    rt.close()
+
+
+def test_ops_run_together_with_f32_buffers(rt):
+    """A training step of a student head through ops alone, f32 buffers in and out: cross entropy, distillation from logits
+    that `matmul` made, distillation from hidden states, all on the same head, and an optimizer step on their sum."""
+    rng = np.random.default_rng(3)
+    rows, dim, vocab, topk = 40, 64, 200, 5
+    x = rng.standard_normal((rows, dim)).astype(np.float32)
+    w = (rng.standard_normal((dim, vocab)) / 8).astype(np.float32)
+    tgt = rng.integers(0, vocab, rows).astype(np.uint32)
+    tgt[::7] = ops.NO_WORD
+    ids = np.stack([rng.choice(vocab, topk, replace=False) for _ in range(rows)]).astype(np.uint32)
+    teacher = rng.standard_normal((rows, topk)).astype(np.float32)
+    xb, wb, tb, ib, lb = rt.upload_f32(x), rt.upload_f32(w), rt.upload(tgt), rt.upload(ids), rt.upload_f32(teacher)
+    ce, dx_ce, dw_ce = ops.linear_cross_entropy(rt, xb, wb, tb, rows, dim, vocab)
+    kd, dx_kd, dw_kd = ops.linear_topk_distill(rt, xb, wb, ib, lb, rows, dim, vocab, topk, temperature=2.0, weight_id=77)
+    z, backward = ops.matmul(rt, xb, wb, rows, dim, vocab, weight_id=77)
+    kd2, dz = ops.topk_distill(rt, z, ib, lb, rows, vocab, topk, temperature=2.0)
+    dx2, dw2 = backward(dz)
+    get = lambda b, shape: b.read_as(np.float32, int(np.prod(shape))).reshape(shape)   # noqa: E731
+    assert np.abs(get(kd, rows) - get(kd2, rows)).max() <= 1e-5          # the same logits: 64 products of |x w| < 2, 2^-23 each
+    # both round the same dz to bf16 (and fp16 on one side): 2^-8 + 2^-11 of sum |dz w| each
+    dzn, w16 = np.abs(get(dz, (rows, vocab))), np.abs(w)
+    assert (np.abs(get(dx_kd, (rows, dim)) - get(dx2, (rows, dim))) <= (2 * UB + 2 * UH) * (dzn @ w16.T) * 1.01 + 1e-6).all()
+    assert (np.abs(get(dw_kd, (dim, vocab)) - get(dw2, (dim, vocab))) <= (2 * UB + 2 * UH) * (np.abs(x).T @ dzn) * 1.01 + 1e-6).all()
+    losses, grad = ops.cross_entropy(rt, z, tb, rows, vocab)
+    got = get(ce, rows)
+    assert abs(losses - got.sum() / rows) <= 1e-5 and (got[::7] == 0).all()
+    n = dim * vocab
+    rt._check(t._lib.lib().t0b_residual_add(rt.handle, dw_ce.gpu_addr(), dw_kd.gpu_addr(), n, 1))
+    m, v = rt.alloc_zero(n * 4), rt.alloc_zero(n * 4)
+    ops.adamw_step(rt, wb, dw_ce, m, v, n, 1, weight_id=77)
+    ce2, none_x, none_w = ops.linear_cross_entropy(rt, xb, wb, tb, rows, dim, vocab, grads=False, weight_id=77)
+    assert none_x is None and none_w is None and get(ce2, rows).sum() != got.sum()
+    # the f32 head was converted anew: with and without a cached copy the same
+    ce3, _, _ = ops.linear_cross_entropy(rt, xb, wb, tb, rows, dim, vocab, grads=False)
+    assert np.array_equal(get(ce2, rows), get(ce3, rows))
+
+
+def _ce(art, th, x, w, tgt, **kw):
+    rows, dim = x.shape
+    vocab = w.shape[0]
+    losses, dx, dw = th.empty(rows, device="cuda"), th.empty((rows, dim), device="cuda"), th.empty((vocab, dim), device="cuda")
+    ops.linear_cross_entropy(art, x.data_ptr(), w.data_ptr(), tgt.data_ptr(), rows, dim, vocab, trans_w=True, x_dtype=OUT_BF16, w_dtype=OUT_BF16,
+                             losses=losses.data_ptr(), dx=dx.data_ptr(), dw=dw.data_ptr(), **kw)
+    return losses, dx, dw
+
+
+def _ce_data(th, rows, dim, vocab, seed):
+    g = th.Generator(device="cuda")
+    g.manual_seed(seed)
+    x = th.randn((rows, dim), device="cuda", generator=g).bfloat16()
+    w = (th.randn((vocab, dim), device="cuda", generator=g) / math.sqrt(dim)).bfloat16()
+    return x, w, th.randint(0, vocab, (rows,), device="cuda", generator=g).to(th.int32)
+
+
+def test_same_bits_every_time_and_on_another_stream(th, art):
+    x, w, tgt = _ce_data(th, 500, 128, 3000, 1)
+    first = _ce(art, th, x, w, tgt)
+    art.synchronize()
+    first = [v.clone() for v in first]
+    other = th.cuda.Stream()
+    other.wait_stream(th.cuda.current_stream())
+    for k in range(4):
+        if k == 2:
+            art.set_stream(other.cuda_stream)
+        got = _ce(art, th, x, w, tgt)
+        art.synchronize()
+        assert all(th.equal(a, b) for a, b in zip(first, got))
+    art.set_stream(th.cuda.current_stream().cuda_stream)
+
+
+def test_two_runtimes_at_once(th):
+    import threading
+
+    x, w, tgt = _ce_data(th, 300, 128, 2000, 2)
+    th.cuda.synchronize()
+    rts = [t.GpuRuntime() for _ in range(2)]
+    outs = [[None] * 6 for _ in rts]
+
+    def work(k):
+        for j in range(6):
+            outs[k][j] = _ce(rts[k], th, x, w, tgt)
+        rts[k].synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    [q.start() for q in threads]
+    [q.join() for q in threads]
+    assert all(th.equal(a, b) for o in outs for got in o for a, b in zip(outs[0][0], got))
+    [r.close() for r in rts]
+
+
+def test_captured_and_replayed(th, art):
+    """Two graphs with a scratch each, replayed on new inputs between eager calls; without a scratch a captured call is refused."""
+    rows, dim, vocab = 400, 64, 1500
+    x, w, tgt = _ce_data(th, rows, dim, vocab, 3)
+    z = th.randn((rows, 700), device="cuda")
+    ids, teacher = make_teacher(th, rows, 6, 700, 4, True)
+    eager = [v.clone() for v in _ce(art, th, x, w, tgt)]
+    art.synchronize()
+    L = t._lib.lib()
+    nbytes = ops.linear_loss_scratch_bytes(art, rows, dim, vocab, trans_w=True, x_dtype=OUT_BF16)
+    graphs, outs = [], []
+    for k in range(2):
+        scratch = art.alloc(nbytes)
+        losses, dz = th.empty(rows, device="cuda"), th.empty_like(z)
+        import ctypes as C
+
+        art.synchronize()
+        art._check(L.t0b_graph_begin(art.handle))
+        out = _ce(art, th, x, w, tgt, scratch=scratch)
+        ops.topk_distill(art, z.data_ptr(), ids.data_ptr(), teacher.data_ptr(), rows, 700, 6, losses=losses.data_ptr(), dlogits=dz.data_ptr())
+        handle = C.c_uint64()
+        art._check(L.t0b_graph_end(art.handle, C.byref(handle)))
+        graphs.append((handle.value, scratch))
+        outs.append((out, losses, dz))
+    art._check(L.t0b_graph_begin(art.handle))
+    with pytest.raises(T0Error, match="scratch"):
+        _ce(art, th, x, w, tgt)
+    handle = C.c_uint64()
+    art._check(L.t0b_graph_end(art.handle, C.byref(handle)))
+    art._check(L.t0b_graph_destroy(art.handle, handle))
+    x2, _, _ = _ce_data(th, rows, dim, vocab, 9)
+    for step in range(2):
+        for handle, _ in graphs:
+            art._check(L.t0b_graph_launch(art.handle, handle, 1))
+        big = _ce(art, th, *_ce_data(th, 900, dim, 5000, 8))          # a larger eager call: the context's workspace grows
+        art.synchronize()
+        want = eager if step == 0 else [v.clone() for v in _ce(art, th, x, w, tgt)]
+        art.synchronize()
+        for out, losses, dz in outs:
+            assert all(th.equal(a, b) for a, b in zip(want, out))
+        x.copy_(x2)
+        del big
+    want_l, want_dz = th.empty(rows, device="cuda"), th.empty_like(z)
+    ops.topk_distill(art, z.data_ptr(), ids.data_ptr(), teacher.data_ptr(), rows, 700, 6, losses=want_l.data_ptr(), dlogits=want_dz.data_ptr())
+    art.synchronize()
+    assert all(th.equal(want_l, o[1]) and th.equal(want_dz, o[2]) for o in outs)
+    for handle, _ in graphs:
+        art._check(L.t0b_graph_destroy(art.handle, handle))
+
+
+def test_an_index_outside_the_vocabulary_is_reported_and_left_out(th, art):
+    x, w, tgt = _ce_data(th, 300, 64, 100, 4)
+    bad = tgt.clone()
+    bad[7] = 100
+    good = tgt.clone()
+    good[7] = -1
+    want = [v.clone() for v in _ce(art, th, x, w, good)]
+    art.synchronize()
+    for sl in (slice(0, 300), slice(0, 40)):
+        got = _ce(art, th, x[sl].contiguous(), w, bad[sl].contiguous())
+        with pytest.raises(T0Error, match="110"):
+            art.synchronize()
+        if sl.stop == 300:
+            assert all(th.equal(a, b) for a, b in zip(want, got))
+    z = th.randn((3, 50), device="cuda")
+    ids = th.tensor([[1, 50], [60, 70], [3, 4]], device="cuda", dtype=th.int32)
+    teacher = th.zeros((3, 2), device="cuda")
+    losses, dz = th.empty(3, device="cuda"), th.empty_like(z)
+    ops.topk_distill(art, z.data_ptr(), ids.data_ptr(), teacher.data_ptr(), 3, 50, 2, losses=losses.data_ptr(), dlogits=dz.data_ptr())
+    with pytest.raises(T0Error, match="110"):
+        art.synchronize()
+    ce = -th.log_softmax(z.double(), 1)
+    assert abs(losses[0].item() - ce[0, 1].item()) < 1e-5 and losses[1] == 0 and (dz[1] == 0).all() and losses[2] > 0
+    assert art.device_status(True) in (0, 110)
+
+
+def test_gradients_against_differences(th, art):
+    """Central differences of the losses' sum: the formulas' gradients are those of the losses the library reports."""
+    rows, cols, topk = 4, 37, 5
+    g = th.Generator(device="cuda")
+    g.manual_seed(11)
+    z = th.randn((rows, cols), device="cuda", generator=g)
+    ids, teacher = make_teacher(th, rows, topk, cols, 2, False)
+    losses, dz = th.empty(rows, device="cuda"), th.empty_like(z)
+    run = lambda zz, out: ops.topk_distill(art, zz.data_ptr(), ids.data_ptr(), teacher.data_ptr(), rows, cols, topk, temperature=1.5, scale=1.0,   # noqa: E731
+                                           losses=losses.data_ptr(), dlogits=out, grads=out is not None)
+    run(z, dz.data_ptr())
+    h = 2.0 ** -6
+    for col in (0, 5, int(ids[0, 0]), cols - 1):
+        diff = th.zeros(rows, device="cuda", dtype=th.float64)
+        for sign in (1, -1):
+            zz = z.clone()
+            zz[:, col] += sign * h
+            run(zz, None)
+            art.synchronize()
+            diff += sign * losses.double()
+        # third derivative of the loss <= 1 / T^3: h^2 / 6; f32 losses of size < 8: 2 * 8 * 8 * 2^-23 / (2 h)
+        assert ((diff / (2 * h) - dz[:, col].double()).abs() <= h * h / 6 + 64 * U32 / h).all()
+
+
+def test_empty_calls(th, art):
+    w = th.ones((30, 16), device="cuda").bfloat16()
+    x = th.ones((1, 16), device="cuda").bfloat16()
+    dw = th.full((30, 16), 7.0, device="cuda")
+    ops.linear_cross_entropy(art, x.data_ptr(), w.data_ptr(), x.data_ptr(), 0, 16, 30, trans_w=True, x_dtype=OUT_BF16, w_dtype=OUT_BF16, losses=x.data_ptr(),
+                             dx=x.data_ptr(), dw=dw.data_ptr())
+    art.synchronize()
+    assert (dw == 0).all() and (x == 1).all()
+    ops.topk_distill(art, x.data_ptr(), x.data_ptr(), x.data_ptr(), 0, 16, 4, losses=x.data_ptr(), grads=False)
+    art.synchronize()
+    assert (x == 1).all()
+
+
+def test_refusals(th, art):
+    x, w, tgt = _ce_data(th, 8, 32, 64, 5)
+    ids, teacher = make_teacher(th, 8, 3, 64, 1, False)
+    out = th.empty((64, 64), device="cuda")
+    p, o = x.data_ptr(), out.data_ptr()
+
+    def linear(match, targets=tgt.data_ptr(), xp=p, wp=w.data_ptr(), rows=8, dim=32, vocab=64, **kw):
+        kw = {**dict(trans_w=True, x_dtype=OUT_BF16, w_dtype=OUT_BF16, losses=o, dx=o, dw=o), **kw}
+        with pytest.raises(T0Error, match=match) as e:
+            ops.linear_cross_entropy(art, xp, wp, targets, rows, dim, vocab, **kw)
+        assert e.value.code in (-1, -5) and not art.is_poisoned()
+
+    linear("null", targets=0)
+    linear("null", xp=0)
+    linear("null", wp=0)
+    linear("empty head", vocab=0)
+    linear("empty head", dim=0)
+    linear("pitch", ldx=31)
+    linear("pitch", ldw=16)
+    linear("x_dtype", x_dtype=5)
+    linear("gradient type", dx_dtype=9)
+    linear("aligned", xp=p + 1)
+    linear("aligned", targets=tgt.data_ptr() + 2)
+    linear("finite", scale=math.nan)
+    linear("scratch", scratch=art.alloc(1024))          # U alone takes 8 * 64 * 2 bytes
+    small = art.alloc(16)
+    linear("does not|needs", xp=small, rows=4096)
+
+    def distill(match, zp=o, topk=3, cols=64, **kw):
+        with pytest.raises(T0Error, match=match):
+            ops.topk_distill(art, zp, kw.pop("ids", ids.data_ptr()), kw.pop("teacher", teacher.data_ptr()), 8, cols, topk, losses=o, grads=False, **kw)
+        with pytest.raises(T0Error, match=match if "logits" not in match and "columns" not in match else None):
+            ops.linear_topk_distill(art, p if zp else 0, w.data_ptr(), kw.pop("ids", ids.data_ptr()) if match != "null" else 0, teacher.data_ptr(), 8, 32,
+                                    64 if cols else 0, topk, trans_w=True, x_dtype=OUT_BF16 if "logits_dtype" not in kw else 7, w_dtype=OUT_BF16, losses=o,
+                                    grads=False, **{k: v for k, v in kw.items() if k in ("temperature", "ldk", "scale")})
+
+    distill("null", zp=0)
+    distill("topk", topk=0)
+    distill("topk", topk=1025)
+    distill("topk", ldk=2)
+    distill("temperature", temperature=0.0)
+    distill("temperature", temperature=-1.0)
+    distill("temperature", temperature=math.inf)
+    distill("logits_dtype", logits_dtype=7)
+    distill("columns", cols=0)
+    with pytest.raises(T0Error, match="their type"):
+        ops.topk_distill(art, o, ids.data_ptr(), teacher.data_ptr(), 8, 64, 3, grad_dtype=OUT_BF16, losses=o, dlogits=o)
+    with pytest.raises(ValueError):
+        ops.linear_cross_entropy(art, p, w.data_ptr(), tgt.data_ptr(), 8, 32, 64, x_dtype=OUT_BF16, w_dtype=3)
+    art.synchronize()
