@@ -112,6 +112,7 @@ struct GemmParams {
     // the most there can be.  K comes as whole blocks of zero rows behind the last (one at least).
     const int* dyn_rows;
     int dyn_off, dyn_k;
+    int late_wait;          // 1: the operands were complete before the kernel in front of this one began; wait for it at the end only
     HeadParams head;        // HEAD kernels only
     int cluster_sk;         // > 1: split-K inside a thread-block cluster of that many CTAs (one per K range): the partial
                             // tiles stay in shared memory and are summed over distributed shared memory; 0 = slabs
@@ -291,50 +292,6 @@ __device__ __forceinline__ float apply_chain(float v, const EpiChain& e, float b
     return v;
 }
 
-// Store one thread's 32 consecutive output columns of one row.
-__device__ __forceinline__ void store_chunk_f32(float* base, long long ld, int row, int col0, int ncols_valid,
-                                                const float (&v)[32], bool vec_ok, bool add = false) {
-    float* dst = base + static_cast<long long>(row) * ld + col0;
-    if (add) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < ncols_valid) dst[j] += v[j];
-    } else if (vec_ok && ncols_valid >= 32) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            reinterpret_cast<float4*>(dst)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < ncols_valid) dst[j] = v[j];
-    }
-}
-
-__device__ __forceinline__ void store_chunk_bf16(__nv_bfloat16* base, long long ld, int row, int col0, int ncols_valid,
-                                                 const float (&v)[32], bool vec_ok) {
-    __nv_bfloat16* dst = base + static_cast<long long>(row) * ld + col0;
-    if (vec_ok && ncols_valid >= 32) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint4 q;
-            __nv_bfloat162 h0 = __floats2bfloat162_rn(v[8 * j + 0], v[8 * j + 1]);
-            __nv_bfloat162 h1 = __floats2bfloat162_rn(v[8 * j + 2], v[8 * j + 3]);
-            __nv_bfloat162 h2 = __floats2bfloat162_rn(v[8 * j + 4], v[8 * j + 5]);
-            __nv_bfloat162 h3 = __floats2bfloat162_rn(v[8 * j + 6], v[8 * j + 7]);
-            q.x = *reinterpret_cast<uint32_t*>(&h0);
-            q.y = *reinterpret_cast<uint32_t*>(&h1);
-            q.z = *reinterpret_cast<uint32_t*>(&h2);
-            q.w = *reinterpret_cast<uint32_t*>(&h3);
-            reinterpret_cast<uint4*>(dst)[j] = q;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < ncols_valid) dst[j] = __float2bfloat16_rn(v[j]);
-    }
-}
-
-
 // Coalesced stores of one warp's 32x32 chunk (lane i holds row i) through a 4 KiB shared-memory transpose tile.
 // 16-byte pieces are XOR-swizzled by row so both the row-wise writes and the line-wise reads are conflict-free.
 // Each global store instruction then writes whole 128-byte (f32) or 64-byte (bf16) row segments.
@@ -364,6 +321,63 @@ __device__ __forceinline__ void flush_chunk_f32(uint32_t stage, int lane, float*
             }
             *dst = q;
         }
+    }
+}
+// 128-byte rows of a staging tile to any address, pitch and number of columns (ES bytes an element, `bytes` of each row): eight
+// lanes a row; the whole 16-byte pieces of the destination are shifted together from two pieces of the tile, what is left at
+// a row's ends goes element by element.  (One row a lane touched 32 sectors with every store: 4416 x 25851 bf16 from 5 rows
+// took 1.2 ms, one element a lane 240 us.)
+template <int ES>
+__device__ __forceinline__ void flush_rows_any(uint32_t stage, int lane, char* base, long long pitch, int rows, int bytes, bool add) {
+    const int c = lane & 7;
+#pragma unroll 2
+    for (int t = 0; t < 8; ++t) {
+        const int r = t * 4 + (lane >> 3);
+        char* dst = base + r * pitch;
+        const int front = min(bytes, static_cast<int>((16u - static_cast<uint32_t>(reinterpret_cast<uint64_t>(dst))) & 15u));
+        const int pieces = (bytes - front) >> 4;
+        const uint32_t row = stage + r * 128;
+        auto piece = [&](int i) {
+            uint4 q;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(row + ((i ^ (r & 7)) << 4)));
+            return q;
+        };
+        if (r < rows && c < pieces) {
+            const uint4 lo = piece(c), hi = piece((c + 1) & 7);   // the last piece of an aligned row has no neighbour and needs none
+            uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+            for (int e = 0; e < 6; ++e) w[e] = (front & 8) ? w[e + 2] : w[e];
+#pragma unroll
+            for (int e = 0; e < 5; ++e) w[e] = (front & 4) ? w[e + 1] : w[e];
+            if constexpr (ES == 2) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = __funnelshift_r(w[e], w[e + 1], (front & 2) * 8);
+            }
+            uint4* out = reinterpret_cast<uint4*>(dst + front) + c;
+            if (ES == 4 && add) {
+                const float4 o = *reinterpret_cast<const float4*>(out);
+                w[0] = __float_as_uint(o.x + __uint_as_float(w[0]));
+                w[1] = __float_as_uint(o.y + __uint_as_float(w[1]));
+                w[2] = __float_as_uint(o.z + __uint_as_float(w[2]));
+                w[3] = __float_as_uint(o.w + __uint_as_float(w[3]));
+            }
+            *out = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        auto element = [&](int at) {   // byte offset in the row
+            const uint32_t addr = row + ((((at >> 4) ^ (r & 7)) << 4) | (at & 15));
+            if constexpr (ES == 2) {
+                uint16_t v;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
+                *reinterpret_cast<uint16_t*>(dst + at) = v;
+            } else {
+                float v;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+                float* d = reinterpret_cast<float*>(dst + at);
+                *d = add ? *d + v : v;
+            }
+        };
+        if (r < rows && c * ES < front) element(c * ES);
+        if (r < rows && front + pieces * 16 + c * ES < bytes) element(front + pieces * 16 + c * ES);
     }
 }
 // TMA-store path: every 32x32 chunk goes out through two 2 KiB half tiles (rows of 64 bytes, 64-byte TMA swizzle:
@@ -527,7 +541,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
     if (threadIdx.x == 0) T0B_STAMP(1);
     // Programmatic dependent launch: everything above (barriers, TMEM, descriptor prefetch) may run while the previous
     // kernel of the stream drains; nothing below may touch global memory before that kernel has completed.
-    ptx::grid_dependency_wait();
+    if (!p.late_wait) ptx::grid_dependency_wait();
     if (threadIdx.x == 0) T0B_STAMP(2);
     ptx::grid_launch_dependents();   // the next GEMM's CTAs may take over SMs as this grid's CTAs exit
     if (p.dyn_rows != nullptr) {
@@ -968,7 +982,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                                 flush_chunk_f32(stage, lane, static_cast<float*>(p.c_dst[d]), ld_out, row0, col0, ext.M, p.N, p.accumulate != 0);
                         }
                     }
-                } else if (row < ext.M && ncols > 0) {
+                } else if (row0 < ext.M && ncols > 0) {   // warp-uniform
                     float v[32];
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
@@ -980,15 +994,31 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                             v[j] = apply_chain(v[j], p.epi, b);
                         }
                     }
-                    if (to_slab) {
-                        store_chunk_f32(p.partial + static_cast<long long>(wi.split) * p.slab_stride, ld_out, row, col0,
-                                        ncols, v, vec_ok);
-                    } else if (p.out_bf16) {
-                        for (int d = 0; d < p.n_dst; ++d)
-                            store_chunk_bf16(static_cast<__nv_bfloat16*>(p.c_dst[d]), ld_out, row, col0, ncols, v, vec_ok);
+                    // Rows that start off 16-byte boundaries: through the transpose tile all the same.
+                    const int rows_here = min(32, ext.M - row0);
+                    if (out16) {
+                        const int half = c & 1;
+                        if (half == 0) __syncwarp();   // the previous pair's reads of the staging tile are done
+                        stage_half_bf16(stage, lane, half, v);
+                        if (half == 1 || ncols <= 32) {
+                            __syncwarp();
+                            const int cbase = col0 - 32 * half;
+                            for (int d = 0; d < p.n_dst; ++d)
+                                flush_rows_any<2>(stage, lane, static_cast<char*>(p.c_dst[d]) + (row0 * ld_out + cbase) * 2, ld_out * 2, rows_here,
+                                                  min(64, p.N - cbase) * 2, false);
+                        }
                     } else {
-                        for (int d = 0; d < p.n_dst; ++d)
-                            store_chunk_f32(static_cast<float*>(p.c_dst[d]), ld_out, row, col0, ncols, v, vec_ok, p.accumulate != 0);
+                        __syncwarp();   // the previous chunk's reads of the staging tile are done
+                        stage_chunk_f32(stage, lane, v);
+                        __syncwarp();
+                        if (to_slab) {
+                            flush_rows_any<4>(stage, lane, reinterpret_cast<char*>(p.partial + static_cast<long long>(wi.split) * p.slab_stride + row0 * ld_out + col0),
+                                              ld_out * 4, rows_here, min(32, ncols) * 4, false);
+                        } else {
+                            for (int d = 0; d < p.n_dst; ++d)
+                                flush_rows_any<4>(stage, lane, static_cast<char*>(p.c_dst[d]) + (row0 * ld_out + col0) * 4, ld_out * 4, rows_here,
+                                                  min(32, ncols) * 4, p.accumulate != 0);
+                        }
                     }
                 }
             }
@@ -1071,6 +1101,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
     }
 
     // ---------------------------------------------------------------------- teardown (normal and abort paths)
+    if (p.late_wait) ptx::grid_dependency_wait();   // whoever waits for this kernel waits for the one in front of it too
     if (csk && threadIdx.x == 64) T0B_STAMP(12);
     ptx::tc_fence_before();
     __syncthreads();

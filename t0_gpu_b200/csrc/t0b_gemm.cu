@@ -85,6 +85,7 @@ struct GemmCall {
     bool accumulate;        // C += A*B (f32 output, one destination, never split)
     const int* dyn_rows;    // rows counted on the device (GemmParams)
     int dyn_off, dyn_k;
+    bool late_wait;
 };
 
 // Expand the public single-op epilogue code into a chain (EPI_BIAS_RELU = bias add, then ReLU).
@@ -368,6 +369,7 @@ int32_t run_gemm(t0b_ctx* ctx, const GemmCall& g) {
         p.out_bf16 = g.out_bf16;
         p.accumulate = g.accumulate ? 1 : 0;
         p.dyn_rows = g.dyn_rows; p.dyn_off = g.dyn_off; p.dyn_k = g.dyn_k;
+        p.late_wait = g.late_wait ? 1 : 0;
         p.raster_along_n = cfg.swap_grid ? 0 : 1;
         {
             p.group = raster_group(ctx, plan.bm, plan.bn, plan.cta_group, cfg.swap_grid != 0);
@@ -453,8 +455,8 @@ GemmCall call_of(const InnerGemm& d) {
     g.trans_a = d.trans_a; g.trans_b = d.trans_b; g.a = d.a; g.b = d.b;
     g.c_dst[0] = d.c; g.n_dst = 1; g.m = d.m; g.n = d.n; g.k = d.k; g.lda = d.lda; g.ldb = d.ldb; g.ldc = d.ldc;
     g.out_bf16 = d.out_bf16; g.accumulate = d.accumulate; g.workspace = d.slabs; g.workspace_bytes = d.slab_bytes;
-    g.no_auto_split = d.accumulate;
     g.dyn_rows = reinterpret_cast<const int*>(d.dyn_rows); g.dyn_off = d.dyn_off; g.dyn_k = d.dyn_k;
+    g.late_wait = d.late_wait;
     return g;
 }
 
@@ -463,13 +465,65 @@ uint64_t rd_u64(const uint8_t* p) { return rd_u32(p) | (static_cast<uint64_t>(rd
 
 }  // namespace
 
+namespace {
+// Tiles and splits of the two gradient products of a head, where the caller has not measured any (t0b_tune, the shipped table).
+// The head's own gradient is a huge output of a contraction over the rows of a batch, never split; the hidden states' gradient
+// is a small output of a contraction over the vocabulary, split until the SMs have work.  The cost model of t0b_gemm is made for
+// neither: here a wave costs what its stores or its operands from L2 cost, whichever is more, and K may be cut into up to 32
+// ranges.  Cycles measured at (m, n, k) = 32000 x 1024 x 128, 50257 x 1000 x 777, 4096 x 32000 x 1024: with k = 128, 128x256
+// tiles take 19.6 us against 25.2 for 256x512; with k = 777, 122 us against 101 for 256x256 and 96 for 256x512.
+t0b_gemm_config head_grad_config(t0b_ctx* ctx, const GemmCall& g, bool split) {
+    struct Cand { const char* name; uint32_t bm, bn, cg; double kb_cycles, epi, floor; };
+    static const Cand cands[] = {{"b200_256x512", 256, 512, 2, 1165.0, 10500.0, 0.0}, {"b200_256x256", 256, 256, 2, 830.0, 0.0, 6500.0},
+                                 {"b200_128x256", 128, 256, 1, 1000.0, 0.0, 4900.0},  {"b200_128x128", 128, 128, 1, 700.0, 0.0, 3000.0},
+                                 {"b200_128x64", 128, 64, 1, 550.0, 0.0, 2500.0}};
+    const uint32_t kb = (g.k + 63) / 64;
+    const Cand* best = nullptr;
+    uint32_t best_sk = 1;
+    double best_cost = 1e300;
+    for (const Cand& c : cands) {
+        const uint64_t tiles = static_cast<uint64_t>((g.m + c.bm - 1) / c.bm) * ((g.n + c.bn - 1) / c.bn), clusters = static_cast<uint64_t>(ctx->num_sms) / c.cg;
+        for (uint32_t sk = 1; sk <= (split ? 32u : 1u); sk *= 2) {
+            if (sk > 1 && (kb / sk < 4 || tiles * (sk / 2) >= clusters)) break;   // split only while SMs are idle
+            double cost = static_cast<double>((tiles * sk + clusters - 1) / clusters) * std::max((kb + sk - 1) / sk * c.kb_cycles + c.epi, c.floor);
+            // The sum over the ranges: inside a cluster over distributed shared memory, or through slabs and a second kernel.
+            if (sk > 1) cost += (c.cg == 1 && (sk <= 4 || (sk == 8 && tiles <= 15))) ? 7000.0 : 14000.0 + 500.0 * sk + static_cast<double>(g.m) * g.n * 4.0 * (sk + 1) / 3300.0;
+            if (cost < best_cost) {
+                best_cost = cost;
+                best = &c;
+                best_sk = sk;
+            }
+        }
+    }
+    t0b_gemm_config cfg{};
+    t0b_config_preset(best->name, &cfg);
+    cfg.swap_grid = g.m >= g.n ? 1 : 0;
+    cfg.split_k = best_sk > 1 ? best_sk : 0;
+    return cfg;
+}
+
+// The config of an inner product: what was measured for it, else the rule above.
+int32_t inner_config(t0b_ctx* ctx, const InnerGemm& d, const GemmCall& g, t0b_gemm_config* cfg) {
+    int source = 0;
+    const char* from = "";
+    if (!ctx->force_config.empty()) {
+        const int32_t rc = choose_config(ctx, g, cfg, &from);
+        if (rc != T0B_OK) return rc;
+    } else if (!tuned_lookup(g.m, g.n, g.k, g.trans_a, g.trans_b, g.out_bf16, cfg, &source)) {
+        *cfg = head_grad_config(ctx, g, !d.head_grad);
+    }
+    if (d.head_grad || g.accumulate) cfg->split_k = 0;
+    return T0B_OK;
+}
+
+}  // namespace
+
 namespace t0b {
 
 size_t inner_gemm_slab_bytes(t0b_ctx* ctx, const InnerGemm& d) {
     const GemmCall g = call_of(d);
     t0b_gemm_config cfg;
-    const char* source = "";
-    if (d.head_grad || g.accumulate || choose_config(ctx, g, &cfg, &source) != T0B_OK) return 0;
+    if (inner_config(ctx, d, g, &cfg) != T0B_OK || cfg.split_k <= 1) return 0;
     t0b_gemm_plan plan;
     const PlanInput pin{g.m, g.n, g.k, g.trans_a, g.trans_b, g.lda, g.ldb, g.a, g.b, ctx->num_sms};
     resolve_plan(&cfg, pin, &plan);
@@ -477,42 +531,15 @@ size_t inner_gemm_slab_bytes(t0b_ctx* ctx, const InnerGemm& d) {
     return static_cast<size_t>(plan.split_k) * g.m * g.n * 4;
 }
 
-// A tile for the head's gradient product: a huge output, a contraction over the rows of a batch, no split.  The cost model of
-// t0b_gemm is made for long contractions; here a wave costs what its stores or its operands from L2 cost, whichever is more.
-// Cycles measured at 32000 x 1024 x 128, 50257 x 1000 x 777 and 4096 x 32000 x 1024 (m, n, rows): with 128 rows 128x256 tiles
-// take 19.6 us against 25.2 for 256x512; with 777 rows 122 us against 101 for 256x256 and 96 for 256x512.
-static t0b_gemm_config head_grad_config(t0b_ctx* ctx, const GemmCall& g) {
-    struct Cand { const char* name; uint32_t bm, bn, cg; double kb_cycles, epi, floor; };
-    static const Cand cands[] = {{"b200_256x512", 256, 512, 2, 1165.0, 10500.0, 0.0}, {"b200_256x256", 256, 256, 2, 830.0, 0.0, 6500.0},
-                                 {"b200_128x256", 128, 256, 1, 1000.0, 0.0, 4900.0},  {"b200_128x128", 128, 128, 1, 700.0, 0.0, 3000.0}};
-    const double kb = (g.k + 63) / 64;
-    const Cand* best = nullptr;
-    double best_cost = 1e300;
-    for (const Cand& c : cands) {
-        const uint64_t tiles = static_cast<uint64_t>((g.m + c.bm - 1) / c.bm) * ((g.n + c.bn - 1) / c.bn), clusters = static_cast<uint64_t>(ctx->num_sms) / c.cg;
-        const double cost = static_cast<double>((tiles + clusters - 1) / clusters) * std::max(kb * c.kb_cycles + c.epi, c.floor);
-        if (cost < best_cost) {
-            best_cost = cost;
-            best = &c;
-        }
-    }
-    t0b_gemm_config cfg{};
-    t0b_config_preset(best->name, &cfg);
-    cfg.swap_grid = g.m >= g.n ? 1 : 0;
-    return cfg;
-}
-
 int32_t inner_gemm(t0b_ctx* ctx, const InnerGemm& d) {
     GemmCall g = call_of(d);
+    t0b_gemm_config cfg;
+    const int32_t rc = inner_config(ctx, d, g, &cfg);
+    if (rc != T0B_OK) return rc;
     // The caller's slabs were sized for the config of that moment; a table entry that appeared since may want more.  The
     // context's own workspace is never used here: it may be freed by a later call while a captured graph still holds it.
-    t0b_gemm_config cfg;
-    if (d.head_grad) {
-        cfg = head_grad_config(ctx, g);
-        g.cfg = &cfg;
-    } else if (inner_gemm_slab_bytes(ctx, d) > d.slab_bytes) {
-        g.no_auto_split = true;
-    }
+    if (cfg.split_k > 1 && inner_gemm_slab_bytes(ctx, d) > d.slab_bytes) cfg.split_k = 0;
+    g.cfg = &cfg;
     return run_gemm(ctx, g);
 }
 

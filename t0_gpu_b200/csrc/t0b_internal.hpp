@@ -135,6 +135,7 @@ struct InnerGemm {
     size_t slab_bytes;
     uint64_t dyn_rows;   // device int, or 0: m (dyn_k: k) is at most *dyn_rows - dyn_off
     int dyn_off, dyn_k;
+    bool late_wait;      // runs beside the product launched just before it, which had the same operands complete (GemmParams)
 };
 size_t inner_gemm_slab_bytes(t0b_ctx* ctx, const InnerGemm& d);
 int32_t inner_gemm(t0b_ctx* ctx, const InnerGemm& d);

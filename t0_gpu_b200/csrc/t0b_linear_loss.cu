@@ -367,6 +367,34 @@ struct Targets {
 };
 __device__ __forceinline__ bool row_live(const Targets& t, uint32_t row) { return t.q ? t.live[row] != 0 : t.ids[row] < t.vocab; }
 
+// One warp: the loss and log-sum-exp of row i of the piece, row r of the call, from its (max z, sum of exp).
+__device__ __forceinline__ void finish_row(float m, float s, uint32_t i, uint32_t r, float inv_t, const Targets& tg, float* losses, float* lse_out,
+                                           int* status) {
+    const uint32_t lane = threadIdx.x & 31;
+    const bool none = m == -INFINITY && s == 0.0f;       // every logit is -inf: the row has no distribution
+    const bool live = row_live(tg, r) && !none;
+    const float log_s = logf(s);
+    float cross = 0.0f;
+    if (live) {
+        const float* z = tg.z_sel + static_cast<size_t>(i) * tg.n_ids;
+        if (tg.q) {
+            for (uint32_t k = lane; k < tg.n_ids; k += 32) {
+                const float q = tg.q[static_cast<size_t>(r) * tg.n_ids + k];
+                if (tg.ids[static_cast<size_t>(r) * tg.n_ids + k] == kNoWord || q == 0.0f || q < 0.0f) continue;
+                cross += q * (log_s - (z[k] - m) * inv_t);
+            }
+            cross = warp_sum(cross) + tg.entropy[r];
+        } else {
+            cross = log_s - (z[0] - m) * inv_t;
+        }
+    }
+    if (lane == 0) {
+        if (losses) losses[r] = live ? cross : 0.0f;
+        if (lse_out) lse_out[r] = live ? m * inv_t + log_s : 0.0f;
+        if (!tg.q && tg.ids[r] >= tg.vocab && tg.ids[r] != kNoWord) *reinterpret_cast<volatile int*>(status) = kDevBadIndex;
+    }
+}
+
 // One block per 32 rows: warps walk the parts (a warp's load is 32 neighbouring rows of one part), the warps' results meet in
 // shared memory, then warp i finishes row i: stats[row] = (max z, sum of exp), the loss and log-sum-exp.
 __global__ void __launch_bounds__(1024) join_parts_kernel(const float2* part, unsigned long long part_ld, uint32_t parts, uint32_t rows,
@@ -401,39 +429,25 @@ __global__ void __launch_bounds__(1024) join_parts_kernel(const float2* part, un
         const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
         join_stats(m, s, m2, s2, c);
     }
-    const bool none = m == -INFINITY && s == 0.0f;       // every logit is -inf: the row has no distribution
-    const bool live = row_live(tg, r) && !none;
-    const float log_s = logf(s);
-    float cross = 0.0f;
-    if (live) {
-        const float* z = tg.z_sel + static_cast<size_t>(i) * tg.n_ids;
-        if (tg.q) {
-            for (uint32_t k = lane; k < tg.n_ids; k += 32) {
-                const float q = tg.q[static_cast<size_t>(r) * tg.n_ids + k];
-                if (tg.ids[static_cast<size_t>(r) * tg.n_ids + k] == kNoWord || q == 0.0f || q < 0.0f) continue;
-                cross += q * (log_s - (z[k] - m) * inv_t);
-            }
-            cross = warp_sum(cross) + tg.entropy[r];
-        } else {
-            cross = log_s - (z[0] - m) * inv_t;
-        }
-    }
-    if (lane == 0) {
-        stats[i] = make_float2(m, s);
-        if (losses) losses[r] = live ? cross : 0.0f;
-        if (lse_out) lse_out[r] = live ? m * inv_t + log_s : 0.0f;
-        if (!tg.q && tg.ids[r] >= tg.vocab && tg.ids[r] != kNoWord) *reinterpret_cast<volatile int*>(status) = kDevBadIndex;
-    }
+    finish_row(m, s, i, r, inv_t, tg, losses, lse_out, status);
+    if (lane == 0) stats[i] = make_float2(m, s);
 }
 
 // ---------------------------------------------------------------------------------------------------- the gradient of z
 // u (fp16, relative to its part's maximum) becomes dz (bf16) in place: a block takes kGradCols columns of one row.  The
-// words of the targets are written last, from their f32 logit.  Bound by HBM: 2 bytes in, 2 bytes out per element.
+// words of the targets are written last, from their f32 logit.  Bound by HBM: 2 bytes in, 2 bytes out per element (4096 x
+// 128000: 358 us, 5.9 TB/s).  Two small steps ride along where their own launch would cost more than they do:
+//   JOIN   every block joins its row's parts itself, and the row's first block finishes the loss (join_parts_kernel is not
+//          launched): for few rows or few parts
+//   x_out  the row's first block copies the hidden state, or zeros in a row without a target, for the head's gradient
 constexpr int kGradVecs = 4;
 constexpr uint32_t kGradCols = 256 * 8 * kGradVecs;
+struct JoinParams { uint32_t parts; float inv_t; float *losses, *lse; int* status; };
+struct CopyParams { const __nv_bfloat16* x; unsigned long long ldx; __nv_bfloat16* out; uint32_t ld_out, dim; };
+template <bool JOIN>
 __global__ void __launch_bounds__(256) dz_kernel(__half* u, unsigned long long ldu, uint32_t rows, uint32_t y0, const float2* part,
                                                  unsigned long long part_ld, uint32_t part_shift, const float2* stats,
-                                                 const float* weights, float scale, float c, Targets tg) {
+                                                 const float* weights, float scale, float c, Targets tg, JoinParams jp, CopyParams cp) {
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
     const uint32_t i = y0 + blockIdx.y;          // the row of the piece, and r of the call
@@ -444,20 +458,52 @@ __global__ void __launch_bounds__(256) dz_kernel(__half* u, unsigned long long l
     const uint32_t r = behind ? 0 : tg.row(i);
     __half* ur = u + i * ldu;
     __nv_bfloat16* gr = reinterpret_cast<__nv_bfloat16*>(ur);
-    const float2 st = behind ? make_float2(0.0f, 1.0f) : stats[i];
-    const bool live = !behind && row_live(tg, r) && !(st.x == -INFINITY && st.y == 0.0f);
-    const float a = live ? scale * (weights ? weights[r] : 1.0f) : 0.0f;
-    const float inv = 1.0f / st.y;
+    const bool wanted = !behind && row_live(tg, r);
     uint4 raw[kGradVecs];
     float top[kGradVecs];
 #pragma unroll
     for (int v = 0; v < kGradVecs; ++v) {
         const uint32_t col = c0 + (v * 256 + threadIdx.x) * 8;
-        if (live && col < ldu) {
+        if (wanted && col < ldu) {
             raw[v] = __ldcs(reinterpret_cast<const uint4*>(ur + col));
             top[v] = part[(col >> part_shift) * part_ld + i].x;
         }
     }
+    if (cp.out && blockIdx.x == 0 && !behind) {
+        const bool vec = rows_vec(cp.x, cp.ldx);
+        for (uint32_t col = threadIdx.x * 8; col < cp.ld_out; col += 256 * 8)
+            *reinterpret_cast<uint4*>(cp.out + static_cast<unsigned long long>(r) * cp.ld_out + col) =
+                wanted ? operand_group(cp.x + r * cp.ldx, col, cp.dim, vec) : make_uint4(0, 0, 0, 0);
+    }
+    float2 st = make_float2(0.0f, 1.0f);
+    if constexpr (JOIN) {
+        __shared__ float2 sh[8];
+        float m = -INFINITY, s = 0.0f;
+        if (!behind)
+            for (uint32_t k = threadIdx.x; k < jp.parts; k += 256) {
+                const float2 v = part[k * part_ld + i];
+                join_stats(m, s, v.x, v.y, c);
+            }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+            join_stats(m, s, m2, s2, c);
+        }
+        if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = make_float2(m, s);
+        __syncthreads();
+        m = sh[0].x;
+        s = sh[0].y;
+        for (int w = 1; w < 8; ++w) join_stats(m, s, sh[w].x, sh[w].y, c);
+        if (!behind) {
+            st = make_float2(m, s);
+            if (blockIdx.x == 0 && threadIdx.x < 32) finish_row(m, s, i, r, jp.inv_t, tg, jp.losses, jp.lse, jp.status);
+        }
+    } else {
+        if (!behind) st = stats[i];
+    }
+    const bool live = wanted && !(st.x == -INFINITY && st.y == 0.0f);
+    const float a = live ? scale * (weights ? weights[r] : 1.0f) : 0.0f;
+    const float inv = 1.0f / st.y;
 #pragma unroll
     for (int v = 0; v < kGradVecs; ++v) {
         const uint32_t col = c0 + (v * 256 + threadIdx.x) * 8;
@@ -490,7 +536,6 @@ __global__ void __launch_bounds__(256) dz_kernel(__half* u, unsigned long long l
     }
 }
 
-
 // Programmatic launch: a kernel's blocks may be placed while the one before drains; every kernel here waits for it before it
 // touches memory.
 template <typename... P, typename... A>
@@ -519,7 +564,9 @@ struct Plan {
     uint32_t parts;
     uint64_t part_ld;
     uint64_t ldu;
-    bool copy_x, copy_w;
+    bool copy_x, copy_w;               // before the head's product
+    bool late_x;                       // the copy of x for the head's gradient is made by dz_kernel; the head reads x itself
+    bool join_in_dz;
     bool gather;                       // the products run over the rows with a target alone
     uint64_t ld_dxg;
     uint64_t row_of, place_of, count, dxg;
@@ -585,10 +632,13 @@ Plan make_plan(t0b_ctx* ctx, const t0b_linear_loss& d, uint32_t n_ids, bool teac
     p.part_ld = (p.piece + 31ull) / 32 * 32;
     // Up to a tile of rows costs the same with and without the rows that are left out.
     p.gather = d.rows > 256;
-    p.copy_x = p.gather || p.grads || d.x_dtype != T0B_OUT_BF16 || !tma_ok(d.x, d.ldx);
-    p.ldx = p.copy_x ? round8(d.dim) : d.ldx;
+    p.copy_x = p.gather || d.x_dtype != T0B_OUT_BF16 || !tma_ok(d.x, d.ldx);
+    p.late_x = p.dw && !p.copy_x;
+    p.ldx = p.copy_x || p.late_x ? round8(d.dim) : d.ldx;
     p.w_rows = d.trans_w ? d.vocab : d.dim;
     p.w_cols = d.trans_w ? d.dim : d.vocab;
+    // A part's (maximum, sum) is 8 bytes of a 32-byte sector to a block that joins one row: up to 16 MB of them in all.
+    p.join_in_dz = p.grads && p.piece * ((p.ldu + kGradCols - 1) / kGradCols) * p.parts * 32ull <= (16ull << 20);
     p.copy_w = !tma_ok(d.w, d.ldw);
     p.ldw = p.copy_w ? round8(p.w_cols) : d.ldw;
     p.acc_dw = p.dw && p.pieces > 1 && d.dw_dtype == T0B_OUT_BF16;
@@ -604,7 +654,7 @@ Plan make_plan(t0b_ctx* ctx, const t0b_linear_loss& d, uint32_t n_ids, bool teac
         p.entropy = take(rows * 4);
         p.live = take(rows * 4);
     }
-    if (p.copy_x) p.x = take(rows * p.ldx * 2);
+    if (p.copy_x || p.late_x) p.x = take(rows * p.ldx * 2);
     if (p.copy_w) p.w = take(p.w_rows * p.ldw * 2);
     if (p.gather) {
         p.row_of = take(rows * 4);
@@ -770,9 +820,9 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
         tg.row0 = r0;
         HeadGemm hg{};
         hg.plan = p.head;
-        hg.x = x + static_cast<uint64_t>(r0) * p.ldx * 2;
+        hg.ldx = p.copy_x ? p.ldx : d.ldx; hg.ldw = p.ldw;
+        hg.x = x + static_cast<uint64_t>(r0) * hg.ldx * 2;
         hg.w = w;
-        hg.ldx = p.ldx; hg.ldw = p.ldw;
         hg.rows = n; hg.dim = d.dim; hg.vocab = d.vocab; hg.trans_w = d.trans_w;
         hg.c = c;
         hg.part = base + p.part; hg.part_ld = p.part_ld;
@@ -787,14 +837,18 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
         rc = head_gemm(ctx, hg);
         if (rc != T0B_OK) return rc;
         float2* stats = reinterpret_cast<float2*>(base + p.stats);
-        launch(ctx, join_parts_kernel, (n + 31) / 32, 1024, 0, reinterpret_cast<const float2*>(base + p.part), p.part_ld, p.parts, n, c, inv_t, tg, stats,
-               losses, lse, ctx->status_dev);
-        ++launched;
+        if (!p.join_in_dz) {
+            launch(ctx, join_parts_kernel, (n + 31) / 32, 1024, 0, reinterpret_cast<const float2*>(base + p.part), p.part_ld, p.parts, n, c, inv_t, tg, stats,
+                   losses, lse, ctx->status_dev);
+            ++launched;
+        }
         if (!p.grads) continue;
+        const JoinParams jp{p.parts, inv_t, losses, lse, ctx->status_dev};
+        const CopyParams cp{xb, d.ldx, p.late_x ? xg : nullptr, static_cast<uint32_t>(p.ldx), d.dim};
         for (uint32_t y0 = 0; y0 < n; y0 += 65535u) {   // gridDim.y is limited to 65535
-            launch(ctx, dz_kernel, dim3(static_cast<uint32_t>((p.ldu + kGradCols - 1) / kGradCols), std::min(65535u, n - y0)), 256, 0,
-                   reinterpret_cast<__half*>(base + p.u), p.ldu, n, y0, reinterpret_cast<const float2*>(base + p.part), p.part_ld, part_shift, stats,
-                   reinterpret_cast<const float*>(d.row_weights), d.scale * inv_t, c, tg);
+            launch(ctx, p.join_in_dz ? dz_kernel<true> : dz_kernel<false>, dim3(static_cast<uint32_t>((p.ldu + kGradCols - 1) / kGradCols), std::min(65535u, n - y0)),
+                   256, 0, reinterpret_cast<__half*>(base + p.u), p.ldu, n, y0, reinterpret_cast<const float2*>(base + p.part), p.part_ld, part_shift, stats,
+                   reinterpret_cast<const float*>(d.row_weights), d.scale * inv_t, c, tg, jp, cp);
             ++launched;
         }
         rc = check_cuda(ctx, cudaGetLastError(), what);
@@ -807,7 +861,11 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
             if (rc != T0B_OK) return rc;
         }
         if (p.dw) {
-            InnerGemm g = dw_gemm(d, p, base + p.u, x, base, r0, n);
+            InnerGemm g = dw_gemm(d, p, base + p.u, p.late_x ? base + p.x : x, base, r0, n);
+            // Both gradient products need dz alone, so after a short first one of few rows the second need not wait for it and
+            // fills the SMs that it leaves (128 x 1024 -> 32000: 95 -> 84 us a step).  Longer ones run one after the other:
+            // side by side they compete for L2 (4096 x 4096 -> 128000: 11.3 -> 11.6 ms, 5806 x 448 -> 6400: 163 -> 172 us).
+            g.late_wait = p.dx && n <= 1024 && 2.0 * n * d.dim * d.vocab < 1e11;
             g.slabs = base + p.slabs;
             g.slab_bytes = p.slab_bytes;
             rc = inner_gemm(ctx, g);
