@@ -113,17 +113,14 @@ __global__ void __launch_bounds__(256) pack_shifted_kernel(const __nv_bfloat16* 
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
     const uint32_t lane = threadIdx.x & 31;
-    const uint32_t per_row = ld_out / 8, warps_per_row = (per_row + 31) / 32;
-    const unsigned long long total = static_cast<unsigned long long>(rows) * warps_per_row;
+    const uint32_t c = (blockIdx.x * 256 + threadIdx.x) * 8;   // a warp's columns are neighbours
     const uint64_t begin = reinterpret_cast<uint64_t>(in), end = begin + ((rows - 1ull) * ld + cols) * 2;
-    for (unsigned long long i = blockIdx.x * 8ull + (threadIdx.x >> 5); i < total; i += gridDim.x * 8ull) {
-        const uint32_t r = static_cast<uint32_t>(i / warps_per_row);
-        const uint32_t c = (static_cast<uint32_t>(i % warps_per_row) * 32 + lane) * 8;
+    auto load = [&](uint64_t addr) {
+        return addr >= begin && addr + 16 <= end ? __ldcs(reinterpret_cast<const uint4*>(addr)) : make_uint4(0, 0, 0, 0);
+    };
+    for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
         const uint64_t at = begin + (r * ld + c) * 2, chunk = at & ~15ull;
         const uint32_t shift = static_cast<uint32_t>(at & 15);
-        auto load = [&](uint64_t addr) {
-            return addr >= begin && addr + 16 <= end ? __ldcs(reinterpret_cast<const uint4*>(addr)) : make_uint4(0, 0, 0, 0);
-        };
         const uint4 a = load(chunk);
         uint4 b;
         b.x = __shfl_down_sync(0xffffffffu, a.x, 1);
@@ -630,8 +627,9 @@ Plan make_plan(t0b_ctx* ctx, const t0b_linear_loss& d, uint32_t n_ids, bool teac
     p.head = head_plan(ctx, p.piece, d.vocab, d.dim);
     p.parts = (d.vocab + p.head.part_cols - 1) / p.head.part_cols;
     p.part_ld = (p.piece + 31ull) / 32 * 32;
-    // Up to a tile of rows costs the same with and without the rows that are left out.
-    p.gather = d.rows > 256;
+    // Up to a tile of rows costs the same with and without the rows that are left out; the losses alone of a small product
+    // cost less than finding the rows (two kernels, 5 us).
+    p.gather = d.rows > 256 && (p.grads || 2.0 * d.rows * d.dim * d.vocab >= 5e10);
     p.copy_x = p.gather || d.x_dtype != T0B_OUT_BF16 || !tma_ok(d.x, d.ldx);
     p.late_x = p.dw && !p.copy_x;
     p.ldx = p.copy_x || p.late_x ? round8(d.dim) : d.ldx;
@@ -797,8 +795,10 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
         launched += 2;
     }
     if (p.copy_w) {
-        launch(ctx, pack_shifted_kernel, lin_blocks(ctx, p.w_rows * ((p.ldw / 8 + 31) / 32 * 32)), 256, 0, reinterpret_cast<const __nv_bfloat16*>(d.w), d.ldw,
-               reinterpret_cast<__nv_bfloat16*>(base + p.w), static_cast<uint32_t>(p.ldw), static_cast<uint32_t>(p.w_rows), static_cast<uint32_t>(p.w_cols));
+        const uint32_t across = static_cast<uint32_t>((p.ldw / 8 + 255) / 256);
+        launch(ctx, pack_shifted_kernel, dim3(across, static_cast<uint32_t>(std::min<uint64_t>(p.w_rows, 65535))), 256, 0,
+               reinterpret_cast<const __nv_bfloat16*>(d.w), d.ldw, reinterpret_cast<__nv_bfloat16*>(base + p.w), static_cast<uint32_t>(p.ldw),
+               static_cast<uint32_t>(p.w_rows), static_cast<uint32_t>(p.w_cols));
         ++launched;
     }
     uint32_t part_shift = 0;
