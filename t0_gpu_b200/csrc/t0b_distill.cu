@@ -711,7 +711,7 @@ extern "C" {
 
 int32_t t0b_topk_distill(t0b_ctx* ctx, uint64_t logits, int32_t logits_dtype, uint64_t ids, uint64_t teacher, uint64_t row_weights,
                          uint64_t losses, uint64_t dlogits, int32_t grad_dtype, uint32_t rows, uint32_t cols, uint64_t ld,
-                         uint32_t topk, uint64_t ldk, float temperature, float scale, int32_t async) {
+                         uint32_t topk, uint64_t ldk, float temperature, float scale, int32_t async) try {
     int32_t rc = precheck(ctx);
     if (rc != T0B_OK) return rc;
     if (rows == 0) return T0B_OK;
@@ -721,8 +721,8 @@ int32_t t0b_topk_distill(t0b_ctx* ctx, uint64_t logits, int32_t logits_dtype, ui
     if (cols == 0 || cols > 0x7fffff00u || ld < cols) return set_error(ctx, T0B_ERR_INVALID, "topk_distill: %u columns with a pitch of %llu", cols, static_cast<unsigned long long>(ld));
     if (topk == 0 || topk > T0B_MAX_TOPK || ldk < topk)
         return set_error(ctx, T0B_ERR_INVALID, "topk_distill: topk %u is outside 1..%d, or its pitch %llu is smaller", topk, T0B_MAX_TOPK, static_cast<unsigned long long>(ldk));
-    if (!(temperature > 0.0f) || !std::isfinite(temperature) || !std::isfinite(scale))
-        return set_error(ctx, T0B_ERR_INVALID, "topk_distill: temperature %g must be positive and finite, scale %g finite", temperature, scale);
+    if (!(temperature > 0.0f) || !std::isfinite(temperature) || !std::isfinite(1.4426950408889634f / temperature) || !std::isfinite(scale))
+        return set_error(ctx, T0B_ERR_INVALID, "topk_distill: temperature %g and its inverse must be positive and finite, scale %g finite", temperature, scale);
     const size_t ie = logits_dtype == T0B_OUT_BF16 ? 2 : 4, oe = grad_dtype == T0B_OUT_BF16 ? 2 : 4;
     if (logits % ie || (dlogits && dlogits % oe) || ids % 4 || teacher % 4 || losses % 4 || row_weights % 4)
         return set_error(ctx, T0B_ERR_INVALID, "topk_distill: a pointer is not aligned to its element");
@@ -749,6 +749,8 @@ int32_t t0b_topk_distill(t0b_ctx* ctx, uint64_t logits, int32_t logits_dtype, ui
     else rc = oe == 2 ? run_distill<float, __nv_bfloat16>(ctx, p, rows) : run_distill<float, float>(ctx, p, rows);
     if (rc != T0B_OK) return rc;
     return finish(ctx, async, "topk_distill");
+} catch (...) {
+    return T0B_ERR_NOMEM;   // no C++ exception leaves a C entry
 }
 
 }  // extern "C"

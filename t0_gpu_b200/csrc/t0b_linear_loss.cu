@@ -896,14 +896,17 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
 
 extern "C" {
 
-size_t t0b_linear_loss_scratch_bytes(t0b_ctx* ctx, const t0b_linear_loss* loss, uint32_t topk) {
+size_t t0b_linear_loss_scratch_bytes(t0b_ctx* ctx, const t0b_linear_loss* loss, uint32_t topk) try {
     if (!ctx || !loss || loss->rows == 0 || loss->dim == 0 || loss->vocab == 0) return 0;
     std::lock_guard<std::recursive_mutex> lk(ctx->mu);
     if (precheck(ctx) != T0B_OK) return 0;
     return make_plan(ctx, *loss, std::max(1u, topk), topk > 0).total;
+} catch (...) {
+    return 0;
 }
 
-int32_t t0b_linear_ce(t0b_ctx* ctx, const t0b_linear_loss* loss, uint64_t targets, int32_t async) {
+// No C++ exception (the host's memory running out) leaves a C entry.
+int32_t t0b_linear_ce(t0b_ctx* ctx, const t0b_linear_loss* loss, uint64_t targets, int32_t async) try {
     int32_t rc = precheck(ctx);
     if (rc != T0B_OK) return rc;
     if (!loss || !targets || targets % 4) return set_error(ctx, T0B_ERR_INVALID, "linear_ce: null or misaligned pointer");
@@ -912,24 +915,28 @@ int32_t t0b_linear_ce(t0b_ctx* ctx, const t0b_linear_loss* loss, uint64_t target
     if (rc == T0B_OK) rc = check_fits(ctx, "linear_ce", {{"targets", targets, loss->rows * 4ull}});
     if (rc != T0B_OK) return rc;
     return run_linear_loss(ctx, "linear_ce", *loss, Teacher{targets, 0, 1, 1}, 1.0f, async);
+} catch (...) {
+    return T0B_ERR_NOMEM;
 }
 
 int32_t t0b_linear_topk_distill(t0b_ctx* ctx, const t0b_linear_loss* loss, uint64_t ids, uint64_t teacher, uint32_t topk, uint64_t ldk,
-                                float temperature, int32_t async) {
+                                float temperature, int32_t async) try {
     int32_t rc = precheck(ctx);
     if (rc != T0B_OK) return rc;
     if (!loss || !ids || !teacher || ids % 4 || teacher % 4) return set_error(ctx, T0B_ERR_INVALID, "linear_topk_distill: null or misaligned pointer");
     if (topk == 0 || topk > T0B_MAX_TOPK || ldk < topk)
         return set_error(ctx, T0B_ERR_INVALID, "linear_topk_distill: topk %u is outside 1..%d, or its pitch %llu is smaller", topk, T0B_MAX_TOPK,
                          static_cast<unsigned long long>(ldk));
-    if (!(temperature > 0.0f) || !std::isfinite(temperature))
-        return set_error(ctx, T0B_ERR_INVALID, "linear_topk_distill: temperature %g must be positive and finite", temperature);
+    if (!(temperature > 0.0f) || !std::isfinite(temperature) || !std::isfinite(1.4426950408889634f / temperature))
+        return set_error(ctx, T0B_ERR_INVALID, "linear_topk_distill: temperature %g must be positive and finite, and so must its inverse", temperature);
     std::lock_guard<std::recursive_mutex> lk(ctx->mu);
     rc = check_desc(ctx, "linear_topk_distill", *loss);
     if (rc == T0B_OK && loss->rows > 0)
         rc = check_fits(ctx, "linear_topk_distill", {{"ids", ids, ((loss->rows - 1ull) * ldk + topk) * 4}, {"teacher", teacher, ((loss->rows - 1ull) * ldk + topk) * 4}});
     if (rc != T0B_OK) return rc;
     return run_linear_loss(ctx, "linear_topk_distill", *loss, Teacher{ids, teacher, ldk, topk}, temperature, async);
+} catch (...) {
+    return T0B_ERR_NOMEM;
 }
 
 }  // extern "C"

@@ -160,13 +160,15 @@ def topk_distill(rt: GpuRuntime, logits, ids, teacher, rows: int, cols: int, top
     return losses, dlogits if grads else None
 
 
-def _linear_loss(rt: GpuRuntime, call, x, w, rows, dim, vocab, topk, scale, row_weights, grads, trans_w, x_dtype, w_dtype, dx_dtype,
-                 dw_dtype, ldx, ldw, weight_id, losses, lse, dx, dw, piece_rows, scratch):
+def _linear_loss(rt: GpuRuntime, call, x, w, rows, dim, vocab, scale, row_weights, grads, x_needs, w_needs, trans_w, x_dtype, w_dtype, dx_dtype,
+                 dw_dtype, ldx, ldw, lddx, lddw, weight_id, losses, lse, dx, dw, piece_rows, scratch):
     w_rows, w_cols = (vocab, dim) if trans_w else (dim, vocab)
     w16 = None
     if w_dtype == OUT_F32:
         if ldw is not None and ldw != w_cols:
             raise ValueError("linear loss: an f32 head is converted as a whole and has no pitch of its own")
+        if scratch is not None:
+            raise ValueError("linear loss: with a scratch (a captured call) the head is bf16: a converted copy would not outlive the call")
         if weight_id is not None:
             w = rt.get_or_create_bf16(weight_id, w if isinstance(w, GpuBuffer) else GpuBuffer(rt, w, 0, False), w_rows * w_cols)
         else:
@@ -176,47 +178,52 @@ def _linear_loss(rt: GpuRuntime, call, x, w, rows, dim, vocab, topk, scale, row_
     elif w_dtype != OUT_BF16:
         raise ValueError(f"linear loss: unknown w_dtype {w_dtype}")
     losses = losses if losses is not None else rt.alloc(max(rows * 4, 16))
-    if grads and dx is None:
-        dx = rt.alloc(max(rows * dim * _ELEM.get(dx_dtype, 4), 16))
-    if grads and dw is None:
-        dw = rt.alloc(max(w_rows * w_cols * _ELEM.get(dw_dtype, 4), 16))
+    x_needs, w_needs = grads and x_needs, grads and w_needs
+    lddx, lddw = lddx if lddx is not None else dim, lddw if lddw is not None else w_cols
+    if x_needs and dx is None:
+        dx = rt.alloc(max(rows * lddx * _ELEM.get(dx_dtype, 4), 16))
+    if w_needs and dw is None:
+        dw = rt.alloc(max(w_rows * lddw * _ELEM.get(dw_dtype, 4), 16))
     d = LinearLossC(x=_addr(x), w=_addr(w), ldx=ldx if ldx is not None else dim, ldw=ldw if ldw is not None else w_cols, row_weights=_addr(row_weights),
-                    losses=_addr(losses), lse=_addr(lse), dx=_addr(dx) if grads else 0, dw=_addr(dw) if grads else 0, lddx=dim, lddw=w_cols,
+                    losses=_addr(losses), lse=_addr(lse), dx=_addr(dx) if x_needs else 0, dw=_addr(dw) if w_needs else 0, lddx=lddx, lddw=lddw,
                     scratch=_addr(scratch), scratch_bytes=scratch.size() if scratch is not None else 0, rows=rows, dim=dim, vocab=vocab,
                     trans_w=int(trans_w), piece_rows=piece_rows, x_dtype=x_dtype, dx_dtype=dx_dtype, dw_dtype=dw_dtype,
                     scale=scale if scale is not None else 1.0 / max(rows, 1))
-    rt._check(call(d))
-    if w16 is not None:
-        rt.recycle(w16)
-    return (losses, dx, dw) if grads else (losses, None, None)
+    try:
+        rt._check(call(d))
+    finally:
+        if w16 is not None:
+            rt.recycle(w16)
+    return losses, dx if x_needs else None, dw if w_needs else None
 
 
 def linear_cross_entropy(rt: GpuRuntime, x, w, targets, rows: int, dim: int, vocab: int, *, scale: Optional[float] = None, row_weights=None,
-                         grads: bool = True, trans_w: bool = False, x_dtype: int = OUT_F32, w_dtype: int = OUT_F32, dx_dtype: int = OUT_F32,
-                         dw_dtype: int = OUT_F32, ldx: Optional[int] = None, ldw: Optional[int] = None, weight_id: Optional[int] = None,
-                         losses=None, lse=None, dx=None, dw=None, piece_rows: int = 0, scratch: Optional[GpuBuffer] = None):
+                         grads: bool = True, x_needs: bool = True, w_needs: bool = True, trans_w: bool = False, x_dtype: int = OUT_F32,
+                         w_dtype: int = OUT_F32, dx_dtype: int = OUT_F32, dw_dtype: int = OUT_F32, ldx: Optional[int] = None,
+                         ldw: Optional[int] = None, lddx: Optional[int] = None, lddw: Optional[int] = None, weight_id: Optional[int] = None, losses=None, lse=None, dx=None, dw=None, piece_rows: int = 0, scratch: Optional[GpuBuffer] = None):
     """`matmul` with the head followed by `cross_entropy`, and both their backwards, without the [rows, vocab] logits: x
     [rows, dim], w [dim, vocab] (`trans_w`: [vocab, dim]), targets u32[rows] (`NO_WORD`: the row is left out).  Returns
-    (losses f32[rows], dx, dw) with the gradients of scale * sum(row_weights * losses) (default scale 1 / rows), or
-    (losses, None, None) without `grads`.  As in `matmul`, f32 operands are multiplied as bf16 (an f32 head is converted in
+    (losses f32[rows], dx, dw) with the gradients of scale * sum(row_weights * losses) (default scale 1 / rows); None for
+    both without `grads`, for one without `x_needs` or `w_needs`.  As in `matmul`, f32 operands are multiplied as bf16 (an f32 head is converted in
     every call, or once through the runtime's cached copy under `weight_id`) and gradients are f32 unless asked otherwise.  Buffers are
     `GpuBuffer`s or device addresses; outputs that are not given come from the pool; `lse` (f32[rows], optional) receives
     log-sum-exp.  Only queues work; inside a captured graph pass `scratch` (`linear_loss_scratch_bytes`)."""
-    return _linear_loss(rt, lambda d: lib().t0b_linear_ce(rt.handle, C.byref(d), _addr(targets), 1), x, w, rows, dim, vocab, 0, scale,
-                        row_weights, grads, trans_w, x_dtype, w_dtype, dx_dtype, dw_dtype, ldx, ldw, weight_id, losses, lse, dx, dw, piece_rows,
-                        scratch)
+    return _linear_loss(rt, lambda d: lib().t0b_linear_ce(rt.handle, C.byref(d), _addr(targets), 1), x, w, rows, dim, vocab, scale,
+                        row_weights, grads, x_needs, w_needs, trans_w, x_dtype, w_dtype, dx_dtype, dw_dtype, ldx, ldw, lddx, lddw, weight_id, losses, lse,
+                        dx, dw, piece_rows, scratch)
 
 
 def linear_topk_distill(rt: GpuRuntime, x, w, ids, teacher, rows: int, dim: int, vocab: int, topk: int, *, temperature: float = 1.0,
-                        ldk: Optional[int] = None, scale: Optional[float] = None, row_weights=None, grads: bool = True, trans_w: bool = False,
-                        x_dtype: int = OUT_F32, w_dtype: int = OUT_F32, dx_dtype: int = OUT_F32, dw_dtype: int = OUT_F32,
-                        ldx: Optional[int] = None, ldw: Optional[int] = None, weight_id: Optional[int] = None, losses=None, lse=None, dx=None,
+                        ldk: Optional[int] = None, scale: Optional[float] = None, row_weights=None, grads: bool = True, x_needs: bool = True,
+                        w_needs: bool = True, trans_w: bool = False, x_dtype: int = OUT_F32, w_dtype: int = OUT_F32, dx_dtype: int = OUT_F32,
+                        dw_dtype: int = OUT_F32, ldx: Optional[int] = None, ldw: Optional[int] = None, lddx: Optional[int] = None,
+                        lddw: Optional[int] = None, weight_id: Optional[int] = None, losses=None, lse=None, dx=None,
                         dw=None, piece_rows: int = 0, scratch: Optional[GpuBuffer] = None):
     """`topk_distill` on the logits x * head, without the logits; arguments and results as for `linear_cross_entropy`."""
     return _linear_loss(rt, lambda d: lib().t0b_linear_topk_distill(rt.handle, C.byref(d), _addr(ids), _addr(teacher), topk,
                                                                     ldk if ldk is not None else topk, temperature, 1),
-                        x, w, rows, dim, vocab, topk, scale, row_weights, grads, trans_w, x_dtype, w_dtype, dx_dtype, dw_dtype, ldx, ldw,
-                        weight_id, losses, lse, dx, dw, piece_rows, scratch)
+                        x, w, rows, dim, vocab, scale, row_weights, grads, x_needs, w_needs, trans_w, x_dtype, w_dtype, dx_dtype, dw_dtype, ldx, ldw,
+                        lddx, lddw, weight_id, losses, lse, dx, dw, piece_rows, scratch)
 
 
 def linear_loss_scratch_bytes(rt: GpuRuntime, rows: int, dim: int, vocab: int, *, topk: int = 0, grads: bool = True, trans_w: bool = False,

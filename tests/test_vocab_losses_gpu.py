@@ -83,7 +83,7 @@ def losses_and_dz(th, z, q, ent, live, temperature, row_scale):
 
 
 def check_linear(th, art, rows, dim, vocab, trans_w, *, topk=0, temperature=1.0, grads=True, x_dtype=OUT_BF16, gdt=OUT_BF16, weights=True, ignore=True,
-                 piece_rows=0, ldx_pad=0, ldw_pad=0, ragged=True, big=1.0, offset=0, keep=None):
+                 piece_rows=0, ldx_pad=0, ldw_pad=0, ragged=True, big=1.0, offset=0, keep=None, ldd_pad=0, x_needs=True, w_needs=True):
     g = th.Generator(device="cuda")
     g.manual_seed(rows * 7919 + dim * 31 + vocab)
     w_rows, w_cols = (vocab, dim) if trans_w else (dim, vocab)
@@ -121,11 +121,12 @@ def check_linear(th, art, rows, dim, vocab, trans_w, *, topk=0, temperature=1.0,
     losses_ref, dz, p, lse_ref = losses_and_dz(th, z, q, ent, live, temperature, row_scale)
     losses, lse = th.full((rows,), 7.0, device="cuda"), th.full((rows,), 7.0, device="cuda")
     odt = th.bfloat16 if gdt == OUT_BF16 else th.float32
-    dx = th.full((rows + 1, dim), 7.0, device="cuda", dtype=odt)
-    dw = th.full((w_rows + 1, w_cols), 7.0, device="cuda", dtype=odt)
+    dxb = th.full((rows + 1, dim + ldd_pad), 7.0, device="cuda", dtype=odt)
+    dwb = th.full((w_rows + 1, w_cols + ldd_pad), 7.0, device="cuda", dtype=odt)
+    dx, dw = dxb[:, :dim], dwb[:, :w_cols]
     kw = dict(grads=grads, trans_w=trans_w, x_dtype=x_dtype, w_dtype=OUT_BF16, dx_dtype=gdt, dw_dtype=gdt, ldx=ldx, ldw=ldw, losses=losses.data_ptr(),
               lse=lse.data_ptr(), dx=dx.data_ptr() if grads else None, dw=dw.data_ptr() if grads else None, piece_rows=piece_rows,
-              row_weights=rw.data_ptr() if weights else None)
+              lddx=dim + ldd_pad, lddw=w_cols + ldd_pad, x_needs=x_needs, w_needs=w_needs, row_weights=rw.data_ptr() if weights else None)
     if topk:
         ops.linear_topk_distill(art, x.data_ptr(), w.data_ptr(), ids.data_ptr(), teacher.data_ptr(), rows, dim, vocab, topk, temperature=temperature, **kw)
     else:
@@ -150,14 +151,16 @@ def check_linear(th, art, rows, dim, vocab, trans_w, *, topk=0, temperature=1.0,
     dx_ref, edx = dz @ wd, edz @ wa + vocab * U32 * (full @ wa)
     bound = edx + uo * (dx_ref.abs() + edx) + 1e-30
     err = (dx[:rows].double() - dx_ref).abs()
-    assert (err <= bound).all(), (err / bound).max()
+    assert not x_needs or (err <= bound).all(), (err / bound).max()
     dw_ref, edw = dz.t() @ xd, edz.t() @ xa + rows * U32 * (full.t() @ xa)
     bound = edw + uo * (dw_ref.abs() + edw) + 1e-30
     got = dw[:w_rows].double() if trans_w else dw[:w_rows].double().t()
     err = (got - dw_ref).abs()
-    assert (err <= bound).all(), (err / bound).max()
-    assert (dx[rows] == 7).all() and (dw[w_rows] == 7).all()                     # nothing behind the last row
-    assert (dx[:rows][~live] == 0).all()
+    assert not w_needs or (err <= bound).all(), (err / bound).max()
+    # nothing behind the last row, behind a row's end, or where no gradient was asked for
+    assert (dxb[rows] == 7).all() and (dwb[w_rows] == 7).all() and (dxb[:, dim:] == 7).all() and (dwb[:, w_cols:] == 7).all()
+    assert (x_needs or (dxb == 7).all()) and (w_needs or (dwb == 7).all())
+    assert not x_needs or (dx[:rows][~live] == 0).all()
 
 
 LINEAR_SIZES = [(1, 64, 64), (1, 8, 1), (3, 40, 17), (33, 64, 129), (128, 128, 1000), (130, 200, 513), (257, 96, 2048), (300, 1000, 777), (64, 72, 5001)]
@@ -213,6 +216,21 @@ def test_linear_pitches_and_offsets(th, art, trans_w):
     check_linear(th, art, 50, 64, 320, trans_w, ldx_pad=3, ldw_pad=5)
     check_linear(th, art, 50, 64, 320, trans_w, offset=1)
     check_linear(th, art, 50, 64, 320, trans_w, grads=False, ignore=False, ldx_pad=1, offset=3)
+
+
+@pytest.mark.parametrize("trans_w", [False, True])
+@pytest.mark.parametrize("gdt", [OUT_F32, OUT_BF16])
+@pytest.mark.parametrize("rows", [50, 300])
+def test_linear_gradient_pitches(th, art, rows, gdt, trans_w):
+    for pad in (8, 3):
+        check_linear(th, art, rows, 72, 321, trans_w, gdt=gdt, ldd_pad=pad, piece_rows=0 if pad == 8 else 128)
+
+
+@pytest.mark.parametrize("rows", [50, 300])
+@pytest.mark.parametrize("x_needs,w_needs", [(True, False), (False, True)])
+def test_linear_one_gradient(th, art, rows, x_needs, w_needs):
+    check_linear(th, art, rows, 64, 200, True, x_needs=x_needs, w_needs=w_needs)
+    check_linear(th, art, rows, 64, 200, False, topk=4, x_needs=x_needs, w_needs=w_needs)
 
 
 @pytest.mark.parametrize("trans_w", [False, True])
@@ -308,6 +326,26 @@ def test_topk_distill_long_rows_are_read_twice(th, art, dtype):
     cols = 450_000 if dtype == OUT_F32 else 900_001
     check_logits(th, art, 3, cols, 5, dtype=dtype)
     check_logits(th, art, 2, cols, 5, dtype=dtype, in_place=True)
+
+
+def test_topk_distill_offsets_past_32_bits(th, art):
+    """4.3e9 logits, in place: all rows but the last two are left out and become zeros."""
+    rows, cols = 33100, 130000
+    z = th.empty((rows, cols), device="cuda", dtype=th.bfloat16)
+    z[-2:] = th.randn((2, cols), device="cuda").bfloat16()
+    z[0], z[rows // 2], last = math.nan, math.nan, z[-2:].double()
+    ids = th.full((rows, 3), -1, device="cuda", dtype=th.int32)
+    ids[-2:] = th.tensor([[5, 77, cols - 1], [0, 1, 2]], device="cuda", dtype=th.int32)
+    teacher = th.randn((rows, 3), device="cuda")
+    losses = th.empty(rows, device="cuda")
+    ops.topk_distill(art, z.data_ptr(), ids.data_ptr(), teacher.data_ptr(), rows, cols, 3, logits_dtype=OUT_BF16, grad_dtype=OUT_BF16,
+                     losses=losses.data_ptr(), dlogits=z.data_ptr(), scale=1.0)
+    art.synchronize()
+    q, ent, live = target_rows(th, ids[-2:], teacher[-2:], 1.0, cols)
+    ref, dz, p, _ = losses_and_dz(th, last, q, ent, live, 1.0, th.ones(2, device="cuda", dtype=th.float64))
+    assert ((losses[-2:].double() - ref).abs() <= 1e-4).all() and (losses[:-2] == 0).all()
+    assert ((z[-2:].double() - dz).abs() <= UB * dz.abs() + (1 + UB) * (p * (UH + 64 * U32) + 2.0 ** -24 * p.amax(1, keepdim=True)) + q * 32 * U32).all()
+    assert (z[0] == 0).all() and (z[rows // 2] == 0).all() and (z[-3] == 0).all()
 
 
 def test_topk_distill_values_at_the_edge(th, art):
@@ -625,10 +663,13 @@ def test_refusals(th, art):
     distill("temperature", temperature=0.0)
     distill("temperature", temperature=-1.0)
     distill("temperature", temperature=math.inf)
+    distill("temperature", temperature=1e-39)
     distill("logits_dtype", logits_dtype=7)
     distill("columns", cols=0)
     with pytest.raises(T0Error, match="their type"):
         ops.topk_distill(art, o, ids.data_ptr(), teacher.data_ptr(), 8, 64, 3, grad_dtype=OUT_BF16, losses=o, dlogits=o)
     with pytest.raises(ValueError):
         ops.linear_cross_entropy(art, p, w.data_ptr(), tgt.data_ptr(), 8, 32, 64, x_dtype=OUT_BF16, w_dtype=3)
+    with pytest.raises(ValueError, match="captured"):
+        ops.linear_cross_entropy(art, p, w.data_ptr(), tgt.data_ptr(), 8, 32, 64, x_dtype=OUT_BF16, scratch=art.alloc(1 << 20))
     art.synchronize()
