@@ -357,11 +357,12 @@ __device__ __forceinline__ uint4 edge_group(const DistillParams& p, const RowSpa
 }
 
 // Rows of more than 64 KB, at least one for every SM: one CTA per row, two an SM.  The row is streamed twice, for the
-// statistics and for the gradient; the second time L2 still has most of it (two rows an SM under way are 76 MB of a
-// 128000-word bf16 batch).  Each thread's 16-byte groups arrive in batches through its own slots of a ring in shared memory,
-// asked for two batches ahead and through both passes, so loads do not stop at the barriers between them.
-// 4096 x 128000 bf16 with gradient: 430 us (4.9 TB/s; 510 us with clusters and the row in shared memory, 640 us with the row
-// in registers); 2048 x 50257 f32, losses alone: 71 us (5.8 TB/s).
+// statistics and for the gradient.  Each thread's 16-byte groups arrive in batches through its own slots of a ring in shared
+// memory, asked for two batches ahead; the last three batches are still there for the second pass, the others come from L2
+// or, where the rows under way (76 MB of a 128000-word bf16 batch) have pushed them out, from HBM again.
+// On one B200, 4096 x 128000 bf16 with gradient: 454 us (2.1 GB once each way, 4.6 TB/s; HBM itself at 5.4 TB/s with what
+// comes twice), 473 us with the ring through both passes, 560 us with clusters that keep fewer rows under way, 640 us with the
+// row in the registers of a cluster.  2048 x 50257 f32, losses alone: 80 us (5.2 TB/s).
 constexpr int kStreamThreads = 512, kRingBatch = 4, kRingBatches = 3;
 template <typename IN, typename OUT>
 __global__ void __launch_bounds__(kStreamThreads, 2) topk_distill_stream_kernel(const DistillParams p) {
@@ -376,12 +377,11 @@ __global__ void __launch_bounds__(kStreamThreads, 2) topk_distill_stream_kernel(
     const IN* zr = static_cast<const IN*>(p.logits) + span.e0;
     const uint4* zg = span.at(p);
     const uint32_t batches = (span.groups + T * B - 1) / (T * B);
-    const uint32_t total = p.dlogits ? 2 * batches : batches;
-    // Batch n of the stream (the second pass repeats the first) goes to ring batch n % S; always one group of copies, empty
-    // or not, so that "all but the last S - 1 groups" is the batch in turn.
+    // Batch n goes to ring batch n % S; always one group of copies, empty or not, so that "all but the last S - 1 groups" is
+    // the batch in turn.
     auto ask = [&](uint32_t n) {
-        if (n < total) {
-            const uint32_t first = (n < batches ? n : n - batches) * (B * T) + tid;
+        if (n < batches) {
+            const uint32_t first = n * (B * T) + tid;
             const uint32_t slot = (n % S) * B;
 #pragma unroll
             for (int u = 0; u < B; ++u)
@@ -474,16 +474,30 @@ __global__ void __launch_bounds__(kStreamThreads, 2) topk_distill_stream_kernel(
         for (int e = 0; e < N; ++e)
             if (e < count) store_as(dr + col + e, v[e]);
     }
-    // In place, too, a thread reads and writes its own groups only.
+    // In place, too, a thread reads and writes its own groups only.  The last S batches are still in the ring; the reads of
+    // the others let go of their lines in L2, and the next batch is under way while one is used.
+    const uint32_t from_l2 = batches > S ? batches - S : 0;
+    uint4 next[B];
+    auto fetch = [&](uint32_t n) {
+#pragma unroll
+        for (int u = 0; u < B; ++u) {
+            const uint32_t i = n * (B * T) + u * T + tid;
+            if (n < from_l2) next[u] = __ldcs(zg + i);   // a batch with others behind it is whole
+            else if (i < span.groups) next[u] = ring[((n % S) * B + u) * T + tid];
+        }
+    };
+    fetch(0);
     for (uint32_t n = 0; n < batches; ++n) {
-        ask(n + batches + S - 1);
-        __pipeline_wait_prior(S - 1);
-        const uint32_t first = n * (B * T) + tid, slot = ((n + batches) % S) * B;
+        uint4 raw[B];
+#pragma unroll
+        for (int u = 0; u < B; ++u) raw[u] = next[u];
+        fetch(n + 1);
+        const uint32_t first = n * (B * T) + tid;
 #pragma unroll
         for (int u = 0; u < B; ++u)
             if (first + u * T < span.groups) {
                 float v[N];
-                gradient(ring[(slot + u) * T + tid], v);
+                gradient(raw[u], v);
                 store_group(dg + static_cast<size_t>(first + u * T) * N, v);
             }
     }
