@@ -205,10 +205,10 @@ __device__ __forceinline__ float group_max(const uint4& q, const __nv_bfloat16*)
     return fmaxf(__low2float(m), __high2float(m));
 }
 
-// The teacher's side of a row in one CTA: each thread owns the words tid, tid + T, ... (at most 1024 in all).
-template <int T>
+// The teacher's side of a row in one CTA of T threads: each owns the words tid, tid + T, ..., kOwn of them at most (one,
+// where the call's topk allows it: three registers a word).
+template <int T, int kOwn>
 struct Words {
-    static constexpr int kOwn = T0B_MAX_TOPK / T;
     uint32_t id[kOwn];
     float t[kOwn], z[kOwn];   // t: the teacher's logit, then q
     float tmax;
@@ -364,8 +364,10 @@ __device__ __forceinline__ uint4 edge_group(const DistillParams& p, const RowSpa
 // comes twice), 473 us with the ring through both passes, 560 us with clusters that keep fewer rows under way, 640 us with the
 // row in the registers of a cluster.  2048 x 50257 f32, losses alone: 80 us (5.2 TB/s).
 constexpr int kStreamThreads = 512, kRingBatch = 4, kRingBatches = 3;
-template <typename IN, typename OUT>
+template <typename IN, typename OUT, int OWN>
 __global__ void __launch_bounds__(kStreamThreads, 2) topk_distill_stream_kernel(const DistillParams p) {
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
     constexpr int N = Vec<IN>::kN, T = kStreamThreads, B = kRingBatch, S = kRingBatches;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float2 red_max[T / 32], red_sum[T / 32], red_loss[T / 32];
@@ -391,7 +393,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) topk_distill_stream_kernel(
     };
 #pragma unroll
     for (int n = 0; n < S - 1; ++n) ask(n);
-    Words<T> words;
+    Words<T, OWN> words;
     words.load(p, row, zr, true);
 
     // This thread's running maximum and sum.
@@ -508,12 +510,14 @@ __global__ void __launch_bounds__(kStreamThreads, 2) topk_distill_stream_kernel(
 // The fast form: base pointers on 16-byte boundaries (any pitch).  A row's whole
 // 16-byte groups are divided among the cluster's threads, G to each at most, and the partial groups at its two ends go to
 // one thread each (an extra group that only their warps look at).
-template <typename IN, typename OUT, int G>
-__global__ void __launch_bounds__(kThreads, G == 16 ? 2 : (G == 8 ? 3 : 4)) topk_distill_kernel(const DistillParams p) {
+template <typename IN, typename OUT, int G, int T, int OWN>
+__global__ void __launch_bounds__(T, (G == 16 ? 2 : (G == 8 ? 3 : 4)) * 256 / T) topk_distill_kernel(const DistillParams p) {
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
     constexpr int N = Vec<IN>::kN;
     constexpr bool kKeepExp = !(sizeof(IN) == 2 && sizeof(OUT) == 4);
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float2 red_max[kThreads / 32], red_sum[kThreads / 32], red_loss[kThreads / 32];
+    __shared__ float2 red_max[T / 32], red_sum[T / 32], red_loss[T / 32];
     __shared__ __align__(16) float2 xch[kMaxCluster];
     uint32_t* ids = reinterpret_cast<uint32_t*>(smem);
     float* q = reinterpret_cast<float*>(ids + p.topk);
@@ -534,19 +538,19 @@ __global__ void __launch_bounds__(kThreads, G == 16 ? 2 : (G == 8 ? 3 : 4)) topk
     uint4 raw[G];
 #pragma unroll
     for (int i = 0; i < G; ++i)
-        if (tid + i * kThreads < n_own) raw[i] = __ldcs(zg + tid + i * kThreads);
+        if (tid + i * T < n_own) raw[i] = __ldcs(zg + tid + i * T);
     uint4 edge = make_uint4(0, 0, 0, 0);
     if (has_edge) edge = edge_group<IN>(p, span, at_back);
-    Words<kThreads> words;
+    Words<T, OWN> words;
     words.load(p, row, zr, rank == 0);
 
     // Maximum of the slice (and of the teacher's logits), over the CTA.
     float m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < G; ++i)
-        if (tid + i * kThreads < n_own) m = fmaxf(m, group_max(raw[i], static_cast<const IN*>(nullptr)));
+        if (tid + i * T < n_own) m = fmaxf(m, group_max(raw[i], static_cast<const IN*>(nullptr)));
     if (has_edge) m = fmaxf(m, group_max(edge, static_cast<const IN*>(nullptr)));
-    block_max2<kThreads>(m, words.tmax, red_max);
+    block_max2<T>(m, words.tmax, red_max);
     // Exponentials relative to it, and their sum.
     const Ref own(m, p.c);
     const bool nothing = m == -INFINITY;   // in this slice
@@ -563,16 +567,16 @@ __global__ void __launch_bounds__(kThreads, G == 16 ? 2 : (G == 8 ? 3 : 4)) topk
     if (own.fused) {
 #pragma unroll
         for (int i = 0; i < G; ++i)
-            if (tid + i * kThreads < n_own) exponentials(raw[i], true);
+            if (tid + i * T < n_own) exponentials(raw[i], true);
     } else {
 #pragma unroll
         for (int i = 0; i < G; ++i)
-            if (tid + i * kThreads < n_own) exponentials(raw[i], false);
+            if (tid + i * T < n_own) exponentials(raw[i], false);
     }
     if (has_edge) exponentials(edge, own.fused);
     const float tref = words.tmax == -INFINITY ? 0.0f : words.tmax;
     float tsum = words.sum(p, tref);
-    block_sum2<kThreads>(s, tsum, red_sum);
+    block_sum2<T>(s, tsum, red_sum);
     bool live = tsum > 0.0f || tsum != tsum;
     float2 cq;
     const RowStats st = exchange(m, s, p.c, nranks, rank, xch, [&] { cq = words.probs(p, tref, tsum, live, ids, q); });
@@ -580,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, G == 16 ? 2 : (G == 8 ? 3 : 4)) topk
     if (st.m == -INFINITY && st.total == 0.0f) live = false;   // every logit is -inf: the row has no distribution
     if (rank == 0 && p.losses) {
         if (live) cq.x += words.cross(p, all);
-        block_sum2<kThreads>(cq.x, cq.y, red_loss);
+        block_sum2<T>(cq.x, cq.y, red_loss);
         if (tid == 0) p.losses[row] = live ? fmaf(cq.y, logf(st.total), cq.x) : 0.0f;
     }
     if (!p.dlogits) return;
@@ -602,10 +606,10 @@ __global__ void __launch_bounds__(kThreads, G == 16 ? 2 : (G == 8 ? 3 : 4)) topk
     };
 #pragma unroll
     for (int i = 0; i < G; ++i)
-        if (tid + i * kThreads < n_own) {
+        if (tid + i * T < n_own) {
             float v[N];
             gradient(raw[i], v);
-            store_group(dg + static_cast<size_t>(tid + i * kThreads) * N, v);
+            store_group(dg + static_cast<size_t>(tid + i * T) * N, v);
         }
     if (has_edge) {
         float v[N];
@@ -626,13 +630,15 @@ __global__ void __launch_bounds__(kThreads, G == 16 ? 2 : (G == 8 ? 3 : 4)) topk
 // Every pass reads the row by element again (from L2, where it fits).
 template <typename IN, typename OUT>
 __global__ void __launch_bounds__(kThreads) topk_distill_any_kernel(const DistillParams p) {
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float2 red_max[kThreads / 32], red_sum[kThreads / 32], red_loss[kThreads / 32];
     uint32_t* ids = reinterpret_cast<uint32_t*>(smem);
     float* q = reinterpret_cast<float*>(ids + p.topk);
     const uint32_t row = blockIdx.x, tid = threadIdx.x;
     const IN* zr = static_cast<const IN*>(p.logits) + row * p.ld;
-    Words<kThreads> words;
+    Words<kThreads, T0B_MAX_TOPK / kThreads> words;
     words.load(p, row, zr, true);
     float m = -INFINITY;
 #pragma unroll 8
@@ -664,26 +670,34 @@ __global__ void __launch_bounds__(kThreads) topk_distill_any_kernel(const Distil
     words.gradient(p, all, a, s, 0, p.cols, ids, q, dr);
 }
 
-template <typename IN, typename OUT, int G>
-int32_t launch_distill(t0b_ctx* ctx, const DistillParams& p, uint32_t rows, uint32_t nranks) {
+// One launch, behind the kernel in front of it in the stream (programmatic: its CTAs may be placed while that one drains).
+template <typename K>
+int32_t launch(t0b_ctx* ctx, K kernel, const DistillParams& p, uint32_t ctas, uint32_t threads, size_t smem, uint32_t cluster) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(rows * nranks);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = p.topk * 8ull;
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = ctx->stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = nranks;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (ctx->pdl) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = cluster;
+        attr[n].val.clusterDim.y = 1;
+        attr[n++].val.clusterDim.z = 1;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return check_cuda(ctx, cudaLaunchKernelEx(&cfg, topk_distill_kernel<IN, OUT, G>, p), "cudaLaunchKernelEx(topk_distill)");
+    cfg.numAttrs = n;
+    return check_cuda(ctx, cudaLaunchKernelEx(&cfg, kernel, p), "cudaLaunchKernelEx(topk_distill)");
 }
 
-template <typename IN, typename OUT>
+template <typename IN, typename OUT, int OWN>
 int32_t launch_stream(t0b_ctx* ctx, const DistillParams& p, uint32_t rows) {
-    auto kfn = topk_distill_stream_kernel<IN, OUT>;
+    auto kfn = topk_distill_stream_kernel<IN, OUT, OWN>;
     constexpr size_t kRing = static_cast<size_t>(kRingBatch) * kRingBatches * kStreamThreads * 16;
     static std::atomic<bool> configured[64];
     std::atomic<bool>& done = configured[ctx->device & 63];
@@ -692,8 +706,20 @@ int32_t launch_stream(t0b_ctx* ctx, const DistillParams& p, uint32_t rows) {
         if (rc != T0B_OK) return rc;
         done.store(true, std::memory_order_release);
     }
-    kfn<<<rows, kStreamThreads, kRing + p.topk * 8ull, ctx->stream>>>(p);
-    return check_cuda(ctx, cudaGetLastError(), "topk_distill launch");
+    return launch(ctx, kfn, p, rows, kStreamThreads, kRing + p.topk * 8ull, 1);
+}
+
+// Rows in registers, G groups a thread: the smallest G that holds the slice.
+template <typename IN, typename OUT, int T, int OWN>
+int32_t launch_registers(t0b_ctx* ctx, const DistillParams& p, uint32_t rows, uint32_t nranks) {
+    const uint32_t g = (p.groups_per_cta + T - 1) / T, ctas = rows * nranks;
+    const size_t smem = p.topk * 8ull;
+    if (g <= 2) return launch(ctx, topk_distill_kernel<IN, OUT, 2, T, OWN>, p, ctas, T, smem, nranks);
+    if (g <= 4) return launch(ctx, topk_distill_kernel<IN, OUT, 4, T, OWN>, p, ctas, T, smem, nranks);
+    if constexpr (T == kThreads) {
+        if (g > 8) return launch(ctx, topk_distill_kernel<IN, OUT, 16, T, OWN>, p, ctas, T, smem, nranks);
+    }
+    return launch(ctx, topk_distill_kernel<IN, OUT, 8, T, OWN>, p, ctas, T, smem, nranks);
 }
 
 template <typename IN, typename OUT>
@@ -701,22 +727,22 @@ int32_t run_distill(t0b_ctx* ctx, DistillParams p, uint32_t rows) {
     constexpr uint32_t N = Vec<IN>::kN;
     const uint32_t groups = p.cols / N + 1;
     const bool aligned = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && reinterpret_cast<uintptr_t>(p.dlogits) % std::min<size_t>(16, N * sizeof(OUT)) == 0;
-    if (!aligned) {
-        topk_distill_any_kernel<IN, OUT><<<rows, kThreads, p.topk * 8ull, ctx->stream>>>(p);
-        return check_cuda(ctx, cudaGetLastError(), "topk_distill launch");
-    }
+    if (!aligned) return launch(ctx, topk_distill_any_kernel<IN, OUT>, p, rows, kThreads, p.topk * 8ull, 1);
     // Rows that one CTA's registers hold stay there.  Longer ones are streamed when there is one for every SM (1001 x 32003
     // f32: 63 us against 69 us for clusters of two); with fewer rows clusters of CTAs share them: enough that a thread's
     // groups fit its registers, and more while SMs would idle and every thread still has two groups (24 x 32000 f32: 5.6 us).
-    if (groups > kThreads * 16 && (rows >= static_cast<uint32_t>(ctx->num_sms) || groups > kMaxCluster * kThreads * 16)) return launch_stream<IN, OUT>(ctx, p, rows);
+    if (groups > kThreads * 16 && (rows >= static_cast<uint32_t>(ctx->num_sms) || groups > kMaxCluster * kThreads * 16)) {
+        return p.topk <= kStreamThreads ? launch_stream<IN, OUT, 1>(ctx, p, rows) : launch_stream<IN, OUT, T0B_MAX_TOPK / kStreamThreads>(ctx, p, rows);
+    }
     uint32_t nranks = 1;
     while (groups > nranks * kThreads * 16) nranks *= 2;
     while (nranks < kMaxCluster && static_cast<uint64_t>(rows) * nranks < static_cast<uint64_t>(ctx->num_sms) && groups >= nranks * kThreads * 4) nranks *= 2;
+    if (static_cast<uint64_t>(rows) * nranks > 0x7fffffffull) return set_error(ctx, T0B_ERR_INVALID, "topk_distill: %u rows are too many", rows);
     p.groups_per_cta = (groups + nranks - 1) / nranks;
-    if (p.groups_per_cta <= 2 * kThreads) return launch_distill<IN, OUT, 2>(ctx, p, rows, nranks);
-    if (p.groups_per_cta <= 4 * kThreads) return launch_distill<IN, OUT, 4>(ctx, p, rows, nranks);
-    if (p.groups_per_cta <= 8 * kThreads) return launch_distill<IN, OUT, 8>(ctx, p, rows, nranks);
-    return launch_distill<IN, OUT, 16>(ctx, p, rows, nranks);
+    // Short rows, many of them: CTAs of 128 threads, so that more rows are under way on an SM.
+    if (nranks == 1 && groups <= 128 * 8 && p.topk <= 128 && rows >= 4u * static_cast<uint32_t>(ctx->num_sms)) return launch_registers<IN, OUT, 128, 1>(ctx, p, rows, 1);
+    return p.topk <= kThreads ? launch_registers<IN, OUT, kThreads, 1>(ctx, p, rows, nranks)
+                              : launch_registers<IN, OUT, kThreads, T0B_MAX_TOPK / kThreads>(ctx, p, rows, nranks);
 }
 
 }  // namespace
