@@ -152,6 +152,7 @@ struct DistillParams {
     unsigned long long ld, ldk;
     float c, inv_t;          // log2(e) / T and 1 / T
     float scale;             // of the gradient, 1 / T included
+    uint32_t table;          // slots of the words' hash table, 0: none
     uint32_t groups_per_cta; // 16-byte groups of one CTA's slice (rows in registers)
     int* status;
 };
@@ -212,6 +213,29 @@ struct Words {
     uint32_t id[kOwn];
     float t[kOwn], z[kOwn];   // t: the teacher's logit, then q
     float tmax;
+
+    // A hash table of the row's words (`size` slots, a power of two, at least twice the words; kNoWord = free) finds out
+    // whether a word is named twice: clear() before one block-wide barrier, mark() behind it, `twice` is valid behind the
+    // next.  Without slots every row counts as one with a word named twice.
+    static __device__ __forceinline__ void clear(uint32_t* table, uint32_t size, int* twice) {
+        for (uint32_t i = threadIdx.x; i < size; i += T) table[i] = kNoWord;
+        if (threadIdx.x == 0) *twice = size == 0;
+    }
+    __device__ __forceinline__ void mark(const DistillParams& p, uint32_t* table, uint32_t size, int* twice) const {
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+            if (mine(p, i) && id[i] != kNoWord) {
+                uint32_t at = (id[i] * 2654435761u) & (size - 1);   // the high bits of the product do not matter: ids are spread
+                uint32_t old;
+                while ((old = atomicCAS(table + at, kNoWord, id[i])) != kNoWord) {   // ends: at most half of the slots are taken
+                    if (old == id[i]) {
+                        *twice = 1;
+                        break;
+                    }
+                    at = (at + 1) & (size - 1);
+                }
+            }
+    }
 
     // Warps beyond the last word skip all of it.
     static __device__ __forceinline__ bool mine(const DistillParams& p, int i) { return i * T + (threadIdx.x & ~31u) < p.topk; }
@@ -279,22 +303,23 @@ struct Words {
             if (mine(p, i) && t[i] != 0.0f) c -= t[i] * all.log_of(z[i], p.c, p.inv_t);
         return c;
     }
-    // The gradient at the words of columns [c_lo, c_hi): one thread per distinct word writes a (p - its q).
+    // The gradient at the words of columns [c_lo, c_hi): one thread per distinct word writes a (p - its q).  Only where a word
+    // may be named twice do the threads look through all of them.
     template <typename OUT>
     __device__ __forceinline__ void gradient(const DistillParams& p, const Ref& all, float a, float total, long long c_lo, long long c_hi,
-                                             const uint32_t* sh_ids, const float* sh_q, OUT* dr) const {
+                                             const uint32_t* sh_ids, const float* sh_q, bool twice, OUT* dr) const {
 #pragma unroll
         for (int i = 0; i < kOwn; ++i)
             if (mine(p, i) && id[i] != kNoWord && id[i] >= c_lo && id[i] < c_hi) {
                 const uint32_t k = threadIdx.x + i * T;
-                bool first = true;
-#pragma unroll 8
-                for (uint32_t j = 0; j < k; ++j) first = first && sh_ids[j] != id[i];
-                if (!first) continue;
                 float qk = t[i];
-#pragma unroll 8
-                for (uint32_t j = k + 1; j < p.topk; ++j)
-                    if (sh_ids[j] == id[i]) qk += sh_q[j];
+                if (twice) {
+                    bool first = true;
+                    for (uint32_t j = 0; j < k; ++j) first = first && sh_ids[j] != id[i];
+                    if (!first) continue;
+                    for (uint32_t j = k + 1; j < p.topk; ++j)
+                        if (sh_ids[j] == id[i]) qk += sh_q[j];
+                }
                 store_as(dr + id[i], a * (exp2_approx(all.arg(z[i], p.c)) / total - qk));
             }
     }
@@ -360,9 +385,9 @@ __device__ __forceinline__ uint4 edge_group(const DistillParams& p, const RowSpa
 // statistics and for the gradient.  Each thread's 16-byte groups arrive in batches through its own slots of a ring in shared
 // memory, asked for two batches ahead; the last three batches are still there for the second pass, the others come from L2
 // or, where the rows under way (76 MB of a 128000-word bf16 batch) have pushed them out, from HBM again.
-// On one B200, 4096 x 128000 bf16 with gradient: 454 us (2.1 GB once each way, 4.6 TB/s; HBM itself at 5.4 TB/s with what
-// comes twice), 473 us with the ring through both passes, 560 us with clusters that keep fewer rows under way, 640 us with the
-// row in the registers of a cluster.  2048 x 50257 f32, losses alone: 80 us (5.2 TB/s).
+// On one B200, 4096 x 128000 bf16 with gradient: 430 us (2.1 GB read and written once, 4.9 TB/s; HBM moves more with what
+// comes twice), 455 us with the ring through both passes, 560 us with clusters that keep fewer rows under way, 640 us with the
+// row in the registers of a cluster.  2048 x 50257 f32, losses alone: 75 us (5.5 TB/s).
 constexpr int kStreamThreads = 512, kRingBatch = 4, kRingBatches = 3;
 template <typename IN, typename OUT, int OWN>
 __global__ void __launch_bounds__(kStreamThreads, 2) topk_distill_stream_kernel(const DistillParams p) {
@@ -504,7 +529,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) topk_distill_stream_kernel(
             }
     }
     __syncthreads();   // the words after their neighbours
-    if (live) words.gradient(p, all, a, s, 0, p.cols, ids, q, dr);
+    if (live) words.gradient(p, all, a, s, 0, p.cols, ids, q, true, dr);
 }
 
 // The fast form: base pointers on 16-byte boundaries (any pitch).  A row's whole
@@ -521,6 +546,8 @@ __global__ void __launch_bounds__(T, (G == 16 ? 2 : (G == 8 ? 3 : 4)) * 256 / T)
     __shared__ __align__(16) float2 xch[kMaxCluster];
     uint32_t* ids = reinterpret_cast<uint32_t*>(smem);
     float* q = reinterpret_cast<float*>(ids + p.topk);
+    uint32_t* table = reinterpret_cast<uint32_t*>(q + p.topk);
+    __shared__ int twice;
     uint32_t nranks;
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(nranks));
     const uint32_t rank = ptx::cluster_ctarank();
@@ -543,6 +570,7 @@ __global__ void __launch_bounds__(T, (G == 16 ? 2 : (G == 8 ? 3 : 4)) * 256 / T)
     if (has_edge) edge = edge_group<IN>(p, span, at_back);
     Words<T, OWN> words;
     words.load(p, row, zr, rank == 0);
+    words.clear(table, p.table, &twice);
 
     // Maximum of the slice (and of the teacher's logits), over the CTA.
     float m = -INFINITY;
@@ -551,6 +579,7 @@ __global__ void __launch_bounds__(T, (G == 16 ? 2 : (G == 8 ? 3 : 4)) * 256 / T)
         if (tid + i * T < n_own) m = fmaxf(m, group_max(raw[i], static_cast<const IN*>(nullptr)));
     if (has_edge) m = fmaxf(m, group_max(edge, static_cast<const IN*>(nullptr)));
     block_max2<T>(m, words.tmax, red_max);
+    if (p.table) words.mark(p, table, p.table, &twice);
     // Exponentials relative to it, and their sum.
     const Ref own(m, p.c);
     const bool nothing = m == -INFINITY;   // in this slice
@@ -623,7 +652,7 @@ __global__ void __launch_bounds__(T, (G == 16 ? 2 : (G == 8 ? 3 : 4)) * 256 / T)
     __syncthreads();   // the words after their neighbours
     const long long c_lo = (rank == 0 ? 0 : static_cast<long long>(span.front) + static_cast<long long>(lo) * N);
     const long long c_hi = (rank == nranks - 1 ? p.cols : static_cast<long long>(span.front) + static_cast<long long>(lo + n_own) * N);
-    words.gradient(p, all, a, st.total, c_lo, c_hi, ids, q, dr);
+    words.gradient(p, all, a, st.total, c_lo, c_hi, ids, q, twice != 0, dr);
 }
 
 // The general form, one CTA per row: base pointers off their 16-byte boundaries, or rows longer than a cluster's registers.
@@ -667,8 +696,10 @@ __global__ void __launch_bounds__(kThreads) topk_distill_any_kernel(const Distil
     for (uint32_t i = tid; i < p.cols; i += kThreads) store_as(dr + i, live ? exp2_approx(all.arg(to_float(zr[i]), p.c)) * inv : 0.0f);
     if (!live) return;
     __syncthreads();
-    words.gradient(p, all, a, s, 0, p.cols, ids, q, dr);
+    words.gradient(p, all, a, s, 0, p.cols, ids, q, true, dr);
 }
+
+size_t words_bytes(const DistillParams& p) { return p.topk * 8ull + p.table * 4ull; }   // ids, q and the hash table
 
 // One launch, behind the kernel in front of it in the stream (programmatic: its CTAs may be placed while that one drains).
 template <typename K>
@@ -706,14 +737,14 @@ int32_t launch_stream(t0b_ctx* ctx, const DistillParams& p, uint32_t rows) {
         if (rc != T0B_OK) return rc;
         done.store(true, std::memory_order_release);
     }
-    return launch(ctx, kfn, p, rows, kStreamThreads, kRing + p.topk * 8ull, 1);
+    return launch(ctx, kfn, p, rows, kStreamThreads, kRing + words_bytes(p), 1);
 }
 
 // Rows in registers, G groups a thread: the smallest G that holds the slice.
 template <typename IN, typename OUT, int T, int OWN>
 int32_t launch_registers(t0b_ctx* ctx, const DistillParams& p, uint32_t rows, uint32_t nranks) {
     const uint32_t g = (p.groups_per_cta + T - 1) / T, ctas = rows * nranks;
-    const size_t smem = p.topk * 8ull;
+    const size_t smem = words_bytes(p);
     if (g <= 2) return launch(ctx, topk_distill_kernel<IN, OUT, 2, T, OWN>, p, ctas, T, smem, nranks);
     if (g <= 4) return launch(ctx, topk_distill_kernel<IN, OUT, 4, T, OWN>, p, ctas, T, smem, nranks);
     if constexpr (T == kThreads) {
@@ -727,9 +758,9 @@ int32_t run_distill(t0b_ctx* ctx, DistillParams p, uint32_t rows) {
     constexpr uint32_t N = Vec<IN>::kN;
     const uint32_t groups = p.cols / N + 1;
     const bool aligned = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && reinterpret_cast<uintptr_t>(p.dlogits) % std::min<size_t>(16, N * sizeof(OUT)) == 0;
-    if (!aligned) return launch(ctx, topk_distill_any_kernel<IN, OUT>, p, rows, kThreads, p.topk * 8ull, 1);
+    if (!aligned) return launch(ctx, topk_distill_any_kernel<IN, OUT>, p, rows, kThreads, words_bytes(p), 1);
     // Rows that one CTA's registers hold stay there.  Longer ones are streamed when there is one for every SM (1001 x 32003
-    // f32: 63 us against 69 us for clusters of two); with fewer rows clusters of CTAs share them: enough that a thread's
+    // f32: 58 us against 69 us for clusters of two); with fewer rows clusters of CTAs share them: enough that a thread's
     // groups fit its registers, and more while SMs would idle and every thread still has two groups (24 x 32000 f32: 5.6 us).
     if (groups > kThreads * 16 && (rows >= static_cast<uint32_t>(ctx->num_sms) || groups > kMaxCluster * kThreads * 16)) {
         return p.topk <= kStreamThreads ? launch_stream<IN, OUT, 1>(ctx, p, rows) : launch_stream<IN, OUT, T0B_MAX_TOPK / kStreamThreads>(ctx, p, rows);
@@ -739,7 +770,14 @@ int32_t run_distill(t0b_ctx* ctx, DistillParams p, uint32_t rows) {
     while (nranks < kMaxCluster && static_cast<uint64_t>(rows) * nranks < static_cast<uint64_t>(ctx->num_sms) && groups >= nranks * kThreads * 4) nranks *= 2;
     if (static_cast<uint64_t>(rows) * nranks > 0x7fffffffull) return set_error(ctx, T0B_ERR_INVALID, "topk_distill: %u rows are too many", rows);
     p.groups_per_cta = (groups + nranks - 1) / nranks;
-    // Short rows, many of them: CTAs of 128 threads, so that more rows are under way on an SM.
+    // The table takes 4000 x 9000 f32 with 100 words from 110 to 98 us; for up to four words the search costs no more (1127 x 1920
+    // bf16, one word: 10.4 us either way), and streamed rows lose by it (4096 x 128000 bf16: 437 and 469 us).
+    if (p.dlogits && p.topk > 4) {
+        p.table = 32;
+        while (p.table < 2 * p.topk) p.table *= 2;
+    }
+    // Short rows, many of them: CTAs of 128 threads, so that more rows are under way on an SM (8000 x 1000 f32: 24 us, 55 us
+    // with 256 threads).
     if (nranks == 1 && groups <= 128 * 8 && p.topk <= 128 && rows >= 4u * static_cast<uint32_t>(ctx->num_sms)) return launch_registers<IN, OUT, 128, 1>(ctx, p, rows, 1);
     return p.topk <= kThreads ? launch_registers<IN, OUT, kThreads, 1>(ctx, p, rows, nranks)
                               : launch_registers<IN, OUT, kThreads, T0B_MAX_TOPK / kThreads>(ctx, p, rows, nranks);

@@ -381,6 +381,22 @@ def test_topk_distill_same_word_twice(th, art):
     assert ((dx.double() - dz @ w.double()).abs() <= edz @ w.double().abs() + 1e-5).all()
 
 
+@pytest.mark.parametrize("rows,cols,topk,offset", [(700, 1000, 20, 0), (3, 32000, 200, 0), (5, 50257, 1024, 0), (150, 40000, 64, 0), (150, 40000, 1000, 0), (4, 3000, 300, 1)])
+def test_topk_distill_same_word_twice_in_every_form(th, art, rows, cols, topk, offset):
+    """Rows with no word twice, with one pair, with many and with one word alone, next to each other; a stride of 2^k between
+    words that differ."""
+    g = th.Generator(device="cuda")
+    g.manual_seed(rows + cols)
+    ids = th.stack([th.randperm(cols, device="cuda", generator=g)[:topk] for _ in range(rows)]).to(th.int32)
+    ids[0, -1] = ids[0, 0]
+    ids[1] = cols - 1
+    ids[2] %= 7
+    if rows > 3:
+        ids[3] = th.arange(topk, device="cuda", dtype=th.int32) * 512 % cols
+    teacher = th.randn((rows, topk), device="cuda", generator=g) * 2
+    check_logits(th, art, rows, cols, topk, ids=ids, teacher=teacher, offset=offset)
+
+
 # ------------------------------------------------------------------------------------------- in a user's program
 
 @pytest.mark.parametrize("rows,d,V", [(64, 256, 1000), (300, 128, 2048)])
