@@ -11,7 +11,9 @@
  *   - after any CUDA error the context is "poisoned" and refuses further launches, as the reference's
  *     GpuRuntime does after a queue timeout (src/ignis/gpu_context.rs:149-157, 270-272, 284-287).
  *   - there is no CPU fallback: without a CUDA device t0b_ctx_create fails.
- *   - a context is thread-safe; all launches of a context go to one CUDA stream.
+ *   - a context is thread-safe; all launches of a context go to one CUDA stream.  On the context's own stream a
+ *     synchronous launch (is_async = 0) starts behind the work that the device's default stream holds; asynchronous ones,
+ *     and all on a stream of the caller's (t0b_ctx_set_stream), are ordered against other streams by the caller.
  */
 #ifndef T0B200_H
 #define T0B200_H

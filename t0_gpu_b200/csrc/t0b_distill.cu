@@ -790,7 +790,7 @@ extern "C" {
 int32_t t0b_topk_distill(t0b_ctx* ctx, uint64_t logits, int32_t logits_dtype, uint64_t ids, uint64_t teacher, uint64_t row_weights,
                          uint64_t losses, uint64_t dlogits, int32_t grad_dtype, uint32_t rows, uint32_t cols, uint64_t ld,
                          uint32_t topk, uint64_t ldk, float temperature, float scale, int32_t async) try {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (rows == 0) return T0B_OK;
     if (logits_dtype != T0B_OUT_F32 && logits_dtype != T0B_OUT_BF16) return set_error(ctx, T0B_ERR_INVALID, "topk_distill: unknown logits_dtype %d", logits_dtype);

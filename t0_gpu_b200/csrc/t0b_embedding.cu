@@ -138,7 +138,7 @@ extern "C" {
 
 int32_t t0b_embedding_fwd(t0b_ctx* ctx, uint64_t table, uint64_t ids, uint64_t out, uint32_t num_tokens, uint32_t dim,
                           uint32_t vocab, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (num_tokens == 0 || dim == 0) return T0B_OK;
     if (!table || !ids || !out || vocab == 0) return set_error(ctx, T0B_ERR_INVALID, "embedding_fwd: null pointer or empty table");
@@ -161,7 +161,7 @@ size_t t0b_embedding_bwd_scratch_bytes(uint32_t num_tokens) {
 
 int32_t t0b_embedding_bwd(t0b_ctx* ctx, uint64_t grad_table, uint64_t ids, uint64_t grad_out, uint32_t num_tokens, uint32_t dim,
                           uint32_t vocab, uint64_t scratch, size_t scratch_bytes, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (num_tokens == 0 || dim == 0) return T0B_OK;
     if (!grad_table || !ids || !grad_out || vocab == 0)

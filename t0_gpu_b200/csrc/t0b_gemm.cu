@@ -637,7 +637,7 @@ int32_t t0b_gemm(t0b_ctx* ctx, const t0b_gemm_config* cfg, int32_t trans_a, int3
                  uint64_t c, uint32_t m, uint32_t n, uint32_t k, uint64_t lda, uint64_t ldb, uint64_t ldc,
                  int32_t out_dtype, int32_t epilogue, uint64_t bias, float alpha, uint64_t workspace,
                  size_t workspace_bytes, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     std::lock_guard<std::recursive_mutex> lk(ctx->mu);
     GemmCall g{};
@@ -657,7 +657,7 @@ int32_t t0b_gemm_chain(t0b_ctx* ctx, const t0b_gemm_config* cfg, int32_t trans_a
                        uint64_t c, uint32_t m, uint32_t n, uint32_t k, uint64_t lda, uint64_t ldb, uint64_t ldc,
                        int32_t out_dtype, const int32_t* ops, int32_t n_ops, uint64_t bias, float scale, float clamp_min,
                        float clamp_max, uint64_t workspace, size_t workspace_bytes, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (n_ops < 0 || (n_ops > 0 && !ops)) return set_error(ctx, T0B_ERR_INVALID, "gemm_chain: bad operation list");
     if (out_dtype != T0B_OUT_F32 && out_dtype != T0B_OUT_BF16) return set_error(ctx, T0B_ERR_INVALID, "gemm: unknown out_dtype %d", out_dtype);
@@ -828,7 +828,7 @@ int32_t t0b_multi_dst_config(uint32_t m, uint32_t k, uint32_t n_local, int32_t n
 int32_t t0b_gemm_multi_dst(t0b_ctx* ctx, const t0b_gemm_config* cfg, int32_t trans_a, int32_t trans_b, uint64_t a,
                            uint64_t b, const uint64_t* c_dsts, int32_t n_dst, uint32_t m, uint32_t n_local, uint32_t k,
                            uint64_t lda, uint64_t ldb, uint64_t ldc, uint64_t col0, int32_t out_dtype, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (!c_dsts || n_dst < 1 || n_dst > kMaxDst) return set_error(ctx, T0B_ERR_INVALID, "gemm_multi_dst: 1..%d destinations", kMaxDst);
     if (col0 + n_local > ldc) return set_error(ctx, T0B_ERR_INVALID, "gemm_multi_dst: column block exceeds the row pitch");
@@ -855,7 +855,7 @@ int32_t t0b_gemm_multi_dst(t0b_ctx* ctx, const t0b_gemm_config* cfg, int32_t tra
 
 int32_t t0b_gemm_slabs(t0b_ctx* ctx, const t0b_gemm_config* cfg, uint64_t x, uint64_t wt, uint64_t y, uint32_t m,
                        uint32_t n, uint32_t k, uint32_t split_k, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (split_k == 0 || (split_k & (split_k - 1)) != 0)
         return set_error(ctx, T0B_ERR_INVALID, "gemm_slabs: split_k=%u must be a power of 2", split_k);
@@ -875,7 +875,7 @@ int32_t t0b_gemm_slabs(t0b_ctx* ctx, const t0b_gemm_config* cfg, uint64_t x, uin
 int32_t t0b_splitk_reduce(t0b_ctx* ctx, uint64_t partial, uint32_t split_k, uint32_t m, uint32_t n,
                           uint64_t slab_stride_elems, uint64_t ld_partial, uint64_t c, uint64_t ldc, int32_t out_dtype,
                           int32_t epilogue, uint64_t bias, float alpha, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (!partial || !c || split_k == 0) return set_error(ctx, T0B_ERR_INVALID, "splitk_reduce: null pointer or zero split");
     if (m == 0 || n == 0) return T0B_OK;
@@ -892,7 +892,7 @@ int32_t t0b_splitk_reduce(t0b_ctx* ctx, uint64_t partial, uint32_t split_k, uint
 
 int32_t t0b_dispatch_kernargs(t0b_ctx* ctx, const t0b_gemm_config* cfg, uint32_t grid_x, uint32_t grid_y,
                               const uint8_t* ka, size_t len, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (!cfg || !ka) return set_error(ctx, T0B_ERR_INVALID, "dispatch_kernargs: null config or kernargs");
     if (len != 40 && len != 44 && len != 48)
@@ -947,7 +947,7 @@ int32_t t0b_dispatch_kernargs(t0b_ctx* ctx, const t0b_gemm_config* cfg, uint32_t
 
 int32_t t0b_tile_dispatch(t0b_ctx* ctx, const t0b_tile_gemm* spec, const uint32_t grid[3], const uint8_t* ka, size_t len,
                           int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (!spec || !grid || !ka) return set_error(ctx, T0B_ERR_INVALID, "tile_dispatch: null spec, grid or kernargs");
     if (!tile_spec_valid(spec)) return set_error(ctx, T0B_ERR_INVALID, "tile_dispatch: invalid TileGemm spec");

@@ -31,6 +31,7 @@ struct t0b_ctx {
     int sm_limit = 0;           // > 0: the persistent GEMM kernels occupy at most this many SMs
     cudaStream_t own_stream = nullptr;
     cudaStream_t stream = nullptr;
+    cudaEvent_t default_event = nullptr;   // the default stream's work that a synchronous call waits for
     std::recursive_mutex mu;
     std::string last_error;
     bool poisoned = false;
@@ -98,7 +99,7 @@ constexpr int kDevBadIndex = 110;
 // on the device.  (Pointers from elsewhere, or into the middle of a buffer, are not known; null ones are skipped.)
 struct Extent { const char* name; uint64_t ptr; uint64_t bytes; };
 int32_t check_fits(t0b_ctx* ctx, const char* what, std::initializer_list<Extent> extents);
-int32_t precheck(t0b_ctx* ctx);                 // null / poisoned checks, sets the device
+int32_t precheck(t0b_ctx* ctx, int32_t async = 1);   // null / poisoned checks, sets the device; a synchronous call waits for the default stream
 // Launch-error check (+ sync and status-word check when !async). `count` kernels are added to the launch counter.
 int32_t finish(t0b_ctx* ctx, int32_t async, const char* what, int count = 1);
 // Read the status word; a non-zero code is moved to ctx->last_status and the word is cleared, so one failed kernel is

@@ -907,7 +907,7 @@ size_t t0b_linear_loss_scratch_bytes(t0b_ctx* ctx, const t0b_linear_loss* loss, 
 
 // No C++ exception (the host's memory running out) leaves a C entry.
 int32_t t0b_linear_ce(t0b_ctx* ctx, const t0b_linear_loss* loss, uint64_t targets, int32_t async) try {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (!loss || !targets || targets % 4) return set_error(ctx, T0B_ERR_INVALID, "linear_ce: null or misaligned pointer");
     std::lock_guard<std::recursive_mutex> lk(ctx->mu);
@@ -921,7 +921,7 @@ int32_t t0b_linear_ce(t0b_ctx* ctx, const t0b_linear_loss* loss, uint64_t target
 
 int32_t t0b_linear_topk_distill(t0b_ctx* ctx, const t0b_linear_loss* loss, uint64_t ids, uint64_t teacher, uint32_t topk, uint64_t ldk,
                                 float temperature, int32_t async) try {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (!loss || !ids || !teacher || ids % 4 || teacher % 4) return set_error(ctx, T0B_ERR_INVALID, "linear_topk_distill: null or misaligned pointer");
     if (topk == 0 || topk > T0B_MAX_TOPK || ldk < topk)

@@ -691,7 +691,7 @@ constexpr size_t kRowCacheMax = 64 * 1024;
 extern "C" {
 
 int32_t t0b_cast_f32_to_bf16(t0b_ctx* ctx, uint64_t src, uint64_t dst, size_t n, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (n == 0) return T0B_OK;
     if (!src || !dst) return set_error(ctx, T0B_ERR_INVALID, "cast: null pointer");
@@ -702,7 +702,7 @@ int32_t t0b_cast_f32_to_bf16(t0b_ctx* ctx, uint64_t src, uint64_t dst, size_t n,
 
 int32_t t0b_cast_f32_to_bf16_transpose(t0b_ctx* ctx, uint64_t src, uint64_t dst, uint32_t rows, uint32_t cols,
                                        int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (rows == 0 || cols == 0) return T0B_OK;
     if (!src || !dst) return set_error(ctx, T0B_ERR_INVALID, "cast_transpose: null pointer");
@@ -715,7 +715,7 @@ int32_t t0b_cast_f32_to_bf16_transpose(t0b_ctx* ctx, uint64_t src, uint64_t dst,
 
 int32_t t0b_rmsnorm_fwd(t0b_ctx* ctx, uint64_t x, uint64_t weight, uint64_t y, uint64_t inv_rms, uint32_t rows,
                         uint32_t cols, float eps, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (rows == 0) return T0B_OK;
     if (cols == 0 || !x || !weight || !y) return set_error(ctx, T0B_ERR_INVALID, "rmsnorm_fwd: null pointer or zero cols");
@@ -744,7 +744,7 @@ size_t t0b_rmsnorm_bwd_scratch_bytes(uint32_t rows, uint32_t cols) {
 
 int32_t t0b_rmsnorm_bwd(t0b_ctx* ctx, uint64_t dy, uint64_t x, uint64_t weight, uint64_t dx, uint64_t dgamma,
                         uint64_t scratch, size_t scratch_bytes, uint32_t rows, uint32_t cols, float eps, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (rows == 0) {
         if (dgamma && cols) return t0b_memset0(ctx, dgamma, static_cast<size_t>(cols) * 4);
@@ -826,7 +826,7 @@ static std::mutex g_rmsnorm_bwd_scratch_mu;
 
 int32_t t0b_rmsnorm_bwd_noalloc(t0b_ctx* ctx, uint64_t dy, uint64_t x, uint64_t weight, uint64_t dx, uint64_t dgamma,
                                 uint32_t rows, uint32_t cols, float eps, int32_t async) {
-    int32_t rc = precheck(ctx);   // makes ctx->device the current device
+    int32_t rc = precheck(ctx, async);   // makes ctx->device the current device
     if (rc != T0B_OK) return rc;
     if (cols == 0 || !dy || !x || !weight || !dgamma)
         return set_error(ctx, T0B_ERR_INVALID, "rmsnorm_bwd_noalloc: null pointer or zero cols");
@@ -880,7 +880,7 @@ int32_t t0b_rmsnorm_bwd_noalloc(t0b_ctx* ctx, uint64_t dy, uint64_t x, uint64_t 
 }
 
 int32_t t0b_softmax_fwd(t0b_ctx* ctx, uint64_t x, uint64_t y, uint32_t rows, uint32_t cols, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (rows == 0) return T0B_OK;
     if (cols == 0 || !x || !y) return set_error(ctx, T0B_ERR_INVALID, "softmax_fwd: null pointer or zero cols");
@@ -902,7 +902,7 @@ int32_t t0b_softmax_fwd(t0b_ctx* ctx, uint64_t x, uint64_t y, uint32_t rows, uin
 }
 
 int32_t t0b_softmax_bwd(t0b_ctx* ctx, uint64_t dy, uint64_t y, uint64_t dx, uint32_t rows, uint32_t cols, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (rows == 0) return T0B_OK;
     if (cols == 0 || !dy || !y || !dx) return set_error(ctx, T0B_ERR_INVALID, "softmax_bwd: null pointer or zero cols");
@@ -914,7 +914,7 @@ int32_t t0b_softmax_bwd(t0b_ctx* ctx, uint64_t dy, uint64_t y, uint64_t dx, uint
 
 static int32_t softmax_ce_impl(t0b_ctx* ctx, uint64_t logits, uint64_t targets, uint64_t losses, uint64_t dlogits, uint32_t rows,
                                uint32_t cols, uint64_t ld, float scale, bool grad16, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (rows == 0) return T0B_OK;
     if (cols == 0 || !logits || !targets || (!losses && !dlogits) || ld < cols)
@@ -956,7 +956,7 @@ int32_t t0b_softmax_ce_bf16(t0b_ctx* ctx, uint64_t logits, uint64_t targets, uin
 }
 
 int32_t t0b_silu_gate_fwd(t0b_ctx* ctx, uint64_t gate, uint64_t up, uint64_t out, size_t n, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (n == 0) return T0B_OK;
     if (!gate || !out) return set_error(ctx, T0B_ERR_INVALID, "silu_gate_fwd: null pointer");
@@ -967,7 +967,7 @@ int32_t t0b_silu_gate_fwd(t0b_ctx* ctx, uint64_t gate, uint64_t up, uint64_t out
 
 int32_t t0b_silu_gate_bwd(t0b_ctx* ctx, uint64_t grad, uint64_t gate, uint64_t up, uint64_t dgate, uint64_t dup, size_t n,
                           int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (n == 0) return T0B_OK;
     if (!grad || !gate || !dgate) return set_error(ctx, T0B_ERR_INVALID, "silu_gate_bwd: null pointer");
@@ -978,7 +978,7 @@ int32_t t0b_silu_gate_bwd(t0b_ctx* ctx, uint64_t grad, uint64_t gate, uint64_t u
 }
 
 int32_t t0b_residual_add(t0b_ctx* ctx, uint64_t y, uint64_t x, size_t n, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (n == 0) return T0B_OK;
     if (!x || !y) return set_error(ctx, T0B_ERR_INVALID, "residual_add: null pointer");
@@ -989,7 +989,7 @@ int32_t t0b_residual_add(t0b_ctx* ctx, uint64_t y, uint64_t x, size_t n, int32_t
 int32_t t0b_adamw_step(t0b_ctx* ctx, uint64_t params, uint64_t grads, uint64_t m, uint64_t v, uint64_t params_bf16, size_t n,
                        float lr, float beta1, float beta2, float eps, float weight_decay, uint32_t t, float grad_scale,
                        int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (n == 0) return T0B_OK;
     if (!params || !grads || !m || !v || t == 0) return set_error(ctx, T0B_ERR_INVALID, "adamw_step: null pointer or t == 0");
@@ -1011,7 +1011,7 @@ static bool rmsnorm_reg_path(uint64_t ptrs, uint32_t cols) {
 
 int32_t t0b_rmsnorm_silu_fwd(t0b_ctx* ctx, uint64_t x, uint64_t weight, uint64_t out_bf16, uint64_t inv_rms, uint32_t rows,
                              uint32_t cols, float eps, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (rows == 0) return T0B_OK;
     if (cols == 0 || !x || !weight || !out_bf16) return set_error(ctx, T0B_ERR_INVALID, "rmsnorm_silu_fwd: null pointer or zero cols");
@@ -1043,7 +1043,7 @@ int32_t t0b_rmsnorm_silu_fwd(t0b_ctx* ctx, uint64_t x, uint64_t weight, uint64_t
 
 int32_t t0b_rmsnorm_silu_bwd(t0b_ctx* ctx, uint64_t dh, uint64_t x, uint64_t weight, uint64_t dx_bf16, uint64_t dgamma,
                              uint64_t scratch, size_t scratch_bytes, uint32_t rows, uint32_t cols, float eps, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (rows == 0) {
         if (dgamma && cols) return t0b_memset0(ctx, dgamma, static_cast<size_t>(cols) * 4);

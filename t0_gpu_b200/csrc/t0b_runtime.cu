@@ -32,7 +32,21 @@ int32_t check_cuda(t0b_ctx* ctx, cudaError_t e, const char* what) {
     return set_error(ctx, T0B_ERR_CUDA, "%s: %s (%s)", what, cudaGetErrorString(e), cudaGetErrorName(e));
 }
 
-int32_t precheck(t0b_ctx* ctx) {
+// A synchronous call on the context's own stream starts behind what the device's default stream holds: its operands may be
+// under way there (a host framework that launches on the default stream), and the own stream does not wait by itself.
+// Asynchronous calls, calls on the caller's stream and captures are ordered by the caller.  Where the default stream cannot be
+// asked (a stream that waits for it is being captured) the order stays the caller's, too.
+static void after_default_stream(t0b_ctx* ctx) {
+    std::lock_guard<std::recursive_mutex> lk(ctx->mu);
+    if (ctx->capturing || ctx->stream != ctx->own_stream) return;
+    cudaError_t e = cudaSuccess;
+    if (!ctx->default_event) e = cudaEventCreateWithFlags(&ctx->default_event, cudaEventDisableTiming);
+    if (e == cudaSuccess) e = cudaEventRecord(ctx->default_event, cudaStreamLegacy);
+    if (e == cudaSuccess) e = cudaStreamWaitEvent(ctx->stream, ctx->default_event, 0);
+    if (e != cudaSuccess) cudaGetLastError();
+}
+
+int32_t precheck(t0b_ctx* ctx, int32_t async) {
     if (!ctx) return T0B_ERR_INVALID;
     if (ctx->poisoned) {
         // Keep the message of the error that poisoned the context.
@@ -40,6 +54,7 @@ int32_t precheck(t0b_ctx* ctx) {
     }
     cudaError_t e = cudaSetDevice(ctx->device);
     if (e != cudaSuccess) return check_cuda(ctx, e, "cudaSetDevice");
+    if (!async) after_default_stream(ctx);
     return T0B_OK;
 }
 
@@ -154,6 +169,7 @@ void t0b_ctx_destroy(t0b_ctx* ctx) {
     if (ctx->d2h_stream) cudaStreamDestroy(ctx->d2h_stream);
     if (ctx->p2p_stream) cudaStreamDestroy(ctx->p2p_stream);
     if (ctx->status_host) cudaFreeHost(ctx->status_host);
+    if (ctx->default_event) cudaEventDestroy(ctx->default_event);
     if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);
     delete ctx;
 }
@@ -563,7 +579,7 @@ int32_t t0b_graph_end(t0b_ctx* ctx, uint64_t* handle) {
 }
 
 int32_t t0b_graph_launch(t0b_ctx* ctx, uint64_t handle, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     auto it = ctx->graphs.find(handle);
     if (it == ctx->graphs.end()) return set_error(ctx, T0B_ERR_INVALID, "t0b_graph_launch: unknown graph %llu",

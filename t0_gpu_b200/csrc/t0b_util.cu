@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(256) copy16_2d_kernel(uint4* __restrict__ dst,
 extern "C" {
 
 int32_t t0b_hash_blocks(t0b_ctx* ctx, uint64_t src, size_t bytes, size_t block_bytes, uint64_t out, int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (bytes == 0) return T0B_OK;
     if (!src || !out || block_bytes == 0 || (bytes % 8) != 0 || (block_bytes % 8) != 0 || (src % 8) != 0 || (out % 8) != 0)
@@ -72,7 +72,7 @@ int32_t t0b_hash_blocks(t0b_ctx* ctx, uint64_t src, size_t bytes, size_t block_b
 
 int32_t t0b_copy_d2d(t0b_ctx* ctx, uint64_t dst, size_t dst_pitch, uint64_t src, size_t src_pitch, size_t width_bytes, size_t rows,
                      int32_t async) {
-    int32_t rc = precheck(ctx);
+    int32_t rc = precheck(ctx, async);
     if (rc != T0B_OK) return rc;
     if (width_bytes == 0 || rows == 0) return T0B_OK;
     if (!dst || !src || ((dst | src | dst_pitch | src_pitch | width_bytes) & 15) != 0 || dst_pitch < width_bytes || src_pitch < width_bytes)
