@@ -109,11 +109,13 @@ int32_t make_chain(t0b_ctx* ctx, const int32_t* ops, int n_ops, uint64_t bias, f
     return T0B_OK;
 }
 
+uint64_t slab_pitch(uint64_t n) { return (n + 3) & ~3ull; }
+
 int32_t launch_reduce(t0b_ctx* ctx, const float* partial, uint32_t sk, uint32_t m, uint32_t n, uint64_t slab_stride,
-                      uint64_t ld_partial, void* c, uint64_t ldc, int out_bf16, const EpiChain& epi) {
+                      uint64_t ld_partial, bool padded, void* c, uint64_t ldc, int out_bf16, const EpiChain& epi) {
     ReduceParams rp{partial, static_cast<long long>(slab_stride), static_cast<long long>(ld_partial), c,
                     static_cast<long long>(ldc), epi, static_cast<int>(m), static_cast<int>(n),
-                    static_cast<int>(sk), out_bf16};
+                    static_cast<int>(sk), out_bf16, padded ? 1 : 0};
     const long long total = static_cast<long long>(m) * ((n + 3) / 4);
     const int blocks = static_cast<int>(std::min<long long>((total + 255) / 256, static_cast<long long>(ctx->num_sms) * 8));
     cudaLaunchConfig_t cfg{};
@@ -275,6 +277,13 @@ int32_t run_gemm(t0b_ctx* ctx, const GemmCall& g) {
     float* partial = nullptr;
     uint64_t slab_stride = static_cast<uint64_t>(g.m) * g.n, ld_partial = g.n;
     uint32_t sk = plan.split_k;
+    // Slabs of its own a call lays out at a pitch of whole 16 bytes, which the sum reads and the epilogue writes in float4; a caller's
+    // workspace may have been sized for the plain pitch.
+    const uint64_t pitch4 = slab_pitch(g.n);
+    if (!g.slabs_only && (!g.workspace || g.workspace_bytes >= static_cast<uint64_t>(sk) * g.m * pitch4 * 4)) {
+        ld_partial = pitch4;
+        slab_stride = static_cast<uint64_t>(g.m) * pitch4;
+    }
     if (g.slabs_only) {
         partial = reinterpret_cast<float*>(g.c_dst[0]);
         if (sk < g.force_split) {
@@ -429,7 +438,7 @@ int32_t run_gemm(t0b_ctx* ctx, const GemmCall& g) {
 
     if (!g.slabs_only && sk > 1 && !cluster_sk) {
         for (int d = 0; d < g.n_dst; ++d) {
-            int32_t rc = launch_reduce(ctx, partial, sk, g.m, g.n, slab_stride, ld_partial, reinterpret_cast<void*>(g.c_dst[d]),
+            int32_t rc = launch_reduce(ctx, partial, sk, g.m, g.n, slab_stride, ld_partial, ld_partial == pitch4, reinterpret_cast<void*>(g.c_dst[d]),
                                        g.ldc, g.out_bf16, g.epi);
             if (rc != T0B_OK) return rc;
             ++ctx->launches;
@@ -528,7 +537,7 @@ size_t inner_gemm_slab_bytes(t0b_ctx* ctx, const InnerGemm& d) {
     const PlanInput pin{g.m, g.n, g.k, g.trans_a, g.trans_b, g.lda, g.ldb, g.a, g.b, ctx->num_sms};
     resolve_plan(&cfg, pin, &plan);
     if (plan.split_k <= 1 || splitk_in_cluster(ctx, g, plan)) return 0;
-    return static_cast<size_t>(plan.split_k) * g.m * g.n * 4;
+    return static_cast<size_t>(plan.split_k) * g.m * slab_pitch(g.n) * 4;
 }
 
 int32_t inner_gemm(t0b_ctx* ctx, const InnerGemm& d) {
@@ -884,7 +893,7 @@ int32_t t0b_splitk_reduce(t0b_ctx* ctx, uint64_t partial, uint32_t split_k, uint
     EpiChain chain;
     rc = make_chain(ctx, &epilogue, 1, bias, alpha, 0.0f, 0.0f, &chain);
     if (rc != T0B_OK) return rc;
-    rc = launch_reduce(ctx, reinterpret_cast<const float*>(partial), split_k, m, n, slab_stride_elems, ld_partial,
+    rc = launch_reduce(ctx, reinterpret_cast<const float*>(partial), split_k, m, n, slab_stride_elems, ld_partial, false,
                        reinterpret_cast<void*>(c), ldc, out_dtype == T0B_OUT_BF16, chain);
     if (rc != T0B_OK) return rc;
     return finish(ctx, async, "t0b_splitk_reduce", 1);

@@ -108,17 +108,20 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const IN* in, unsigned l
 // The same copy of a bf16 matrix whose rows start off 16-byte boundaries (a head with an odd vocabulary, [dim, vocab]): a warp
 // reads whole 16-byte chunks of the source, a lane shifts its chunk and its neighbour's into the 16 bytes it writes.  Chunks
 // that reach over the matrix' ends are read by element.  2048 x 50257: 206 MB each way, bound by HBM.
+// HIGH rows to a block: 8 for narrow matrices (37980 x 157: 9 us, 41 us with 1), else 1 (1664 x 32028: 43 us, and 50 us with
+// the row per thread).
+template <uint32_t HIGH>
 __global__ void __launch_bounds__(256) pack_shifted_kernel(const __nv_bfloat16* in, unsigned long long ld, __nv_bfloat16* out, uint32_t ld_out,
                                                            uint32_t rows, uint32_t cols) {
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
     const uint32_t lane = threadIdx.x & 31;
-    const uint32_t c = (blockIdx.x * 256 + threadIdx.x) * 8;   // a warp's columns are neighbours
+    const uint32_t c = (blockIdx.x * (256 / HIGH) + threadIdx.x) * 8;   // a warp's columns are neighbours
     const uint64_t begin = reinterpret_cast<uint64_t>(in), end = begin + ((rows - 1ull) * ld + cols) * 2;
     auto load = [&](uint64_t addr) {
         return addr >= begin && addr + 16 <= end ? __ldcs(reinterpret_cast<const uint4*>(addr)) : make_uint4(0, 0, 0, 0);
     };
-    for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    for (uint32_t r = HIGH == 1 ? blockIdx.y : blockIdx.y * HIGH + threadIdx.y; r < rows; r += gridDim.y * HIGH) {
         const uint64_t at = begin + (r * ld + c) * 2, chunk = at & ~15ull;
         const uint32_t shift = static_cast<uint32_t>(at & 15);
         const uint4 a = load(chunk);
@@ -795,8 +798,9 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
         launched += 2;
     }
     if (p.copy_w) {
-        const uint32_t across = static_cast<uint32_t>((p.ldw / 8 + 255) / 256);
-        launch(ctx, pack_shifted_kernel, dim3(across, static_cast<uint32_t>(std::min<uint64_t>(p.w_rows, 65535))), 256, 0,
+        const uint32_t groups = static_cast<uint32_t>(p.ldw / 8), high = groups <= 32 ? 8 : (groups <= 128 ? 2 : 1), wide = 256 / high;
+        auto copy = high == 8 ? pack_shifted_kernel<8> : (high == 2 ? pack_shifted_kernel<2> : pack_shifted_kernel<1>);
+        launch(ctx, copy, dim3((groups + wide - 1) / wide, static_cast<uint32_t>(std::min<uint64_t>((p.w_rows + high - 1) / high, 65535))), dim3(wide, high), 0,
                reinterpret_cast<const __nv_bfloat16*>(d.w), d.ldw, reinterpret_cast<__nv_bfloat16*>(base + p.w), static_cast<uint32_t>(p.ldw),
                static_cast<uint32_t>(p.w_rows), static_cast<uint32_t>(p.w_cols));
         ++launched;

@@ -233,6 +233,13 @@ def test_linear_one_gradient(th, art, rows, x_needs, w_needs):
     check_linear(th, art, rows, 64, 200, False, topk=4, x_needs=x_needs, w_needs=w_needs)
 
 
+@pytest.mark.parametrize("trans_w,dim,vocab", [(True, 5, 700), (True, 157, 3001), (True, 499, 700), (True, 1030, 333), (False, 64, 157), (False, 99, 2101)])
+def test_linear_heads_with_rows_off_16_bytes(th, art, trans_w, dim, vocab):
+    """Copies in rows of 32, 64, 128 and 256 threads, the last ones partly idle."""
+    check_linear(th, art, 6, dim, vocab, trans_w)
+    check_linear(th, art, 182, dim, vocab, trans_w, topk=3)
+
+
 @pytest.mark.parametrize("trans_w", [False, True])
 def test_linear_large_logits(th, art, trans_w):
     check_linear(th, art, 100, 64, 700, trans_w, big=40.0)
