@@ -496,7 +496,7 @@ t0b_gemm_config head_grad_config(t0b_ctx* ctx, const GemmCall& g, bool split) {
             if (sk > 1 && (kb / sk < 4 || tiles * (sk / 2) >= clusters)) break;   // split only while SMs are idle
             double cost = static_cast<double>((tiles * sk + clusters - 1) / clusters) * std::max((kb + sk - 1) / sk * c.kb_cycles + c.epi, c.floor);
             // The sum over the ranges: inside a cluster over distributed shared memory, or through slabs and a second kernel.
-            if (sk > 1) cost += (c.cg == 1 && (sk <= 4 || (sk == 8 && tiles <= 15))) ? 7000.0 : 14000.0 + 500.0 * sk + static_cast<double>(g.m) * g.n * 4.0 * (sk + 1) / 3300.0;
+            if (sk > 1) cost += (c.cg == 1 && (sk <= 4 || (sk == 8 && tiles <= 15))) ? 7000.0 : 8000.0 + 100.0 * sk + static_cast<double>(g.m) * g.n * 4.0 * (sk + 1) / 3300.0;
             if (cost < best_cost) {
                 best_cost = cost;
                 best = &c;
