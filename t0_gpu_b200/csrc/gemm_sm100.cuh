@@ -910,11 +910,11 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                         stage_chunk_bf16_sw64(half_tile, lane, v);
                         ptx::fence_proxy_async_smem();
                         __syncwarp();
-                        if (lane == 0) {
-                            ptx::tma_store_2d(&tmap_c, half_tile, col0, row0);
-                            ptx::bulk_commit_group();
-                        }
+                        if (lane == 0) ptx::tma_store_2d(&tmap_c, half_tile, col0, row0);
                     }
+                    // One group per chunk, empty where the chunk lies behind column N: the wait above counts groups, and a tile
+                    // with an odd number of chunks would otherwise leave its last store in the half that the next tile begins with.
+                    if (lane == 0) ptx::bulk_commit_group();
                 } else if (staged && out16) {
                     const int half = c & 1;
                     if (half == 0) __syncwarp();   // the previous pair's reads of the staging tile are done
