@@ -459,9 +459,10 @@ T0B_API int32_t t0b_embedding_bwd(t0b_ctx* ctx, uint64_t grad_table, uint64_t id
  *   dz        = (p sum(q) - q) * scale * row_weights[r] / T    the gradient of scale * sum_r row_weights[r] losses[r]
  * A row is left out when it has no target (target T0B_NO_WORD; no teacher word other than T0B_NO_WORD whose logit is above
  * -inf) or no logit above -inf: its loss, its log-sum-exp and its gradients are 0, whatever its logits, hidden state, weight
- * and teacher logits hold.  An index >= vocab that is not T0B_NO_WORD counts as T0B_NO_WORD and sets the device status word
- * to 110.  A NaN or +inf logit makes its row's loss and gradient NaN; a masked word (-inf logit) has p = 0 and, where it
- * is a target, an infinite loss.  Outputs must not overlap inputs or each other, except as said below.
+ * and teacher logits hold (dx is a product with the head, which has to be finite for that).  An index >= vocab that is not
+ * T0B_NO_WORD counts as T0B_NO_WORD and sets the device status word to 110.  A NaN or +inf logit makes its row's loss and
+ * gradient NaN; a masked word (-inf logit) has p = 0 and, where it is a target, an infinite loss.  Outputs must not overlap
+ * inputs or each other, except as said below.
  * ---------------------------------------------------------------------------------------------- */
 #define T0B_NO_WORD 0xffffffffu
 #define T0B_MAX_TOPK 1024

@@ -439,11 +439,13 @@ __global__ void __launch_bounds__(1024) join_parts_kernel(const float2* part, un
 // 128000: 358 us, 5.9 TB/s).  Two small steps ride along where their own launch would cost more than they do:
 //   JOIN   every block joins its row's parts itself, and the row's first block finishes the loss (join_parts_kernel is not
 //          launched): for few rows or few parts
-//   x_out  the row's first block copies the hidden state, or zeros in a row without a target, for the head's gradient
+//   cp.x   the row's first block copies the hidden state, or zeros in a row that is left out, for the head's gradient
+// Where that copy was made before the logits were known, the row's first block clears it in a row whose logits are all -inf:
+// an infinity in the hidden state would meet dz = 0 in the head's gradient.
 constexpr int kGradVecs = 4;
 constexpr uint32_t kGradCols = 256 * 8 * kGradVecs;
 struct JoinParams { uint32_t parts; float inv_t; float *losses, *lse; int* status; };
-struct CopyParams { const __nv_bfloat16* x; unsigned long long ldx; __nv_bfloat16* out; uint32_t ld_out, dim; };
+struct CopyParams { const __nv_bfloat16* x; unsigned long long ldx; __nv_bfloat16* out; uint32_t ld_out, dim; };   // out null: no gradient of the head
 template <bool JOIN>
 __global__ void __launch_bounds__(256) dz_kernel(__half* u, unsigned long long ldu, uint32_t rows, uint32_t y0, const float2* part,
                                                  unsigned long long part_ld, uint32_t part_shift, const float2* stats,
@@ -469,12 +471,11 @@ __global__ void __launch_bounds__(256) dz_kernel(__half* u, unsigned long long l
             top[v] = part[(col >> part_shift) * part_ld + i].x;
         }
     }
-    if (cp.out && blockIdx.x == 0 && !behind) {
-        const bool vec = rows_vec(cp.x, cp.ldx);
-        for (uint32_t col = threadIdx.x * 8; col < cp.ld_out; col += 256 * 8)
-            *reinterpret_cast<uint4*>(cp.out + static_cast<unsigned long long>(r) * cp.ld_out + col) =
-                wanted ? operand_group(cp.x + r * cp.ldx, col, cp.dim, vec) : make_uint4(0, 0, 0, 0);
-    }
+    // The first 2048 columns of the hidden state are asked for with the exponentials; whether they are copied is known later.
+    const bool first = cp.out && blockIdx.x == 0 && !behind;
+    const bool copy_x = first && cp.x != nullptr, vec_x = copy_x && rows_vec(cp.x, cp.ldx);
+    uint4 x0 = make_uint4(0, 0, 0, 0);
+    if (copy_x && wanted && threadIdx.x * 8 < cp.ld_out) x0 = operand_group(cp.x + r * cp.ldx, threadIdx.x * 8, cp.dim, vec_x);
     float2 st = make_float2(0.0f, 1.0f);
     if constexpr (JOIN) {
         __shared__ float2 sh[8];
@@ -504,6 +505,14 @@ __global__ void __launch_bounds__(256) dz_kernel(__half* u, unsigned long long l
     const bool live = wanted && !(st.x == -INFINITY && st.y == 0.0f);
     const float a = live ? scale * (weights ? weights[r] : 1.0f) : 0.0f;
     const float inv = 1.0f / st.y;
+    if (copy_x || (first && wanted && !live)) {
+        __nv_bfloat16* xr = cp.out + static_cast<unsigned long long>(tg.row0 + i) * cp.ld_out;
+        for (uint32_t col = threadIdx.x * 8; col < cp.ld_out; col += 256 * 8) {
+            uint4 o = make_uint4(0, 0, 0, 0);
+            if (copy_x && live) o = col < 256 * 8 ? x0 : operand_group(cp.x + r * cp.ldx, col, cp.dim, vec_x);
+            *reinterpret_cast<uint4*>(xr + col) = o;
+        }
+    }
 #pragma unroll
     for (int v = 0; v < kGradVecs; ++v) {
         const uint32_t col = c0 + (v * 256 + threadIdx.x) * 8;
@@ -565,7 +574,7 @@ struct Plan {
     uint64_t part_ld;
     uint64_t ldu;
     bool copy_x, copy_w;               // before the head's product
-    bool late_x;                       // the copy of x for the head's gradient is made by dz_kernel; the head reads x itself
+    bool late_x;                       // the copy of x for the head's gradient (which always reads one) is made by dz_kernel; the head reads x itself
     bool join_in_dz;
     bool gather;                       // the products run over the rows with a target alone
     uint64_t ld_dxg;
@@ -848,7 +857,7 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
         }
         if (!p.grads) continue;
         const JoinParams jp{p.parts, inv_t, losses, lse, ctx->status_dev};
-        const CopyParams cp{xb, d.ldx, p.late_x ? xg : nullptr, static_cast<uint32_t>(p.ldx), d.dim};
+        const CopyParams cp{p.late_x ? xb : nullptr, d.ldx, p.dw ? xg : nullptr, static_cast<uint32_t>(p.ldx), d.dim};
         for (uint32_t y0 = 0; y0 < n; y0 += 65535u) {   // gridDim.y is limited to 65535
             launch(ctx, p.join_in_dz ? dz_kernel<true> : dz_kernel<false>, dim3(static_cast<uint32_t>((p.ldu + kGradCols - 1) / kGradCols), std::min(65535u, n - y0)),
                    256, 0, reinterpret_cast<__half*>(base + p.u), p.ldu, n, y0, reinterpret_cast<const float2*>(base + p.part), p.part_ld, part_shift, stats,

@@ -1,0 +1,77 @@
+"""Vocabulary losses where their contract ends: rows that the logits leave without a distribution.  Bounds as in
+test_vocab_losses_gpu.py."""
+import math
+
+import pytest
+
+from t0_gpu_b200 import OUT_BF16, OUT_F32, ops
+from test_vocab_losses_gpu import U32, UB, UH, art, losses_and_dz, make_teacher, target_rows, th  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("trans_w", [False, True])
+@pytest.mark.parametrize("rows,vocab,topk,x_dtype,piece_rows", [
+    (40, 300, 0, OUT_BF16, 0),         # x is copied for the head's gradient only, rows joined with their gradient
+    (256, 50000, 0, OUT_BF16, 0),      # the same, joined by a kernel of its own
+    (40, 300, 0, OUT_F32, 0),          # x is copied first
+    (40, 300, 3, OUT_F32, 0),          # ... together with the teacher's words
+    (40, 300, 3, OUT_BF16, 0),
+    (300, 300, 0, OUT_BF16, 0),        # rows with a target gathered
+    (300, 300, 3, OUT_F32, 0),
+    (300, 300, 0, OUT_BF16, 128),      # in pieces
+    (100, 300, 0, OUT_BF16, 33),
+])
+def test_a_row_without_finite_logits_reaches_no_gradient(th, art, rows, vocab, topk, x_dtype, piece_rows, trans_w):  # noqa: F811
+    """An infinity in the hidden state and a column of the head with one sign: every logit is -inf, and the row is left out of
+    the gradients (0 * inf would be NaN in the head's)."""
+    dim = 64
+    g = th.Generator(device="cuda")
+    g.manual_seed(rows + vocab + topk)
+    w = (th.randn((vocab, dim), device="cuda", generator=g) / 8).bfloat16()
+    w[:, 0] = -0.25 - w[:, 0].abs()
+    x = (th.randn((rows, dim), device="cuda", generator=g) * 2).bfloat16()
+    dead = th.zeros(rows, device="cuda", dtype=th.bool)
+    dead[::5] = True
+    dead[-1] = True
+    xd = x.double().masked_fill(dead[:, None], 0.0)
+    x[dead, 0] = math.inf
+    x = x if x_dtype == OUT_BF16 else x.float()
+    if topk:
+        ids, teacher = make_teacher(th, rows, topk, vocab, 5, False)
+        q, ent, live = target_rows(th, ids, teacher, 1.0, vocab)
+    else:
+        tgt = th.randint(0, vocab, (rows,), device="cuda", generator=g)
+        tgt[1::7] = -1
+        live = tgt >= 0
+        q = th.zeros((rows, vocab), dtype=th.float64, device="cuda")
+        q[th.arange(rows, device="cuda"), tgt.clamp_min(0)] = live.double()
+        ent = th.zeros(rows, dtype=th.float64, device="cuda")
+        tgt = tgt.to(th.int32)
+    live = live & ~dead
+    wd = w.double()
+    z = xd @ wd.t()
+    scale = th.full((rows,), 1.0 / rows, device="cuda", dtype=th.float64)
+    losses_ref, dz, p, lse_ref = losses_and_dz(th, z, q, ent, live, 1.0, scale)
+    head = w if trans_w else w.t().contiguous()
+    losses, lse = th.full((rows,), 7.0, device="cuda"), th.full((rows,), 7.0, device="cuda")
+    dx, dw = th.full((rows, dim), 7.0, device="cuda"), th.full(head.shape, 7.0, device="cuda")
+    kw = dict(trans_w=trans_w, x_dtype=x_dtype, w_dtype=OUT_BF16, losses=losses.data_ptr(), lse=lse.data_ptr(), dx=dx.data_ptr(), dw=dw.data_ptr(),
+              piece_rows=piece_rows)
+    if topk:
+        ops.linear_topk_distill(art, x.data_ptr(), head.data_ptr(), ids.data_ptr(), teacher.data_ptr(), rows, dim, vocab, topk, **kw)
+    else:
+        ops.linear_cross_entropy(art, x.data_ptr(), head.data_ptr(), tgt.data_ptr(), rows, dim, vocab, **kw)
+    art.synchronize()
+    xa, wa = xd.abs(), wd.abs()
+    ez = dim * U32 * (xa @ wa.t()).amax(1)
+    down = z.amax(1, keepdim=True) - z
+    tol = 2 * ez + ((down * (q > 0)).amax(1) + 16 + lse_ref.abs()) * 8 * U32
+    assert ((losses.double() - losses_ref).abs() <= tol).all()
+    assert (losses[~live] == 0).all() and (lse[~live] == 0).all() and (dx[~live] == 0).all()
+    a = (live / rows)[:, None]
+    edz = UB * dz.abs() + a * (p * (2 * ez[:, None] + down * 4 * U32 + 8 * U32 + UH + UB * UH) + 2.0 ** -24 * p.amax(1, keepdim=True))
+    full = dz.abs() + edz
+    for got, want, err in ((dx, dz @ wd, edz @ wa + vocab * U32 * (full @ wa)),
+                           (dw if trans_w else dw.t(), dz.t() @ xd, edz.t() @ xa + rows * U32 * (full.t() @ xa))):
+        assert ((got.double() - want).abs() <= err + U32 * (want.abs() + err) + 1e-30).all()
