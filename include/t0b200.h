@@ -14,6 +14,9 @@
  *   - a context is thread-safe; all launches of a context go to one CUDA stream.  On the context's own stream a
  *     synchronous launch (is_async = 0) starts behind the work that the device's default stream holds; asynchronous ones,
  *     and all on a stream of the caller's (t0b_ctx_set_stream), are ordered against other streams by the caller.
+ *     That order is an event recorded on the default stream, which waits for all blocking streams and which they wait for.
+ *     It is left out while a blocking stream is being captured, whose capture it would invalidate.  A program in which
+ *     another thread may begin such a capture at that very moment switches it off (T0B_DEFAULT_STREAM_ORDER=0).
  */
 #ifndef T0B200_H
 #define T0B200_H
@@ -158,6 +161,7 @@ T0B_API int32_t t0b_resolve_plan(const t0b_gemm_config* cfg, uint32_t m, uint32_
  *   T0_DUMP_CONFIG=1          one stderr line per new GEMM shape: config name, who chose it (caller, forced, tuned in
  *                             this process, shipped table, cost model) and the kernel variant it resolves to;
  *   T0B_PDL=0                 launches without programmatic stream serialization;
+ *   T0B_DEFAULT_STREAM_ORDER=0  synchronous calls do not wait for the default stream's work (see the top of this file);
  *   T0B_CLUSTER_SPLITK=0      split-K always through slabs and the reduce kernel;
  *   T0B_RASTER_GROUP=<n>      rasterisation group width for every GEMM (a measurement knob);
  *   T0B_WAIT_HINT_NS=<ns>     suspend-time hint of the epilogue warps' accumulator wait (default 20000; 0 = busy polling,

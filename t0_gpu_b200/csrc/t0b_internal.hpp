@@ -32,6 +32,7 @@ struct t0b_ctx {
     cudaStream_t own_stream = nullptr;
     cudaStream_t stream = nullptr;
     cudaEvent_t default_event = nullptr;   // the default stream's work that a synchronous call waits for
+    bool default_order = true;             // T0B_DEFAULT_STREAM_ORDER=0: synchronous calls leave the default stream alone
     std::recursive_mutex mu;
     std::string last_error;
     bool poisoned = false;

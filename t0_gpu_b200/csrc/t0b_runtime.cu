@@ -34,13 +34,16 @@ int32_t check_cuda(t0b_ctx* ctx, cudaError_t e, const char* what) {
 
 // A synchronous call on the context's own stream starts behind what the device's default stream holds: its operands may be
 // under way there (a host framework that launches on the default stream), and the own stream does not wait by itself.
-// Asynchronous calls, calls on the caller's stream and captures are ordered by the caller.  Where the default stream cannot be
-// asked (a stream that waits for it is being captured) the order stays the caller's, too.
+// Asynchronous calls, calls on the caller's stream and captures are ordered by the caller.  While a blocking stream of the
+// process is being captured, any use of the default stream would invalidate that capture; asking whether one is does not
+// (cudaStreamIsCapturing then answers cudaErrorStreamCaptureImplicit), and the order stays the caller's, too.
 static void after_default_stream(t0b_ctx* ctx) {
     std::lock_guard<std::recursive_mutex> lk(ctx->mu);
-    if (ctx->capturing || ctx->stream != ctx->own_stream) return;
-    cudaError_t e = cudaSuccess;
-    if (!ctx->default_event) e = cudaEventCreateWithFlags(&ctx->default_event, cudaEventDisableTiming);
+    if (!ctx->default_order || ctx->capturing || ctx->stream != ctx->own_stream) return;
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    cudaError_t e = cudaStreamIsCapturing(cudaStreamLegacy, &st);
+    if (e == cudaSuccess && st != cudaStreamCaptureStatusNone) return;
+    if (e == cudaSuccess && !ctx->default_event) e = cudaEventCreateWithFlags(&ctx->default_event, cudaEventDisableTiming);
     if (e == cudaSuccess) e = cudaEventRecord(ctx->default_event, cudaStreamLegacy);
     if (e == cudaSuccess) e = cudaStreamWaitEvent(ctx->stream, ctx->default_event, 0);
     if (e != cudaSuccess) cudaGetLastError();
@@ -132,6 +135,7 @@ int32_t t0b_ctx_create(int32_t device, t0b_ctx** out) {
     if (rc == T0B_OK) {
         ctx->num_sms = prop.multiProcessorCount;
         if (const char* e = std::getenv("T0B_PDL")) ctx->pdl = std::atoi(e) != 0;
+        if (const char* e = std::getenv("T0B_DEFAULT_STREAM_ORDER")) ctx->default_order = std::atoi(e) != 0;
         if (const char* e = std::getenv("T0B_CLUSTER_SPLITK")) ctx->cluster_splitk = std::atoi(e) != 0;
         if (const char* e = std::getenv("T0B_WAIT_HINT_NS")) ctx->wait_hint_ns = static_cast<unsigned>(std::max(0, std::atoi(e)));
         if (const char* e = std::getenv("T0_FORCE_CONFIG")) ctx->force_config = e;
