@@ -702,8 +702,8 @@ int32_t check_desc(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d) {
     const uint64_t xe = d.x_dtype == T0B_OUT_BF16 ? 2 : 4, dxe = d.dx_dtype == T0B_OUT_BF16 ? 2 : 4, dwe = d.dw_dtype == T0B_OUT_BF16 ? 2 : 4;
     if (d.x % xe || d.w % 2 || (d.dx && d.dx % dxe) || (d.dw && d.dw % dwe) || d.losses % 4 || d.lse % 4 || d.row_weights % 4)
         return bad("a pointer is not aligned to its element");
-    if (d.rows == 0) return T0B_OK;
     const uint64_t wr = d.trans_w ? d.vocab : d.dim, wc = d.trans_w ? d.dim : d.vocab;
+    if (d.rows == 0) return check_fits(ctx, what, {{"dw", d.dw, ((wr - 1) * d.lddw + wc) * dwe}});   // becomes zeros
     return check_fits(ctx, what, {{"x", d.x, ((d.rows - 1ull) * d.ldx + d.dim) * xe}, {"w", d.w, ((wr - 1) * d.ldw + wc) * 2},
                                   {"dx", d.dx, ((d.rows - 1ull) * d.lddx + d.dim) * dxe}, {"dw", d.dw, ((wr - 1) * d.lddw + wc) * dwe},
                                   {"losses", d.losses, d.rows * 4ull}, {"lse", d.lse, d.rows * 4ull}, {"row_weights", d.row_weights, d.rows * 4ull}});
@@ -751,7 +751,15 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
     if (d.rows == 0) {
         if (!d.dw) return T0B_OK;
         const uint64_t wr = d.trans_w ? d.vocab : d.dim, wc = d.trans_w ? d.dim : d.vocab;
-        const int32_t rc = check_cuda(ctx, cudaMemset2DAsync(reinterpret_cast<void*>(d.dw), d.lddw * dwe, 0, wc * dwe, wr, ctx->stream), "cudaMemset2DAsync(dw)");
+        const bool dense = wr == 1 || d.lddw == wc;
+        const uint64_t pitch = d.lddw * dwe, run = dense ? wr * wc * dwe : wc * dwe;
+        int32_t rc = T0B_OK;
+        if (dense || pitch > 0x7fffffffull) {   // the 2-D form ends at pitches of 2 GiB
+            for (uint64_t r = 0; r < (dense ? 1 : wr) && rc == T0B_OK; ++r)
+                rc = check_cuda(ctx, cudaMemsetAsync(reinterpret_cast<void*>(d.dw + r * pitch), 0, run, ctx->stream), "cudaMemsetAsync(dw)");
+        } else {
+            rc = check_cuda(ctx, cudaMemset2DAsync(reinterpret_cast<void*>(d.dw), pitch, 0, run, wr, ctx->stream), "cudaMemset2DAsync(dw)");
+        }
         return rc != T0B_OK ? rc : finish(ctx, async, what, 0);
     }
     const bool teacher = te.logits != 0;

@@ -4,7 +4,7 @@ import math
 
 import pytest
 
-from t0_gpu_b200 import OUT_BF16, OUT_F32, ops
+from t0_gpu_b200 import OUT_BF16, OUT_F32, T0Error, ops
 from test_vocab_losses_gpu import U32, UB, UH, art, losses_and_dz, make_teacher, target_rows, th  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -75,3 +75,35 @@ def test_a_row_without_finite_logits_reaches_no_gradient(th, art, rows, vocab, t
     for got, want, err in ((dx, dz @ wd, edz @ wa + vocab * U32 * (full @ wa)),
                            (dw if trans_w else dw.t(), dz.t() @ xd, edz.t() @ xa + rows * U32 * (full.t() @ xa))):
         assert ((got.double() - want).abs() <= err + U32 * (want.abs() + err) + 1e-30).all()
+
+
+@pytest.mark.parametrize("trans_w", [False, True])
+def test_an_empty_call_checks_the_gradient_it_clears(th, art, trans_w):  # noqa: F811
+    """No rows: the head's gradient becomes zeros, in a buffer that holds it or not at all."""
+    dim, vocab = 64, 80
+    w = th.ones((dim * vocab,), device="cuda").bfloat16()
+    small, whole = art.alloc_zero(4096), art.alloc_zero(dim * vocab * 4)
+    kw = dict(trans_w=trans_w, x_dtype=OUT_BF16, w_dtype=OUT_BF16, losses=w.data_ptr(), x_needs=False)
+    with pytest.raises(T0Error, match="dw needs"):
+        ops.linear_cross_entropy(art, w.data_ptr(), w.data_ptr(), w.data_ptr(), 0, dim, vocab, dw=small, **kw)
+    for lddw in (None, (dim if trans_w else vocab) + 8):
+        rows = (vocab if trans_w else dim)
+        out = th.full((rows, lddw or (dim if trans_w else vocab)), 7.0, device="cuda")
+        ops.linear_cross_entropy(art, w.data_ptr(), w.data_ptr(), w.data_ptr(), 0, dim, vocab, dw=out.data_ptr(), lddw=lddw, **kw)
+        art.synchronize()
+        cols = dim if trans_w else vocab
+        assert (out[:, :cols] == 0).all() and (out[:, cols:] == 7).all()
+    ops.linear_cross_entropy(art, w.data_ptr(), w.data_ptr(), w.data_ptr(), 0, dim, vocab, dw=whole, **kw)
+    art.synchronize()
+    assert not art.is_poisoned()
+
+
+def test_an_empty_call_with_rows_two_gib_apart(th, art):  # noqa: F811
+    pitch = 2 ** 29 + 8
+    out = th.full((2 * pitch,), 7.0, device="cuda")
+    w = th.ones((64,), device="cuda").bfloat16()
+    ops.linear_cross_entropy(art, w.data_ptr(), w.data_ptr(), w.data_ptr(), 0, 2, 20, x_dtype=OUT_BF16, w_dtype=OUT_BF16, losses=w.data_ptr(),
+                             x_needs=False, dw=out.data_ptr(), lddw=pitch)
+    art.synchronize()
+    rows = out.view(2, pitch)
+    assert (rows[:, :20] == 0).all() and (rows[:, 20:] == 7).all()
