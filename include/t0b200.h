@@ -507,7 +507,7 @@ typedef struct t0b_linear_loss {
     float scale;
 } t0b_linear_loss;
 /* Scratch of a call with these sizes, pitches and outputs (pointers count only as 0 or not, and by their alignment);
- * topk = 0 for t0b_linear_ce.  The choice of tiles behind it follows t0b_tune: ask again after tuning. */
+ * topk = 0 for t0b_linear_ce; 0 for sizes that no call takes.  The choice of tiles behind it follows t0b_tune: ask again after tuning. */
 T0B_API size_t t0b_linear_loss_scratch_bytes(t0b_ctx* ctx, const t0b_linear_loss* loss, uint32_t topk);
 /* Softmax cross entropy, targets u32[rows]. */
 T0B_API int32_t t0b_linear_ce(t0b_ctx* ctx, const t0b_linear_loss* loss, uint64_t targets, int32_t async);

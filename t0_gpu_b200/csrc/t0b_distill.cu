@@ -806,8 +806,8 @@ int32_t t0b_topk_distill(t0b_ctx* ctx, uint64_t logits, int32_t logits_dtype, ui
         return set_error(ctx, T0B_ERR_INVALID, "topk_distill: a pointer is not aligned to its element");
     if (dlogits == logits && ie != oe) return set_error(ctx, T0B_ERR_INVALID, "topk_distill: a gradient in the place of the logits needs their type");
     std::lock_guard<std::recursive_mutex> lk(ctx->mu);
-    rc = check_fits(ctx, "topk_distill", {{"logits", logits, ((rows - 1ull) * ld + cols) * ie}, {"dlogits", dlogits, ((rows - 1ull) * ld + cols) * oe},
-                                          {"ids", ids, ((rows - 1ull) * ldk + topk) * 4}, {"teacher", teacher, ((rows - 1ull) * ldk + topk) * 4},
+    rc = check_fits(ctx, "topk_distill", {{"logits", logits, span_bytes(rows, ld, cols, ie)}, {"dlogits", dlogits, span_bytes(rows, ld, cols, oe)},
+                                          {"ids", ids, span_bytes(rows, ldk, topk, 4)}, {"teacher", teacher, span_bytes(rows, ldk, topk, 4)},
                                           {"losses", losses, rows * 4ull}, {"row_weights", row_weights, rows * 4ull}});
     if (rc != T0B_OK) return rc;
 

@@ -97,8 +97,16 @@ int32_t check_cuda(t0b_ctx* ctx, cudaError_t e, const char* what);
 // bounded waits.
 constexpr int kDevBadIndex = 110;
 // Buffers that start one of the runtime's own allocations must fit in it: an undersized one is reported instead of faulting
-// on the device.  (Pointers from elsewhere, or into the middle of a buffer, are not known; null ones are skipped.)
+// on the device.  (Pointers from elsewhere, or into the middle of a buffer, are not known; null ones are skipped.)  No buffer
+// spans more than kMaxSpan bytes: a pitch that says so is refused, whoever allocated.
 struct Extent { const char* name; uint64_t ptr; uint64_t bytes; };
+constexpr uint64_t kMaxSpan = 1ull << 47;
+// From the first to the last byte of `rows` (at least one) rows of `cols` elements at a pitch of `ld`; more than kMaxSpan where
+// the true number does not fit 64 bits.
+inline uint64_t span_bytes(uint64_t rows, uint64_t ld, uint64_t cols, uint64_t elem) {
+    const unsigned __int128 n = (static_cast<unsigned __int128>(rows - 1) * ld + cols) * elem;
+    return n > kMaxSpan ? kMaxSpan + 1 : static_cast<uint64_t>(n);
+}
 int32_t check_fits(t0b_ctx* ctx, const char* what, std::initializer_list<Extent> extents);
 int32_t precheck(t0b_ctx* ctx, int32_t async = 1);   // null / poisoned checks, sets the device; a synchronous call waits for the default stream
 // Launch-error check (+ sync and status-word check when !async). `count` kernels are added to the launch counter.

@@ -687,11 +687,14 @@ Plan make_plan(t0b_ctx* ctx, const t0b_linear_loss& d, uint32_t n_ids, bool teac
     return p;
 }
 
+// Sizes that int and the row and tile counters hold.
+bool sizes_ok(const t0b_linear_loss& d) { return d.rows <= 0x7fffff00u && d.dim <= 0x7fffff00u && d.vocab <= 0x7fffff00u; }
+
 int32_t check_desc(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d) {
     auto bad = [&](const char* msg) { return set_error(ctx, T0B_ERR_INVALID, "%s: %s", what, msg); };
     if (!d.x || !d.w) return bad("null x or w");
     if (d.dim == 0 || d.vocab == 0) return bad("an empty head");
-    if (d.rows > 0x7fffff00u || d.dim > 0x7fffff00u || d.vocab > 0x7fffff00u) return bad("a size is over 2^31");
+    if (!sizes_ok(d)) return bad("a size is over 2^31");
     if (!d.losses && !d.lse && !d.dx && !d.dw) return bad("no output is asked for");
     if (d.ldx < d.dim || d.ldw < (d.trans_w ? d.dim : d.vocab) || (d.dx && d.lddx < d.dim) || (d.dw && d.lddw < (d.trans_w ? d.dim : d.vocab)))
         return bad("a pitch is smaller than its row");
@@ -703,9 +706,9 @@ int32_t check_desc(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d) {
     if (d.x % xe || d.w % 2 || (d.dx && d.dx % dxe) || (d.dw && d.dw % dwe) || d.losses % 4 || d.lse % 4 || d.row_weights % 4)
         return bad("a pointer is not aligned to its element");
     const uint64_t wr = d.trans_w ? d.vocab : d.dim, wc = d.trans_w ? d.dim : d.vocab;
-    if (d.rows == 0) return check_fits(ctx, what, {{"dw", d.dw, ((wr - 1) * d.lddw + wc) * dwe}});   // becomes zeros
-    return check_fits(ctx, what, {{"x", d.x, ((d.rows - 1ull) * d.ldx + d.dim) * xe}, {"w", d.w, ((wr - 1) * d.ldw + wc) * 2},
-                                  {"dx", d.dx, ((d.rows - 1ull) * d.lddx + d.dim) * dxe}, {"dw", d.dw, ((wr - 1) * d.lddw + wc) * dwe},
+    if (d.rows == 0) return check_fits(ctx, what, {{"dw", d.dw, span_bytes(wr, d.lddw, wc, dwe)}});   // becomes zeros
+    return check_fits(ctx, what, {{"x", d.x, span_bytes(d.rows, d.ldx, d.dim, xe)}, {"w", d.w, span_bytes(wr, d.ldw, wc, 2)},
+                                  {"dx", d.dx, span_bytes(d.rows, d.lddx, d.dim, dxe)}, {"dw", d.dw, span_bytes(wr, d.lddw, wc, dwe)},
                                   {"losses", d.losses, d.rows * 4ull}, {"lse", d.lse, d.rows * 4ull}, {"row_weights", d.row_weights, d.rows * 4ull}});
 }
 
@@ -918,7 +921,8 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
 extern "C" {
 
 size_t t0b_linear_loss_scratch_bytes(t0b_ctx* ctx, const t0b_linear_loss* loss, uint32_t topk) try {
-    if (!ctx || !loss || loss->rows == 0 || loss->dim == 0 || loss->vocab == 0) return 0;
+    if (!ctx || !loss || loss->rows == 0 || loss->dim == 0 || loss->vocab == 0 || !sizes_ok(*loss) || topk > T0B_MAX_TOPK) return 0;
+    if (span_bytes(loss->vocab, loss->dim, loss->dim, 4) > kMaxSpan) return 0;   // a head that no call takes
     std::lock_guard<std::recursive_mutex> lk(ctx->mu);
     if (precheck(ctx) != T0B_OK) return 0;
     return make_plan(ctx, *loss, std::max(1u, topk), topk > 0).total;
@@ -953,7 +957,7 @@ int32_t t0b_linear_topk_distill(t0b_ctx* ctx, const t0b_linear_loss* loss, uint6
     std::lock_guard<std::recursive_mutex> lk(ctx->mu);
     rc = check_desc(ctx, "linear_topk_distill", *loss);
     if (rc == T0B_OK && loss->rows > 0)
-        rc = check_fits(ctx, "linear_topk_distill", {{"ids", ids, ((loss->rows - 1ull) * ldk + topk) * 4}, {"teacher", teacher, ((loss->rows - 1ull) * ldk + topk) * 4}});
+        rc = check_fits(ctx, "linear_topk_distill", {{"ids", ids, span_bytes(loss->rows, ldk, topk, 4)}, {"teacher", teacher, span_bytes(loss->rows, ldk, topk, 4)}});
     if (rc != T0B_OK) return rc;
     return run_linear_loss(ctx, "linear_topk_distill", *loss, Teacher{ids, teacher, ldk, topk}, temperature, async);
 } catch (...) {

@@ -64,6 +64,7 @@ int32_t precheck(t0b_ctx* ctx, int32_t async) {
 int32_t check_fits(t0b_ctx* ctx, const char* what, std::initializer_list<Extent> extents) {
     for (const Extent& e : extents) {
         if (!e.ptr) continue;
+        if (e.bytes > kMaxSpan) return set_error(ctx, T0B_ERR_INVALID, "%s: the pitch of %s spans more than any buffer does", what, e.name);
         auto it = ctx->live.find(reinterpret_cast<void*>(e.ptr));
         if (it != ctx->live.end() && e.bytes > it->second)
             return set_error(ctx, T0B_ERR_INVALID, "%s: %s needs %llu bytes, its buffer has %llu", what, e.name,

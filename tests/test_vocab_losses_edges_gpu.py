@@ -107,3 +107,33 @@ def test_an_empty_call_with_rows_two_gib_apart(th, art):  # noqa: F811
     art.synchronize()
     rows = out.view(2, pitch)
     assert (rows[:, :20] == 0).all() and (rows[:, 20:] == 7).all()
+
+
+@pytest.mark.parametrize("pitch", [2 ** 61, 2 ** 62 - 3, 2 ** 63, 2 ** 64 - 8, 2 ** 46])
+def test_pitches_that_leave_the_address_space_are_refused(th, art, pitch):  # noqa: F811
+    """(rows - 1) * pitch * element size may come out small in 64 bits; no row would be where that says."""
+    rows, dim, vocab, topk = 5, 64, 80, 2
+    x, w = art.alloc_zero(rows * vocab * 4), art.alloc_zero(dim * vocab * 4)
+    z, out = art.alloc_zero(rows * vocab * 4), art.alloc_zero(dim * vocab * 4)
+    ids = art.alloc_zero(rows * vocab * 4)
+
+    def refused(f, *a, **kw):
+        with pytest.raises(T0Error, match="pitch of"):
+            f(art, *a, **kw)
+        assert not art.is_poisoned()
+
+    refused(ops.topk_distill, z, ids, z, rows, vocab, topk, ld=pitch, losses=out, dlogits=x)
+    refused(ops.topk_distill, z, ids, z, rows, vocab, topk, ldk=pitch, losses=out, dlogits=x)
+    kw = dict(x_dtype=OUT_BF16, w_dtype=OUT_BF16, losses=out, dx=x, dw=w)
+    for name in ("ldx", "ldw", "lddx", "lddw"):
+        refused(ops.linear_cross_entropy, x, w, ids, rows, dim, vocab, **{name: pitch}, **kw)
+    refused(ops.linear_topk_distill, x, w, ids, z, rows, dim, vocab, topk, ldk=pitch, **kw)
+    refused(ops.linear_cross_entropy, x, w, ids, 0, dim, vocab, lddw=pitch, **kw)
+    art.synchronize()
+
+
+@pytest.mark.parametrize("rows,dim,vocab,piece_rows", [(2 ** 32 - 1, 64, 1000, 0), (2 ** 32 - 1, 64, 1000, 2 ** 31), (2 ** 31, 8, 8, 256), (16, 2 ** 30, 2 ** 30, 0),
+                                                       (16, 64, 2 ** 32 - 1, 0)])
+def test_no_scratch_for_sizes_that_no_call_takes(th, art, rows, dim, vocab, piece_rows):  # noqa: F811
+    assert ops.linear_loss_scratch_bytes(art, rows, dim, vocab, piece_rows=piece_rows) == 0
+    assert ops.linear_loss_scratch_bytes(art, 16, 64, 1000, topk=1025) == 0
