@@ -137,3 +137,31 @@ def test_pitches_that_leave_the_address_space_are_refused(th, art, pitch):  # no
 def test_no_scratch_for_sizes_that_no_call_takes(th, art, rows, dim, vocab, piece_rows):  # noqa: F811
     assert ops.linear_loss_scratch_bytes(art, rows, dim, vocab, piece_rows=piece_rows) == 0
     assert ops.linear_loss_scratch_bytes(art, 16, 64, 1000, topk=1025) == 0
+
+
+@pytest.mark.parametrize("rows,cols,topk,stride", [(2000, 16000, 31, 512), (64, 131000, 256, 512), (1000, 16000, 120, 128)])
+def test_words_a_power_of_two_apart_cost_what_others_cost(th, art, rows, cols, topk, stride):  # noqa: F811
+    """Finding words named twice takes the same time whatever the ids (ids with the same low bits once took 2.6 to 6 times as long)."""
+    g = th.Generator(device="cuda")
+    g.manual_seed(rows + topk)
+    z = th.randn((rows, cols), device="cuda", generator=g)
+    dz, losses = th.empty_like(z), th.empty(rows, device="cuda")
+    teacher = th.randn((rows, topk), device="cuda", generator=g)
+    spread = th.stack([th.randperm(cols, device="cuda", generator=g)[:topk] for _ in range(rows)]).to(th.int32)
+    apart = (th.arange(topk, device="cuda") * stride % cols).to(th.int32).repeat(rows, 1)
+    assert apart[0].unique().numel() == topk
+
+    def run(ids):
+        ops.topk_distill(art, z.data_ptr(), ids.data_ptr(), teacher.data_ptr(), rows, cols, topk, losses=losses.data_ptr(), dlogits=dz.data_ptr())
+
+    took = {}
+    for _ in range(21):
+        for name, ids in (("spread", spread), ("apart", apart)):
+            a, b = th.cuda.Event(enable_timing=True), th.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(4):
+                run(ids)
+            b.record()
+            b.synchronize()
+            took.setdefault(name, []).append(a.elapsed_time(b))
+    assert sorted(took["apart"])[10] < 1.6 * sorted(took["spread"])[10]
