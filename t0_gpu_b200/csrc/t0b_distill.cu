@@ -78,18 +78,23 @@ __device__ __forceinline__ void block_sum2(float& a, float& b, float2* red) {
 
 // exp(z / T) relative to the largest z of a set, as 2^(z c - mc) with c = log2(e) / T and mc = m c rounded: one fused
 // multiply-add whose only rounding is that of the small difference, and references that subtract exactly from one another.
-// Where m c leaves f32's range (logits at the type's lowest value) the difference is taken first.
+// The rounding of mc, up to |mc| 2^-24, is part of every exponent; up to |mc| = 2^22 that is a factor of at most 2^(1/4), which
+// cancels.  Beyond (a row masked with -1e9 as a whole, logits at the type's lowest value) the difference is taken first.
 struct Ref {
     float m, mc;
     bool fused;
-    __device__ __forceinline__ Ref(float m_, float c) : m(m_), mc(m_ * c), fused(fabsf(m_ * c) < 1e37f) {
+    __device__ __forceinline__ Ref(float m_, float c) : m(m_), mc(m_ * c), fused(fabsf(m_ * c) <= 4194304.0f) {
         if (m_ == -INFINITY) { m = mc = 0.0f; fused = true; }   // nothing in the set: exponentials 0, not exp(-inf + inf)
     }
     __device__ __forceinline__ float arg(float z, float c) const { return fused ? fmaf(z, c, -mc) : (z - m) * c; }
     // (z - m) / T, as the exponent's counterpart in the loss.
     __device__ __forceinline__ float log_of(float z, float c, float inv_t) const { return fused ? 0.6931471805599453f * fmaf(z, c, -mc) : (z - m) * inv_t; }
-    // What an exponential relative to this reference is worth relative to `other` (>= this one).
-    __device__ __forceinline__ float to(const Ref& other, float c) const { return exp2_approx(fused && other.fused ? mc - other.mc : (m - other.m) * c); }
+    // What an exponential relative to this reference is worth relative to `other` (>= this one): 2 to the difference of the two
+    // references, mc where a side is fused and m c, unrounded, where it is not.
+    __device__ __forceinline__ float to(const Ref& other, float c) const {
+        const float d = fused ? (other.fused ? mc - other.mc : fmaf(-other.m, c, mc)) : (other.fused ? fmaf(m, c, -other.mc) : (m - other.m) * c);
+        return exp2_approx(d);
+    }
 };
 
 // 16 bytes of logits as floats.

@@ -5,7 +5,7 @@ import math
 import pytest
 
 from t0_gpu_b200 import OUT_BF16, OUT_F32, T0Error, ops
-from test_vocab_losses_gpu import U32, UB, UH, art, losses_and_dz, make_teacher, target_rows, th  # noqa: F401
+from test_vocab_losses_gpu import U32, UB, UH, art, check_logits, losses_and_dz, make_teacher, target_rows, th  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -165,3 +165,37 @@ def test_words_a_power_of_two_apart_cost_what_others_cost(th, art, rows, cols, t
             b.synchronize()
             took.setdefault(name, []).append(a.elapsed_time(b))
     assert sorted(took["apart"])[10] < 1.6 * sorted(took["spread"])[10]
+
+
+# Rows in one CTA's registers, in those of a cluster, in CTAs of 128 threads, streamed, and off 16-byte boundaries.
+FORMS = [(12, 500, 0), (12, 32000, 0), (700, 700, 0), (150, 40000, 0), (12, 500, 1)]
+
+
+@pytest.mark.parametrize("dtype", [OUT_F32, OUT_BF16])
+@pytest.mark.parametrize("temperature", [1.0, 1.5])
+@pytest.mark.parametrize("rows,cols,offset", FORMS)
+def test_logits_of_any_size(th, art, rows, cols, offset, temperature, dtype):  # noqa: F811
+    """Rows masked as a whole with -1e9, -1e30 and the like, whose words are then equally likely; rows whose largest logits are
+    large themselves; masks of that size beside ordinary logits."""
+    def edit(z):
+        for r, v in enumerate((-1e4, -1e9, -1e20, -1e30, -1e37, 1e7, 1e9, 1e30)):
+            z[r] = v
+        z[8, 1:] = -1e30
+        z[9, ::2] = -1e9
+        z[10, :cols // 2] = -3e8
+        z[10, cols // 2:] = -3e8 - 2 ** 23
+        z[11] = 3e6
+        z[11, 7] = 3e6 + 2 ** 14
+
+    check_logits(th, art, rows, cols, 5, dtype=dtype, temperature=temperature, ragged=False, edit=edit, offset=offset)
+
+
+@pytest.mark.parametrize("rows,cols,offset", FORMS)
+def test_slices_whose_maxima_differ_little_and_are_large(th, art, rows, cols, offset):  # noqa: F811
+    """Maxima of a row's slices around 2^21, 2^22 and 2^23 over log2(e), a few apart."""
+    def edit(z):
+        for r, v in enumerate((2 ** 21, 2 ** 22, 2 ** 23, -2 ** 21, -2 ** 22, -2 ** 23)):
+            z[r] = v * math.log(2) + th.randint(-3, 4, (cols,), device="cuda")
+            z[r, ::100] += th.arange(len(z[r, ::100]), device="cuda") % 5
+
+    check_logits(th, art, rows, cols, 5, ragged=False, edit=edit, offset=offset)
