@@ -475,7 +475,8 @@ T0B_API int32_t t0b_embedding_bwd(t0b_ctx* ctx, uint64_t grad_table, uint64_t id
  * ids u32 and teacher f32 [rows, topk] at a pitch of ldk, topk <= T0B_MAX_TOPK, in any order: the words the teacher scored
  * and its logits, of which q is the softmax at the same temperature T.  A word that a row names twice counts twice.
  * losses f32[rows] or 0; dlogits [rows, cols] f32 or bf16 (grad_dtype), same ld, or 0 -- it may be `logits` itself when the
- * types agree; row_weights f32[rows] or 0 (all 1). */
+ * types agree; row_weights f32[rows] or 0 (all 1).  bf16 logits with a bf16 gradient may go through fp16 exponentials on the way to
+ * it, 2^-11 of themselves or 2^-40 of the row's largest off before the gradient is rounded; everything else is f32. */
 T0B_API int32_t t0b_topk_distill(t0b_ctx* ctx, uint64_t logits, int32_t logits_dtype, uint64_t ids, uint64_t teacher,
                                  uint64_t row_weights, uint64_t losses, uint64_t dlogits, int32_t grad_dtype, uint32_t rows,
                                  uint32_t cols, uint64_t ld, uint32_t topk, uint64_t ldk, float temperature, float scale,

@@ -199,3 +199,31 @@ def test_slices_whose_maxima_differ_little_and_are_large(th, art, rows, cols, of
             z[r, ::100] += th.arange(len(z[r, ::100]), device="cuda") % 5
 
     check_logits(th, art, rows, cols, 5, ragged=False, edit=edit, offset=offset)
+
+
+@pytest.mark.parametrize("rows,cols,offset", FORMS)
+def test_gradients_of_unlikely_words(th, art, rows, cols, offset):  # noqa: F811
+    """One word takes almost all of the probability; the others' gradients, 2^-25 to 2^-37 of its, stay.  bf16 in and out: the
+    exponentials may have gone through fp16, 2^15 times what they are relative to the largest: 2^-11 of themselves or 2^-40 of the
+    largest off, then rounded to bf16."""
+    g = th.Generator(device="cuda")
+    g.manual_seed(cols)
+    buf = th.empty(rows * cols + offset, device="cuda", dtype=th.bfloat16)
+    z = buf[offset:].view(rows, cols)
+    z.copy_(th.randn((rows, cols), device="cuda", generator=g) - 18)
+    z[:, 5] = 4
+    ids = th.tensor([[5, 9]], device="cuda", dtype=th.int32).repeat(rows, 1)
+    teacher = th.zeros((rows, 2), device="cuda")
+    losses, out = th.empty(rows, device="cuda"), th.empty_like(buf)
+    dz = out[offset:].view(rows, cols)
+    ops.topk_distill(art, z.data_ptr(), ids.data_ptr(), teacher.data_ptr(), rows, cols, 2, logits_dtype=OUT_BF16, grad_dtype=OUT_BF16, scale=1.0,
+                     losses=losses.data_ptr(), dlogits=dz.data_ptr())
+    art.synchronize()
+    zd = z.double()
+    p = th.softmax(zd, 1)
+    down = zd.amax(1, keepdim=True) - zd
+    others = th.ones(cols, device="cuda", dtype=th.bool)
+    others[[5, 9]] = False
+    bound = UB * p + (1 + UB) * (p * (UH + (down * 4 + 16) * 2 * U32) + 2.0 ** -40 * p.amax(1, keepdim=True))
+    assert ((dz.double() - p).abs() <= bound)[:, others].all()
+    assert (dz[:, others] > 0).all() and p[:, others].min() < 2.0 ** -34 and p[:, others].max() < 2.0 ** -24
