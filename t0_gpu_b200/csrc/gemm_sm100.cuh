@@ -20,6 +20,7 @@
 #include <cstdint>
 
 #include "ptx_sm100.cuh"
+#include "t0b_internal.hpp"
 
 namespace t0b {
 
@@ -65,9 +66,9 @@ constexpr int kMaxDst = 8;
 // warp leaves, for each of its 32 rows and its own columns (a "part" of the row, GemmTraits::kPartCols wide),
 //   part[j] = (max z, sum of exp((z - max) / T)),
 // which a later kernel joins over the parts of the row; the raw z of the columns that the row asks for (`ids`); and, when a
-// gradient follows, u = exp((z - max) / T) in fp16 through the third tensor map.  u lies in [0, 1] with at least one 1 in
-// every part, so fp16 keeps 11 significant bits of everything above 2^-14 of the part's largest exponential and is off by
-// at most 2^-25 of it below; bf16 would lose three bits on the probabilities that carry the gradient.
+// gradient follows, u = kHeadUScale exp((z - max) / T) in fp16 through the third tensor map.  The exponentials lie in [0, 1] with
+// at least one 1 in every part, so fp16 keeps 11 significant bits of everything above 2^-29 of the part's largest and is off by
+// at most 2^-40 of it below; bf16 would lose three bits on the probabilities that carry the gradient.
 // The tensor core's own sums drop what falls below the accumulator's last bit, at every 16 products; over a long contraction
 // that is a bias.  So a row's logit is summed in pieces of 512 products, in alternating accumulators, and the pieces are
 // added in the epilogue's registers, behind the next piece's products.  Losses over 50257 words at dim 2048 are then off by
@@ -454,7 +455,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-// fp16 form of stage_chunk_bf16_sw64.
+// fp16 form of stage_chunk_bf16_sw64, times kHeadUScale.
 __device__ __forceinline__ void stage_chunk_f16_sw64(uint32_t half_tile, int lane, const float* v) {
     const uint32_t row = half_tile + lane * 64;
     const int x = (lane >> 1) & 3;
@@ -463,7 +464,7 @@ __device__ __forceinline__ void stage_chunk_f16_sw64(uint32_t half_tile, int lan
         uint32_t h[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const __half2 t = __floats2half2_rn(v[8 * j + 2 * e], v[8 * j + 2 * e + 1]);
+            const __half2 t = __floats2half2_rn(kHeadUScale * v[8 * j + 2 * e], kHeadUScale * v[8 * j + 2 * e + 1]);
             h[e] = *reinterpret_cast<const uint32_t*>(&t);
         }
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + ((j ^ x) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");

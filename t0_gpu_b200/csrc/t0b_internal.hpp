@@ -151,6 +151,7 @@ size_t inner_gemm_slab_bytes(t0b_ctx* ctx, const InnerGemm& d);
 int32_t inner_gemm(t0b_ctx* ctx, const InnerGemm& d);
 
 // The product x * head whose epilogue leaves softmax statistics instead of logits (HeadParams, gemm_sm100.cuh).
+constexpr float kHeadUScale = 32768.0f;   // of the exponentials that it leaves in fp16
 struct HeadPlan { uint32_t bm, bn, cta_group, part_cols; };
 HeadPlan head_plan(t0b_ctx* ctx, uint32_t rows, uint32_t vocab, uint32_t dim);
 struct HeadGemm {

@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(1024) join_parts_kernel(const float2* part, un
 }
 
 // ---------------------------------------------------------------------------------------------------- the gradient of z
-// u (fp16, relative to its part's maximum) becomes dz (bf16) in place: a block takes kGradCols columns of one row.  The
+// u (fp16, kHeadUScale relative to its part's maximum) becomes dz (bf16) in place: a block takes kGradCols columns of one row.  The
 // words of the targets are written last, from their f32 logit.  Bound by HBM: 2 bytes in, 2 bytes out per element (4096 x
 // 128000: 358 us, 5.9 TB/s).  Two small steps ride along where their own launch would cost more than they do:
 //   JOIN   every block joins its row's parts itself, and the row's first block finishes the loss (join_parts_kernel is not
@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(256) dz_kernel(__half* u, unsigned long long l
         if (col >= ldu) continue;
         uint4 o = make_uint4(0, 0, 0, 0);
         if (live) {
-            const float f = a * (exp2_approx((top[v] - st.x) * c) * inv);
+            const float f = a * (exp2_approx((top[v] - st.x) * c) * inv) * (1.0f / kHeadUScale);
             const uint32_t w[4] = {raw[v].x, raw[v].y, raw[v].z, raw[v].w};
             float g[8];
 #pragma unroll

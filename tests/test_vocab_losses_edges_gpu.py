@@ -227,3 +227,37 @@ def test_gradients_of_unlikely_words(th, art, rows, cols, offset):  # noqa: F811
     bound = UB * p + (1 + UB) * (p * (UH + (down * 4 + 16) * 2 * U32) + 2.0 ** -40 * p.amax(1, keepdim=True))
     assert ((dz.double() - p).abs() <= bound)[:, others].all()
     assert (dz[:, others] > 0).all() and p[:, others].min() < 2.0 ** -34 and p[:, others].max() < 2.0 ** -24
+
+
+@pytest.mark.parametrize("trans_w", [False, True])
+@pytest.mark.parametrize("rows,vocab", [(40, 300), (300, 500)])
+def test_head_gradients_of_unlikely_words(th, art, rows, vocab, trans_w):  # noqa: F811
+    """One word takes almost all of the probability in every row: the head's gradient at the others, p of 2^-26 to 2^-36, is a
+    sum of terms with one sign.  Bounds as for the other linear tests, with 2^-40 of the part's largest below fp16's range."""
+    dim = 64
+    g = th.Generator(device="cuda")
+    g.manual_seed(rows)
+    x = th.rand((rows, dim), device="cuda", generator=g).bfloat16()
+    x[:, 0] = 8
+    w = (th.randn((vocab, dim), device="cuda", generator=g) / 8).bfloat16()
+    w[:, 0] = 0
+    w[5, 0] = 2.75
+    tgt = th.full((rows,), 5, device="cuda", dtype=th.int32)
+    head = w if trans_w else w.t().contiguous()
+    losses, dx, dw = th.empty(rows, device="cuda"), th.empty((rows, dim), device="cuda"), th.empty(head.shape, device="cuda")
+    ops.linear_cross_entropy(art, x.data_ptr(), head.data_ptr(), tgt.data_ptr(), rows, dim, vocab, trans_w=trans_w, x_dtype=OUT_BF16, w_dtype=OUT_BF16,
+                             scale=1.0, losses=losses.data_ptr(), dx=dx.data_ptr(), dw=dw.data_ptr())
+    art.synchronize()
+    xd, wd = x.double(), w.double()
+    z = xd @ wd.t()
+    p = th.softmax(z, 1)
+    ez = dim * U32 * (xd @ wd.abs().t()).amax(1, keepdim=True)
+    down = z.amax(1, keepdim=True) - z
+    ep = 2 * ez + down * 4 * U32 + 8 * U32
+    edz = UB * p + p * (ep + UH + UB * UH) + 2.0 ** -40 * p.amax(1, keepdim=True)
+    others = th.ones(vocab, device="cuda", dtype=th.bool)
+    others[5] = False
+    got = (dw if trans_w else dw.t()).double()
+    want, err = p.t() @ xd, edz.t() @ xd + rows * U32 * ((p + edz).t() @ xd)
+    assert ((got - want).abs() <= err + U32 * (want + err))[others].all()
+    assert (got[others] > 0).all() and p[:, others].min() < 2.0 ** -33
