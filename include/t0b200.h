@@ -487,10 +487,12 @@ T0B_API int32_t t0b_topk_distill(t0b_ctx* ctx, uint64_t logits, int32_t logits_d
  * [dim, vocab] as Linear stores it (trans_w = 0) or [vocab, dim] as an embedding table (trans_w = 1); any sizes and pitches
  * (elements), copied into the scratch first where TMA cannot address them.
  * With dx and dw 0 only the losses (and lse[r] = log sum exp(z / T)) are computed.  With dx and / or dw, which have the
- * shapes of x and w in f32 or bf16, the exponentials of a piece of the rows (at most 1 GiB; piece_rows rows where that is
- * not 0) stand in the scratch until the piece's gradient is done, in fp16: 2^-11 of themselves or 2^-40 of the largest in their
- * 64 or 128 columns off; dw sums over the pieces in f32.  The operands of the two gradient products are bf16 (dz is rounded to
- * it, where dx and dw are f32 too), their sums f32; results do not depend on run, stream or scratch.
+ * shapes of x and w in f32 or bf16, the exponentials of a piece of the rows (as many as 1 GiB holds, and 256 at least;
+ * piece_rows where that is not 0) stand in the scratch until the piece's gradient is done, in fp16: 2^-11 of themselves or 2^-40
+ * of the largest in their 64 or 128 columns off; dw sums over the pieces in f32.  The operands of the two gradient products are
+ * bf16 (dz is rounded to it, where dx and dw are f32 too), their sums f32.  The same call gives the same bits on every run and
+ * stream.  The order of dx's sum follows the choice of tiles (t0b_tune), and a scratch that ends before the place for its
+ * partial sums is taken too: dx is then summed in one piece.
  * scratch: 256-byte aligned, t0b_linear_loss_scratch_bytes() bytes; 0 = a workspace of the context that grows as needed.  A
  * call that is being captured into a graph must bring its own and keep it as long as the graph; graphs (or contexts) that
  * may run at the same time need one each. */

@@ -6,7 +6,7 @@
 // row's part (head_gemm); a join over the parts gives the row's log-sum-exp and its loss.  That is all that an evaluation
 // does: 2 rows dim vocab operations, and nothing of the size rows x vocab is written.
 // For the gradient the same epilogue also leaves the exponentials of a piece of the rows, relative to their part's maximum,
-// in 16 bits (at most 1 GiB, whatever the number of rows); one pass turns them into dz in place, and two products give dx
+// in 16 bits (at most 1 GiB, or what 256 rows take, whatever the number of rows); one pass turns them into dz in place, and two products give dx
 // and the head's gradient, which sums over the pieces in f32.  6 rows dim vocab operations in all: computing the exponentials
 // anew once the sums are known would cost 8, and the pass over 16-bit exponentials costs 4 bytes per element against
 // 2 dim operations (at dim 4096: 4 % of the step instead of 33 %).

@@ -261,3 +261,33 @@ def test_head_gradients_of_unlikely_words(th, art, rows, vocab, trans_w):  # noq
     want, err = p.t() @ xd, edz.t() @ xd + rows * U32 * ((p + edz).t() @ xd)
     assert ((got - want).abs() <= err + U32 * (want + err))[others].all()
     assert (got[others] > 0).all() and p[:, others].min() < 2.0 ** -33
+
+
+def test_a_scratch_without_room_for_partial_sums(th, art):  # noqa: F811
+    """A scratch sized before a tuning that splits dx's sum: dx is summed in one piece, losses and dw are the same bits; a scratch
+    that ends earlier is refused."""
+    rows, dim, vocab = 64, 256, 20000
+    g = th.Generator(device="cuda")
+    g.manual_seed(2)
+    x = th.randn((rows, dim), device="cuda", generator=g).bfloat16()
+    w = (th.randn((vocab, dim), device="cuda", generator=g) / 16).bfloat16()
+    tgt = th.randint(0, vocab, (rows,), device="cuda", generator=g).to(th.int32)
+    whole = ops.linear_loss_scratch_bytes(art, rows, dim, vocab, trans_w=True, x_dtype=OUT_BF16)
+    got = []
+    for size in (whole, whole - 256):
+        losses, dx, dw = th.empty(rows, device="cuda"), th.empty((rows, dim), device="cuda"), th.empty((vocab, dim), device="cuda")
+        scratch = art.alloc(size)
+        ops.linear_cross_entropy(art, x.data_ptr(), w.data_ptr(), tgt.data_ptr(), rows, dim, vocab, trans_w=True, x_dtype=OUT_BF16, w_dtype=OUT_BF16,
+                                 losses=losses.data_ptr(), dx=dx.data_ptr(), dw=dw.data_ptr(), scratch=scratch)
+        art.synchronize()
+        got.append((losses, dx, dw))
+    (l0, dx0, dw0), (l1, dx1, dw1) = got
+    assert th.equal(l0, l1) and th.equal(dw0, dw1)
+    # the same products in another order: each sum is off by at most vocab 2^-23 of the sum of their sizes, |dz| <= p + q
+    z = x.double() @ w.double().t()
+    size = (th.softmax(z, 1) / rows) @ w.double().abs() + w.double().abs()[tgt.long()] / rows
+    assert ((dx0 - dx1).double().abs() <= 2 * vocab * U32 * size).all()
+    small = art.alloc(rows * vocab * 2)      # the exponentials alone
+    with pytest.raises(T0Error, match="scratch must be"):
+        ops.linear_cross_entropy(art, x.data_ptr(), w.data_ptr(), tgt.data_ptr(), rows, dim, vocab, trans_w=True, x_dtype=OUT_BF16, w_dtype=OUT_BF16,
+                                 losses=l0.data_ptr(), dx=dx0.data_ptr(), dw=dw0.data_ptr(), scratch=small)
