@@ -825,6 +825,8 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
                static_cast<uint32_t>(p.w_rows), static_cast<uint32_t>(p.w_cols));
         ++launched;
     }
+    rc = check_cuda(ctx, cudaGetLastError(), what);   // what follows takes row numbers from these kernels
+    if (rc != T0B_OK) return rc;
     uint32_t part_shift = 0;
     while ((1u << part_shift) < p.head.part_cols) ++part_shift;
     for (uint32_t r0 = 0; r0 < d.rows; r0 += p.piece) {
