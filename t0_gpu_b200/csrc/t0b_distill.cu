@@ -815,6 +815,7 @@ int32_t t0b_topk_distill(t0b_ctx* ctx, uint64_t logits, int32_t logits_dtype, ui
         return set_error(ctx, T0B_ERR_INVALID, "topk_distill: topk %u is outside 1..%d, or its pitch %llu is smaller", topk, T0B_MAX_TOPK, static_cast<unsigned long long>(ldk));
     if (!(temperature > 0.0f) || !std::isfinite(temperature) || !std::isfinite(1.4426950408889634f / temperature) || !std::isfinite(scale))
         return set_error(ctx, T0B_ERR_INVALID, "topk_distill: temperature %g and its inverse must be positive and finite, scale %g finite", temperature, scale);
+    if (!std::isfinite(scale / temperature)) return set_error(ctx, T0B_ERR_INVALID, "topk_distill: scale %g over temperature %g is not finite", scale, temperature);
     const size_t ie = logits_dtype == T0B_OUT_BF16 ? 2 : 4, oe = grad_dtype == T0B_OUT_BF16 ? 2 : 4;
     if (logits % ie || (dlogits && dlogits % oe) || ids % 4 || teacher % 4 || losses % 4 || row_weights % 4)
         return set_error(ctx, T0B_ERR_INVALID, "topk_distill: a pointer is not aligned to its element");

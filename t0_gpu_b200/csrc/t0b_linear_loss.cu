@@ -874,7 +874,7 @@ int32_t run_linear_loss(t0b_ctx* ctx, const char* what, const t0b_linear_loss& d
         for (uint32_t y0 = 0; y0 < n; y0 += 65535u) {   // gridDim.y is limited to 65535
             launch(ctx, p.join_in_dz ? dz_kernel<true> : dz_kernel<false>, dim3(static_cast<uint32_t>((p.ldu + kGradCols - 1) / kGradCols), std::min(65535u, n - y0)),
                    256, 0, reinterpret_cast<__half*>(base + p.u), p.ldu, n, y0, reinterpret_cast<const float2*>(base + p.part), p.part_ld, part_shift, stats,
-                   reinterpret_cast<const float*>(d.row_weights), d.scale * inv_t, c, tg, jp, cp);
+                   reinterpret_cast<const float*>(d.row_weights), d.scale / temperature, c, tg, jp, cp);
             ++launched;
         }
         rc = check_cuda(ctx, cudaGetLastError(), what);
@@ -956,6 +956,8 @@ int32_t t0b_linear_topk_distill(t0b_ctx* ctx, const t0b_linear_loss* loss, uint6
                          static_cast<unsigned long long>(ldk));
     if (!(temperature > 0.0f) || !std::isfinite(temperature) || !std::isfinite(1.4426950408889634f / temperature))
         return set_error(ctx, T0B_ERR_INVALID, "linear_topk_distill: temperature %g must be positive and finite, and so must its inverse", temperature);
+    if (!std::isfinite(loss->scale / temperature))
+        return set_error(ctx, T0B_ERR_INVALID, "linear_topk_distill: scale %g over temperature %g is not finite", loss->scale, temperature);
     std::lock_guard<std::recursive_mutex> lk(ctx->mu);
     rc = check_desc(ctx, "linear_topk_distill", *loss);
     if (rc == T0B_OK && loss->rows > 0)

@@ -291,3 +291,16 @@ def test_a_scratch_without_room_for_partial_sums(th, art):  # noqa: F811
     with pytest.raises(T0Error, match="scratch must be"):
         ops.linear_cross_entropy(art, x.data_ptr(), w.data_ptr(), tgt.data_ptr(), rows, dim, vocab, trans_w=True, x_dtype=OUT_BF16, w_dtype=OUT_BF16,
                                  losses=l0.data_ptr(), dx=dx0.data_ptr(), dw=dw0.data_ptr(), scratch=small)
+
+
+def test_a_gradient_scale_outside_f32_is_refused(th, art):  # noqa: F811
+    """scale / temperature multiplies every gradient: infinite, it would leave no finite one."""
+    x = th.zeros((4, 64), device="cuda")
+    ids = th.zeros((4, 2), device="cuda", dtype=th.int32)
+    a = x.data_ptr()
+    for scale in (3e38, -3e38):
+        with pytest.raises(T0Error, match="scale"):
+            ops.topk_distill(art, a, ids.data_ptr(), a, 4, 64, 2, temperature=0.1, scale=scale, losses=a, dlogits=a)
+        with pytest.raises(T0Error, match="scale"):
+            ops.linear_topk_distill(art, a, a, ids.data_ptr(), a, 4, 8, 8, 2, temperature=0.1, scale=scale, x_dtype=OUT_BF16, w_dtype=OUT_BF16, losses=a, dx=a, dw=a)
+    art.synchronize()
