@@ -21,9 +21,9 @@ TRACE_OUT = os.path.join(OUT_DIR, "libt0b200_trace.so")
 TRACE_OBJ_DIR = os.path.join(OUT_DIR, "obj_trace")
 
 SOURCES = ["t0b_runtime.cu", "t0b_gemm.cu", "t0b_rowops.cu", "t0b_embedding.cu", "t0b_distill.cu", "t0b_linear_loss.cu", "t0b_util.cu", "t0b_gemm_gen.cpp", "t0b_tile_ir.cpp"]
-# The GEMM kernel variants (BN, CG, MT, ND, HEAD): gemm_variant.cu compiled once per entry, side by side.
-GEMM_VARIANTS = ["256,2,2,1,0", "256,2,2,0,0", "256,2,1,0,0", "128,2,1,0,0", "256,1,1,0,0", "128,1,1,0,0", "64,1,1,0,0",
-                 "256,2,1,0,1", "256,1,1,0,1", "128,1,1,0,1"]
+# The GEMM kernel variants (BN, CG, MT, ND, KIND): gemm_variant.cu compiled once per entry, side by side.
+GEMM_TILES = ["256,2,2,1", "256,2,2,0", "256,2,1,0", "128,2,1,0", "256,1,1,0", "128,1,1,0", "64,1,1,0"]
+GEMM_VARIANTS = [t + k for k in (",0", ",2") for t in GEMM_TILES] + ["256,2,1,0,1", "256,1,1,0,1", "128,1,1,0,1"]
 HEADERS = ["gemm_sm100.cuh", "gemm_launch.cuh", "ptx_sm100.cuh", "t0b_internal.hpp", "t0b_tuned_table.inc", os.path.join("..", "..", "include", "t0b200.h")]
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -46,7 +46,7 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False) -> st
     hdr_time = _newest([os.path.join(CSRC, h) for h in HEADERS])
     objs, jobs = [], []
     units = [(src, os.path.splitext(src)[0] + ".o", []) for src in SOURCES]
-    units += [("gemm_variant.cu", "gemm_variant_" + v.replace(",", "_") + ".o", ["-DT0B_V_%s=%s" % (k, x) for k, x in zip(("BN", "CG", "MT", "ND", "HEAD"), v.split(","))])
+    units += [("gemm_variant.cu", "gemm_variant_" + v.replace(",", "_") + ".o", ["-DT0B_V_%s=%s" % (k, x) for k, x in zip(("BN", "CG", "MT", "ND", "KIND"), v.split(","))])
               for v in GEMM_VARIANTS]
     for src, obj_name, defines in units:
         sp = os.path.join(CSRC, src)

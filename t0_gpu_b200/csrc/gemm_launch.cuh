@@ -10,11 +10,11 @@
 
 namespace t0b {
 
-template <int BN, int CG, int MT, int ND = 0, int HEAD = 0>
+template <int BN, int CG, int MT, int ND = 0, int KIND = 0>
 int32_t launch_variant(t0b_ctx* ctx, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc,
-                       const GemmParams& p, int num_work, int cluster_sk = 0) {
+                       const KernelParams<KIND>& p, int num_work, int cluster_sk = 0) {
     using T = GemmTraits<BN, CG, MT, ND>;
-    auto kfn = gemm_bf16_tcgen05_kernel<BN, CG, MT, ND, HEAD>;
+    auto kfn = gemm_bf16_tcgen05_kernel<BN, CG, MT, ND, KIND>;
     static bool configured[64] = {};
     static int max_clusters[64] = {};
     static std::mutex config_mu;   // several contexts (threads) may launch the same variant for the first time at once
@@ -110,15 +110,16 @@ int max_active_splitk_clusters(t0b_ctx* ctx, int cluster_sk) {
     return nc;
 }
 
-#define T0B_GEMM_VARIANTS(X) X(256, 2, 2, 1, 0) X(256, 2, 2, 0, 0) X(256, 2, 1, 0, 0) X(128, 2, 1, 0, 0) X(256, 1, 1, 0, 0) X(128, 1, 1, 0, 0) X(64, 1, 1, 0, 0) \
-    X(256, 2, 1, 0, 1) X(256, 1, 1, 0, 1) X(128, 1, 1, 0, 1)
+#define T0B_GEMM_TILES(X, KIND) \
+    X(256, 2, 2, 1, KIND) X(256, 2, 2, 0, KIND) X(256, 2, 1, 0, KIND) X(128, 2, 1, 0, KIND) X(256, 1, 1, 0, KIND) X(128, 1, 1, 0, KIND) X(64, 1, 1, 0, KIND)
+#define T0B_GEMM_VARIANTS(X) T0B_GEMM_TILES(X, 0) T0B_GEMM_TILES(X, 2) X(256, 2, 1, 0, 1) X(256, 1, 1, 0, 1) X(128, 1, 1, 0, 1)
 #ifndef T0B_VARIANT
 extern template int max_active_splitk_clusters<256>(t0b_ctx*, int);
 extern template int max_active_splitk_clusters<128>(t0b_ctx*, int);
 extern template int max_active_splitk_clusters<64>(t0b_ctx*, int);
-#define T0B_EXTERN_VARIANT(BN, CG, MT, ND, HEAD)                                                                        \
-    extern template int32_t launch_variant<BN, CG, MT, ND, HEAD>(t0b_ctx*, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, \
-                                                            const GemmParams&, int, int);
+#define T0B_EXTERN_VARIANT(BN, CG, MT, ND, KIND)                                                                        \
+    extern template int32_t launch_variant<BN, CG, MT, ND, KIND>(t0b_ctx*, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, \
+                                                            const KernelParams<KIND>&, int, int);
 T0B_GEMM_VARIANTS(T0B_EXTERN_VARIANT)
 #undef T0B_EXTERN_VARIANT
 #endif

@@ -8,7 +8,9 @@
 // the K tail contributes zeros, :768-787) -- here the zero fill is TMA's out-of-bounds fill, so callers
 // do not have to pad.
 //
-// HEAD = 1 replaces the store of C by the softmax epilogue of a vocabulary head (HeadParams).
+// KIND 0 is the product alone; 1 replaces the store of C by the softmax epilogue of a vocabulary head (HeadParams); 2 is a
+// product inside another operator (InnerParams).  In one kernel, what the last two need made launch-bound products 0.3 to 0.5 us
+// slower (512^3: 6.9 instead of 6.55 us); 112 bytes more of parameters alone cost 0.13 us.
 //
 // Roles per CTA: warp 0 = TMA producer, warp 1 = TMEM owner + MMA issuer, then four or eight epilogue warps
 // (TMEM -> registers -> shared-memory transpose tile -> TMA store or coalesced row stores): 192 threads for the
@@ -62,7 +64,7 @@ enum DeviceStatus : int {
 
 constexpr int kMaxDst = 8;
 
-// The softmax epilogue of a vocabulary head (kernels with HEAD = 1): instead of the products z of a tile, every epilogue
+// The softmax epilogue of a vocabulary head (KIND = 1): instead of the products z of a tile, every epilogue
 // warp leaves, for each of its 32 rows and its own columns (a "part" of the row, GemmTraits::kPartCols wide),
 //   part[j] = (max z, sum of exp((z - max) / T)),
 // which a later kernel joins over the parts of the row; the raw z of the columns that the row asks for (`ids`); and, when a
@@ -109,16 +111,23 @@ struct GemmParams {
 #ifdef T0B_TRACE
     unsigned long long* trace;   // timeline build only: [CTA][16] stamps of this launch (null = no stamps)
 #endif
-    int accumulate;         // 1: C += the product (f32 output, one destination, no split-K)
+    int cluster_sk;         // > 1: split-K inside a thread-block cluster of that many CTAs (one per K range): the partial
+                            // tiles stay in shared memory and are summed over distributed shared memory; 0 = slabs
+};
+
+// What a product inside another operator adds.
+struct InnerParams {
     // Rows counted on the device: M (dyn_k = 0) or K (dyn_k = 1) is at most *dyn_rows - dyn_off, and the launch was sized for
     // the most there can be.  K comes as whole blocks of zero rows behind the last (one at least).
     const int* dyn_rows;
     int dyn_off, dyn_k;
+    int accumulate;         // 1: C += the product (f32 output, one destination, no split-K)
     int late_wait;          // 1: the operands were complete before the kernel in front of this one began; wait for it at the end only
-    HeadParams head;        // HEAD kernels only
-    int cluster_sk;         // > 1: split-K inside a thread-block cluster of that many CTAs (one per K range): the partial
-                            // tiles stay in shared memory and are summed over distributed shared memory; 0 = slabs
 };
+template <int KIND> struct KernelParams;
+template <> struct KernelParams<0> : GemmParams {};
+template <> struct KernelParams<1> : GemmParams { InnerParams inner; HeadParams head; };   // of inner the rows alone
+template <> struct KernelParams<2> : GemmParams { InnerParams inner; };
 
 constexpr int kBmCta = 128;   // accumulator rows per MMA per CTA (TMEM lanes)
 constexpr int kBk = 64;       // K block: 64 bf16 = one 128-byte swizzle row
@@ -325,12 +334,25 @@ __device__ __forceinline__ void flush_chunk_f32(uint32_t stage, int lane, float*
         }
     }
 }
-// 128-byte rows of a staging tile to any address, pitch and number of columns (ES bytes an element, `bytes` of each row): eight
-// lanes a row; the whole 16-byte pieces of the destination are shifted together from two pieces of the tile, what is left at
-// a row's ends goes element by element.  (One row a lane touched 32 sectors with every store: 4416 x 25851 bf16 from 5 rows
-// took 1.2 ms, one element a lane 240 us.)
-template <int ES>
-__device__ __forceinline__ void flush_rows_any(uint32_t stage, int lane, char* base, long long pitch, int rows, int bytes, bool add) {
+// Rows of a staging tile to any address, pitch and number of columns.  (One row a lane touched 32 sectors with every store:
+// 4416 x 25851 bf16 from 5 rows took 1.2 ms, 4096 x 1003 x 1024 bf16 54 us.)
+// f32, a 32x32 chunk: one column a lane, one row an iteration -- whole rows of 128 bytes, whatever they start on (4096 x 1003 x
+// 1024: 14.3 us; shifting 16-byte pieces together as below 19.3 us).
+__device__ __forceinline__ void flush_rows_f32(uint32_t stage, int lane, float* base, long long ld, int rows, int cols, bool add) {
+    const uint32_t piece = lane >> 2, rest = (lane & 3) * 4;
+    float* dst = base + lane;
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+        float v;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(stage + r * 128 + ((piece ^ (r & 7)) << 4) + rest));
+        if (r < rows && lane < cols) *dst = add ? *dst + v : v;
+        dst += ld;
+    }
+}
+// bf16, 32x64 (`bytes` of each row, `pitch` in bytes too): eight lanes a row; the whole 16-byte pieces of the destination are
+// shifted together from two pieces of the tile, what is left at a row's ends goes element by element (44 x 1664 -> 32027 with
+// gradients: 174 us; one column a lane as above 214 us).
+__device__ __forceinline__ void flush_rows_bf16(uint32_t stage, int lane, char* base, long long pitch, int rows, int bytes) {
     const int c = lane & 7;
 #pragma unroll 2
     for (int t = 0; t < 8; ++t) {
@@ -351,36 +373,28 @@ __device__ __forceinline__ void flush_rows_any(uint32_t stage, int lane, char* b
             for (int e = 0; e < 6; ++e) w[e] = (front & 8) ? w[e + 2] : w[e];
 #pragma unroll
             for (int e = 0; e < 5; ++e) w[e] = (front & 4) ? w[e + 1] : w[e];
-            if constexpr (ES == 2) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = __funnelshift_r(w[e], w[e + 1], (front & 2) * 8);
-            }
-            uint4* out = reinterpret_cast<uint4*>(dst + front) + c;
-            if (ES == 4 && add) {
-                const float4 o = *reinterpret_cast<const float4*>(out);
-                w[0] = __float_as_uint(o.x + __uint_as_float(w[0]));
-                w[1] = __float_as_uint(o.y + __uint_as_float(w[1]));
-                w[2] = __float_as_uint(o.z + __uint_as_float(w[2]));
-                w[3] = __float_as_uint(o.w + __uint_as_float(w[3]));
-            }
-            *out = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int e = 0; e < 4; ++e) w[e] = __funnelshift_r(w[e], w[e + 1], (front & 2) * 8);
+            reinterpret_cast<uint4*>(dst + front)[c] = make_uint4(w[0], w[1], w[2], w[3]);
         }
         auto element = [&](int at) {   // byte offset in the row
             const uint32_t addr = row + ((((at >> 4) ^ (r & 7)) << 4) | (at & 15));
-            if constexpr (ES == 2) {
-                uint16_t v;
-                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
-                *reinterpret_cast<uint16_t*>(dst + at) = v;
-            } else {
-                float v;
-                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
-                float* d = reinterpret_cast<float*>(dst + at);
-                *d = add ? *d + v : v;
-            }
+            uint16_t v;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
+            *reinterpret_cast<uint16_t*>(dst + at) = v;
         };
-        if (r < rows && c * ES < front) element(c * ES);
-        if (r < rows && front + pieces * 16 + c * ES < bytes) element(front + pieces * 16 + c * ES);
+        if (r < rows && c * 2 < front) element(c * 2);
+        if (r < rows && front + pieces * 16 + c * 2 < bytes) element(front + pieces * 16 + c * 2);
     }
+}
+// The same out of line.  Inlined, they take registers from the paths of every aligned product where 320 threads leave 168 to each
+// (128 x 4096 x 4096: 13.3 us, and 12.6 us with calls); the 64-column tile's 192 threads have enough, and calls slow it down
+// (512^3: 6.93 us, and 6.55 us without).
+static __device__ __noinline__ void flush_rows_f32_call(uint32_t stage, int lane, float* base, long long ld, int rows, int cols, bool add) {
+    flush_rows_f32(stage, lane, base, ld, rows, cols, add);
+}
+static __device__ __noinline__ void flush_rows_bf16_call(uint32_t stage, int lane, char* base, long long pitch, int rows, int bytes) {
+    flush_rows_bf16(stage, lane, base, pitch, rows, bytes);
 }
 // TMA-store path: every 32x32 chunk goes out through two 2 KiB half tiles (rows of 64 bytes, 64-byte TMA swizzle:
 // 16-byte piece c of row r sits at piece c ^ ((r >> 1) & 3)), so that one half is being read by its TMA store while
@@ -471,10 +485,10 @@ __device__ __forceinline__ void stage_chunk_f16_sw64(uint32_t half_tile, int lan
     }
 }
 
-template <int BN, int CG, int MT, int ND = 0, int HEAD = 0>
+template <int BN, int CG, int MT, int ND = 0, int KIND = 0>
 __global__ void __launch_bounds__(GemmTraits<BN, CG, MT, ND>::kThreads, 1)
 gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                         const __grid_constant__ CUtensorMap tmap_c, const GemmParams p) {
+                         const __grid_constant__ CUtensorMap tmap_c, const KernelParams<KIND> p) {
     using T = GemmTraits<BN, CG, MT, ND>;
     constexpr int S = T::kStages;
     constexpr int BM = T::kBm;
@@ -543,20 +557,28 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
     if (threadIdx.x == 0) T0B_STAMP(1);
     // Programmatic dependent launch: everything above (barriers, TMEM, descriptor prefetch) may run while the previous
     // kernel of the stream drains; nothing below may touch global memory before that kernel has completed.
-    if (!p.late_wait) ptx::grid_dependency_wait();
+    bool late_wait = false, accumulate = false;
+    if constexpr (KIND == 2) {
+        late_wait = p.inner.late_wait != 0;
+        accumulate = p.inner.accumulate != 0;
+    }
+    if (!late_wait) ptx::grid_dependency_wait();
     if (threadIdx.x == 0) T0B_STAMP(2);
     ptx::grid_launch_dependents();   // the next GEMM's CTAs may take over SMs as this grid's CTAs exit
-    if (p.dyn_rows != nullptr) {
-        const int n = max(0, min(*p.dyn_rows - p.dyn_off, p.dyn_k ? p.K : p.M));
-        if (p.dyn_k) {
-            ext.kb_total = max(1, (n + kBk - 1) / kBk);
-            if (n == 0 && p.accumulate) ext.num_work = 0;   // nothing to add
-        } else {
-            ext.M = n;
-            ext.tiles_m = (n + BM - 1) / BM;
-            ext.num_work = ext.tiles_m * p.tiles_n * p.split_k;
+    if constexpr (KIND != 0) {
+        const InnerParams& in = p.inner;
+        if (in.dyn_rows != nullptr) {
+            const int n = max(0, min(*in.dyn_rows - in.dyn_off, in.dyn_k ? p.K : p.M));
+            if (in.dyn_k) {
+                ext.kb_total = max(1, (n + kBk - 1) / kBk);
+                if (n == 0 && accumulate) ext.num_work = 0;   // nothing to add
+            } else {
+                ext.M = n;
+                ext.tiles_m = (n + BM - 1) / BM;
+                ext.num_work = ext.tiles_m * p.tiles_n * p.split_k;
+            }
+            if (cluster_id < ext.num_work) first_wi = decode_work(p, ext, cluster_id, BM, BNT);
         }
-        if (cluster_id < ext.num_work) first_wi = decode_work(p, ext, cluster_id, BM, BNT);
     }
     const int num_work = ext.num_work;
 
@@ -640,7 +662,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                 }
                 int kb_acc = wi.kb_begin;   // first K block of the sum that the accumulator holds
                 for (int kb = wi.kb_begin; kb < wi.kb_end; ++kb) {
-                    if constexpr (HEAD != 0) {
+                    if constexpr (KIND == 1) {
                         if (kb - kb_acc == kHeadSumKb) {
                             // Hand the partial sum over and go on in the other slot (HeadParams).
                             if constexpr (CG == 1) ptx::mma_commit(tfull_bar(acc));
@@ -741,6 +763,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
         const bool out16 = !to_slab && p.out_bf16;
         const bool tma_out = p.tma_store != 0;   // implies one destination, no slabs, TMA-addressable C
         const bool staged = tma_out || (vec_ok && (p.N % (out16 ? 8 : 4) == 0));
+        const bool any_rows = !staged && !csk;
         if (tma_out && lane == 0) ptx::prefetch_tmap(&tmap_c);
         const uint32_t stage = ctrl + T::kCtrlBytes + static_cast<uint32_t>(warp - 2) * 4096u;
         for (int w = cluster_id; w < num_work; w += num_clusters) {
@@ -752,7 +775,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
             const int n_base = wi.n0 + (ND == 1 ? group * BN : 0);
             const int row = row0 + lane;
             const uint32_t t_row = tmem_base + static_cast<uint32_t>(slot * BN) + (static_cast<uint32_t>(q * 32) << 16);
-            if constexpr (HEAD != 0) {
+            if constexpr (KIND == 1) {
                 // Softmax epilogue: the warp's columns come into registers in one go (the accumulator is free again at
                 // once), so the maximum is known before the first exponential and nothing is rescaled.
                 constexpr int W = T::kPartCols;
@@ -860,131 +883,26 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                 }
                 continue;
             }
-            // The TMEM read of chunk c+1 is in flight while chunk c is transposed and stored.
-            uint32_t nxt[32];
-            ptx::tmem_ld_32x32(t_row + c_begin * 32, nxt);
-#pragma unroll 2
-            for (int c = c_begin; c < c_begin + kChunks; ++c) {
-                uint32_t raw[32];
-                ptx::tmem_ld_wait_regs(nxt);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) raw[j] = nxt[j];
-                if (c + 1 < c_begin + kChunks) ptx::tmem_ld_32x32(t_row + (c + 1) * 32, nxt);
-                if (c == c_begin + kChunks - 1) {
-                    // All of this warp's reads of the accumulator are done: hand it back to the MMA issuer.
-                    ptx::tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if constexpr (CG == 1) ptx::mbar_arrive(tempty_bar(slot));
-                        else ptx::mbar_arrive_cluster(ptx::mapa(tempty_bar(slot), 0));
-                    }
+            auto hand_back = [&] {   // all of this warp's reads of the accumulator are done: the MMA issuer may have it
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (CG == 1) ptx::mbar_arrive(tempty_bar(slot));
+                    else ptx::mbar_arrive_cluster(ptx::mapa(tempty_bar(slot), 0));
                 }
-                const int col0 = n_base + c * 32;
-                const int ncols = p.N - col0;
-                if (csk) {
-                    // The partial tile goes to shared memory (the operand ring is idle: this CTA has one work item and
-                    // its last MMA has completed), row-major [128][BN] f32 with the 16-byte pieces of every 128-byte
-                    // segment XOR-swizzled by row, for the cluster-wide sum after the barrier below.
-                    const int rl = q * 32 + lane;
-                    const uint32_t seg = smem_base + static_cast<uint32_t>(rl * BN * 4 + c * 128);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(seg + ((j ^ (rl & 7)) << 4)), "r"(raw[4 * j]),
-                                     "r"(raw[4 * j + 1]), "r"(raw[4 * j + 2]), "r"(raw[4 * j + 3])
-                                     : "memory");
-                } else if (tma_out && out16) {
-                    if (row0 < ext.M && ncols > 0) {   // warp-uniform
-                        float v[32];
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
-                        if (has_epi) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                float b = 0.0f;
-                                if (need_bias && j < ncols) b = __ldg(p.epi.bias + col0 + j);
-                                v[j] = apply_chain(v[j], p.epi, b);
-                            }
-                        }
-                        const uint32_t half_tile = stage + static_cast<uint32_t>(c & 1) * 2048u;
-                        if (lane == 0) ptx::bulk_wait_group_read<1>();   // the store that last used this half has read it
-                        __syncwarp();
-                        stage_chunk_bf16_sw64(half_tile, lane, v);
-                        ptx::fence_proxy_async_smem();
-                        __syncwarp();
-                        if (lane == 0) ptx::tma_store_2d(&tmap_c, half_tile, col0, row0);
-                    }
-                    // One group per chunk, empty where the chunk lies behind column N: the wait above counts groups, and a tile
-                    // with an odd number of chunks would otherwise leave its last store in the half that the next tile begins with.
-                    if (lane == 0) ptx::bulk_commit_group();
-                } else if (staged && out16) {
-                    const int half = c & 1;
-                    if (half == 0) __syncwarp();   // the previous pair's reads of the staging tile are done
-                    if (row0 < ext.M && ncols > 0) {   // warp-uniform
-                        float v[32];
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
-                        if (has_epi) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                float b = 0.0f;
-                                if (need_bias && j < ncols) b = __ldg(p.epi.bias + col0 + j);
-                                v[j] = apply_chain(v[j], p.epi, b);
-                            }
-                        }
-                        stage_half_bf16(stage, lane, half, v);
-                    }
-                    if (half == 1) {
-                        __syncwarp();
-                        const int cbase = col0 - 32;
-                        if (row0 < ext.M && cbase < p.N) {
-                            for (int d = 0; d < p.n_dst; ++d)
-                                flush_pair_bf16(stage, lane, static_cast<__nv_bfloat16*>(p.c_dst[d]), ld_out, row0, cbase, ext.M, p.N);
-                        }
-                    }
-                } else if (staged) {
-                    if (row0 < ext.M && ncols > 0) {   // warp-uniform
-                        float v[32];
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
-                        if (has_epi) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                float b = 0.0f;
-                                if (need_bias && j < ncols) b = __ldg(p.epi.bias + col0 + j);
-                                v[j] = apply_chain(v[j], p.epi, b);
-                            }
-                        }
-                        if (tma_out) {
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const uint32_t half_tile = stage + static_cast<uint32_t>(h) * 2048u;
-                                if (lane == 0) ptx::bulk_wait_group_read<1>();   // the store that last used this half has read it
-                                __syncwarp();
-                                stage_half_f32_sw64(half_tile, lane, v + 16 * h);
-                                ptx::fence_proxy_async_smem();
-                                __syncwarp();
-                                if (lane == 0) {
-                                    if (col0 + 16 * h < p.N) {
-                                        if (p.accumulate) ptx::tma_reduce_add_2d(&tmap_c, half_tile, col0 + 16 * h, row0);
-                                        else ptx::tma_store_2d(&tmap_c, half_tile, col0 + 16 * h, row0);
-                                    }
-                                    ptx::bulk_commit_group();   // one group per half, empty or not: the wait above counts groups
-                                }
-                            }
-                            continue;
-                        }
-                        __syncwarp();   // the previous chunk's reads of the staging tile are done
-                        stage_chunk_f32(stage, lane, v);
-                        __syncwarp();
-                        if (to_slab) {
-                            flush_chunk_f32(stage, lane, p.partial + static_cast<long long>(wi.split) * p.slab_stride, ld_out,
-                                            row0, col0, ext.M, p.N);
-                        } else {
-                            for (int d = 0; d < p.n_dst; ++d)
-                                flush_chunk_f32(stage, lane, static_cast<float*>(p.c_dst[d]), ld_out, row0, col0, ext.M, p.N, p.accumulate != 0);
-                        }
-                    }
-                } else if (row0 < ext.M && ncols > 0) {   // warp-uniform
+            };
+            if (any_rows) {
+                // Rows that start off 16-byte boundaries: through the transpose tile all the same.  A loop of its own, without the
+                // next chunk in flight: the one below needs its registers for the paths of aligned products.
+#pragma unroll 1
+                for (int c = c_begin; c < c_begin + kChunks; ++c) {
+                    uint32_t raw[32];
+                    ptx::tmem_ld_32x32(t_row + c * 32, raw);
+                    ptx::tmem_ld_wait_regs(raw);
+                    if (c == c_begin + kChunks - 1) hand_back();
+                    const int col0 = n_base + c * 32;
+                    const int ncols = p.N - col0;
+                    if (row0 >= ext.M || ncols <= 0) continue;   // warp-uniform
                     float v[32];
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
@@ -996,30 +914,146 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                             v[j] = apply_chain(v[j], p.epi, b);
                         }
                     }
-                    // Rows that start off 16-byte boundaries: through the transpose tile all the same.
-                    const int rows_here = min(32, ext.M - row0);
-                    if (out16) {
+                    const int rows_here = min(32, ext.M - row0), half = c & 1;
+                    if (!out16 || half == 0) __syncwarp();   // the previous reads of the staging tile are done
+                    if (out16) stage_half_bf16(stage, lane, half, v);
+                    else stage_chunk_f32(stage, lane, v);
+                    if (out16 && half == 0 && ncols > 32) continue;
+                    __syncwarp();
+                    for (int d = 0; d < (to_slab ? 1 : p.n_dst); ++d) {
+                        if (out16) {
+                            const int cbase = col0 - 32 * half, bytes = min(64, p.N - cbase) * 2;
+                            char* out = static_cast<char*>(p.c_dst[d]) + (row0 * ld_out + cbase) * 2;
+                            if constexpr (BN == 64) flush_rows_bf16(stage, lane, out, ld_out * 2, rows_here, bytes);
+                            else flush_rows_bf16_call(stage, lane, out, ld_out * 2, rows_here, bytes);
+                        } else {
+                            float* out = (to_slab ? p.partial + static_cast<long long>(wi.split) * p.slab_stride : static_cast<float*>(p.c_dst[d])) + row0 * ld_out + col0;
+                            if constexpr (BN == 64) flush_rows_f32(stage, lane, out, ld_out, rows_here, min(32, ncols), accumulate);
+                            else flush_rows_f32_call(stage, lane, out, ld_out, rows_here, min(32, ncols), accumulate);
+                        }
+                    }
+                }
+            } else {
+                // The TMEM read of chunk c+1 is in flight while chunk c is transposed and stored.
+                uint32_t nxt[32];
+                ptx::tmem_ld_32x32(t_row + c_begin * 32, nxt);
+#pragma unroll 2
+                for (int c = c_begin; c < c_begin + kChunks; ++c) {
+                    uint32_t raw[32];
+                    ptx::tmem_ld_wait_regs(nxt);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) raw[j] = nxt[j];
+                    if (c + 1 < c_begin + kChunks) ptx::tmem_ld_32x32(t_row + (c + 1) * 32, nxt);
+                    if (c == c_begin + kChunks - 1) hand_back();
+                    const int col0 = n_base + c * 32;
+                    const int ncols = p.N - col0;
+                    if (csk) {
+                        // The partial tile goes to shared memory (the operand ring is idle: this CTA has one work item and
+                        // its last MMA has completed), row-major [128][BN] f32 with the 16-byte pieces of every 128-byte
+                        // segment XOR-swizzled by row, for the cluster-wide sum after the barrier below.
+                        const int rl = q * 32 + lane;
+                        const uint32_t seg = smem_base + static_cast<uint32_t>(rl * BN * 4 + c * 128);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(seg + ((j ^ (rl & 7)) << 4)), "r"(raw[4 * j]),
+                                         "r"(raw[4 * j + 1]), "r"(raw[4 * j + 2]), "r"(raw[4 * j + 3])
+                                         : "memory");
+                    } else if (tma_out && out16) {
+                        if (row0 < ext.M && ncols > 0) {   // warp-uniform
+                            float v[32];
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
+                            if (has_epi) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) {
+                                    float b = 0.0f;
+                                    if (need_bias && j < ncols) b = __ldg(p.epi.bias + col0 + j);
+                                    v[j] = apply_chain(v[j], p.epi, b);
+                                }
+                            }
+                            const uint32_t half_tile = stage + static_cast<uint32_t>(c & 1) * 2048u;
+                            if (lane == 0) ptx::bulk_wait_group_read<1>();   // the store that last used this half has read it
+                            __syncwarp();
+                            stage_chunk_bf16_sw64(half_tile, lane, v);
+                            ptx::fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0) {
+                                ptx::tma_store_2d(&tmap_c, half_tile, col0, row0);
+                                ptx::bulk_commit_group();
+                            }
+                        } else if (lane == 0) {
+                            // One group per chunk, empty where the chunk lies behind column N: the wait above counts groups, and a
+                            // tile with an odd number of chunks would otherwise leave its last store in the half that the next tile
+                            // begins with.
+                            ptx::bulk_commit_group();
+                        }
+                    } else if (staged && out16) {
                         const int half = c & 1;
                         if (half == 0) __syncwarp();   // the previous pair's reads of the staging tile are done
-                        stage_half_bf16(stage, lane, half, v);
-                        if (half == 1 || ncols <= 32) {
-                            __syncwarp();
-                            const int cbase = col0 - 32 * half;
-                            for (int d = 0; d < p.n_dst; ++d)
-                                flush_rows_any<2>(stage, lane, static_cast<char*>(p.c_dst[d]) + (row0 * ld_out + cbase) * 2, ld_out * 2, rows_here,
-                                                  min(64, p.N - cbase) * 2, false);
+                        if (row0 < ext.M && ncols > 0) {   // warp-uniform
+                            float v[32];
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
+                            if (has_epi) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) {
+                                    float b = 0.0f;
+                                    if (need_bias && j < ncols) b = __ldg(p.epi.bias + col0 + j);
+                                    v[j] = apply_chain(v[j], p.epi, b);
+                                }
+                            }
+                            stage_half_bf16(stage, lane, half, v);
                         }
-                    } else {
-                        __syncwarp();   // the previous chunk's reads of the staging tile are done
-                        stage_chunk_f32(stage, lane, v);
-                        __syncwarp();
-                        if (to_slab) {
-                            flush_rows_any<4>(stage, lane, reinterpret_cast<char*>(p.partial + static_cast<long long>(wi.split) * p.slab_stride + row0 * ld_out + col0),
-                                              ld_out * 4, rows_here, min(32, ncols) * 4, false);
-                        } else {
-                            for (int d = 0; d < p.n_dst; ++d)
-                                flush_rows_any<4>(stage, lane, static_cast<char*>(p.c_dst[d]) + (row0 * ld_out + col0) * 4, ld_out * 4, rows_here,
-                                                  min(32, ncols) * 4, p.accumulate != 0);
+                        if (half == 1) {
+                            __syncwarp();
+                            const int cbase = col0 - 32;
+                            if (row0 < ext.M && cbase < p.N) {
+                                for (int d = 0; d < p.n_dst; ++d)
+                                    flush_pair_bf16(stage, lane, static_cast<__nv_bfloat16*>(p.c_dst[d]), ld_out, row0, cbase, ext.M, p.N);
+                            }
+                        }
+                    } else if (staged) {
+                        if (row0 < ext.M && ncols > 0) {   // warp-uniform
+                            float v[32];
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
+                            if (has_epi) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) {
+                                    float b = 0.0f;
+                                    if (need_bias && j < ncols) b = __ldg(p.epi.bias + col0 + j);
+                                    v[j] = apply_chain(v[j], p.epi, b);
+                                }
+                            }
+                            if (tma_out) {
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const uint32_t half_tile = stage + static_cast<uint32_t>(h) * 2048u;
+                                    if (lane == 0) ptx::bulk_wait_group_read<1>();   // the store that last used this half has read it
+                                    __syncwarp();
+                                    stage_half_f32_sw64(half_tile, lane, v + 16 * h);
+                                    ptx::fence_proxy_async_smem();
+                                    __syncwarp();
+                                    if (lane == 0) {
+                                        if (col0 + 16 * h < p.N) {
+                                            if (accumulate) ptx::tma_reduce_add_2d(&tmap_c, half_tile, col0 + 16 * h, row0);
+                                            else ptx::tma_store_2d(&tmap_c, half_tile, col0 + 16 * h, row0);
+                                        }
+                                        ptx::bulk_commit_group();   // one group per half, empty or not: the wait above counts groups
+                                    }
+                                }
+                                continue;
+                            }
+                            __syncwarp();   // the previous chunk's reads of the staging tile are done
+                            stage_chunk_f32(stage, lane, v);
+                            __syncwarp();
+                            if (to_slab) {
+                                flush_chunk_f32(stage, lane, p.partial + static_cast<long long>(wi.split) * p.slab_stride, ld_out,
+                                                row0, col0, ext.M, p.N);
+                            } else {
+                                for (int d = 0; d < p.n_dst; ++d)
+                                    flush_chunk_f32(stage, lane, static_cast<float*>(p.c_dst[d]), ld_out, row0, col0, ext.M, p.N, accumulate);
+                            }
                         }
                     }
                 }
@@ -1103,7 +1137,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
     }
 
     // ---------------------------------------------------------------------- teardown (normal and abort paths)
-    if (p.late_wait) ptx::grid_dependency_wait();   // whoever waits for this kernel waits for the one in front of it too
+    if (late_wait) ptx::grid_dependency_wait();   // whoever waits for this kernel waits for the one in front of it too
     if (csk && threadIdx.x == 64) T0B_STAMP(12);
     ptx::tc_fence_before();
     __syncthreads();

@@ -178,6 +178,21 @@ int raster_group(t0b_ctx* ctx, uint32_t bm, uint32_t bn, uint32_t cta_group, boo
     return std::max(1, std::min(grp, 16));
 }
 
+// The kernel of a plan's tile.
+template <int KIND>
+int32_t launch_plan(t0b_ctx* ctx, const t0b_gemm_plan& plan, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc,
+                    const KernelParams<KIND>& p, int num_work) {
+    if (plan.cta_group == 2) {
+        if (plan.n_tiles == 2) return launch_variant<256, 2, 2, 1, KIND>(ctx, ta, tb, tc, p, num_work);
+        if (plan.m_tiles == 2) return launch_variant<256, 2, 2, 0, KIND>(ctx, ta, tb, tc, p, num_work);
+        if (plan.bn == 256) return launch_variant<256, 2, 1, 0, KIND>(ctx, ta, tb, tc, p, num_work);
+        return launch_variant<128, 2, 1, 0, KIND>(ctx, ta, tb, tc, p, num_work);
+    }
+    if (plan.bn == 256) return launch_variant<256, 1, 1, 0, KIND>(ctx, ta, tb, tc, p, num_work, p.cluster_sk);
+    if (plan.bn == 128) return launch_variant<128, 1, 1, 0, KIND>(ctx, ta, tb, tc, p, num_work, p.cluster_sk);
+    return launch_variant<64, 1, 1, 0, KIND>(ctx, ta, tb, tc, p, num_work, p.cluster_sk);
+}
+
 int32_t run_gemm(t0b_ctx* ctx, const GemmCall& g) {
     if (g.m == 0 || g.n == 0) return T0B_OK;
     if (!g.a || !g.b || g.n_dst < 1 || g.n_dst > kMaxDst)
@@ -358,7 +373,7 @@ int32_t run_gemm(t0b_ctx* ctx, const GemmCall& g) {
         else rc = get_tmap(ctx, g.b, g.n, g.k, g.ldb, 64, 64, &tb);
         if (rc != T0B_OK) return rc;
 
-        GemmParams p{};
+        KernelParams<0> p{};
         for (int d = 0; d < g.n_dst; ++d) p.c_dst[d] = reinterpret_cast<void*>(g.c_dst[d]);
         p.n_dst = g.n_dst;
         p.ldc = static_cast<long long>(g.ldc);
@@ -376,9 +391,6 @@ int32_t run_gemm(t0b_ctx* ctx, const GemmCall& g) {
         p.a_mn_major = g.trans_a ? 1 : 0;     // A stored [K,M]: M contiguous
         p.b_mn_major = g.trans_b ? 0 : 1;     // B stored [K,N]: N contiguous
         p.out_bf16 = g.out_bf16;
-        p.accumulate = g.accumulate ? 1 : 0;
-        p.dyn_rows = g.dyn_rows; p.dyn_off = g.dyn_off; p.dyn_k = g.dyn_k;
-        p.late_wait = g.late_wait ? 1 : 0;
         p.raster_along_n = cfg.swap_grid ? 0 : 1;
         {
             p.group = raster_group(ctx, plan.bm, plan.bn, plan.cta_group, cfg.swap_grid != 0);
@@ -422,15 +434,15 @@ int32_t run_gemm(t0b_ctx* ctx, const GemmCall& g) {
             ++ctx->trace_next;
         }
 #endif
-        if (plan.cta_group == 2) {
-            if (plan.n_tiles == 2) rc = launch_variant<256, 2, 2, 1>(ctx, ta, tb, tc, p, num_work);
-            else if (plan.m_tiles == 2) rc = launch_variant<256, 2, 2>(ctx, ta, tb, tc, p, num_work);
-            else if (plan.bn == 256) rc = launch_variant<256, 2, 1>(ctx, ta, tb, tc, p, num_work);
-            else rc = launch_variant<128, 2, 1>(ctx, ta, tb, tc, p, num_work);
+        if (g.accumulate || g.dyn_rows || g.late_wait) {
+            KernelParams<2> q{};
+            static_cast<GemmParams&>(q) = p;
+            q.inner.dyn_rows = g.dyn_rows; q.inner.dyn_off = g.dyn_off; q.inner.dyn_k = g.dyn_k;
+            q.inner.accumulate = g.accumulate ? 1 : 0;
+            q.inner.late_wait = g.late_wait ? 1 : 0;
+            rc = launch_plan<2>(ctx, plan, ta, tb, tc, q, num_work);
         } else {
-            if (plan.bn == 256) rc = launch_variant<256, 1, 1>(ctx, ta, tb, tc, p, num_work, p.cluster_sk);
-            else if (plan.bn == 128) rc = launch_variant<128, 1, 1>(ctx, ta, tb, tc, p, num_work, p.cluster_sk);
-            else rc = launch_variant<64, 1, 1>(ctx, ta, tb, tc, p, num_work, p.cluster_sk);
+            rc = launch_plan<0>(ctx, plan, ta, tb, tc, p, num_work);
         }
         if (rc != T0B_OK) return rc;
         ++ctx->launches;
@@ -589,7 +601,7 @@ int32_t head_gemm(t0b_ctx* ctx, const HeadGemm& d) {
         rc = get_tmap(ctx, d.u, d.ldu, d.rows, d.ldu, 32, 32, &tc);   // 16-bit elements, moved as they are
         if (rc != T0B_OK) return rc;
     }
-    GemmParams p{};
+    KernelParams<1> p{};
     p.n_dst = 1;
     p.M = static_cast<int>(d.rows); p.N = static_cast<int>(d.vocab); p.K = static_cast<int>(d.dim);
     p.tiles_m = static_cast<int>((d.rows + plan.bm - 1) / plan.bm);
@@ -610,8 +622,8 @@ int32_t head_gemm(t0b_ctx* ctx, const HeadGemm& d) {
     p.head.c = d.c;
     p.head.ids = reinterpret_cast<const uint32_t*>(d.ids);
     p.head.row_of = reinterpret_cast<const uint32_t*>(d.row_of);
-    p.dyn_rows = reinterpret_cast<const int*>(d.dyn_rows);
-    p.dyn_off = d.dyn_off;
+    p.inner.dyn_rows = reinterpret_cast<const int*>(d.dyn_rows);
+    p.inner.dyn_off = d.dyn_off;
     p.head.n_ids = static_cast<int>(d.n_ids);
     p.head.z_sel = reinterpret_cast<float*>(d.z_sel);
     p.head.store_u = d.u ? 1 : 0;
