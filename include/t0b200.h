@@ -493,8 +493,8 @@ T0B_API int32_t t0b_topk_distill(t0b_ctx* ctx, uint64_t logits, int32_t logits_d
  * bf16 (dz is rounded to it, where dx and dw are f32 too), their sums f32.  The same call gives the same bits on every run and
  * stream.  The order of dx's sum follows the choice of tiles (t0b_tune), and a scratch that ends before the place for its
  * partial sums is taken too: dx is then summed in one piece.
- * scratch: 256-byte aligned, t0b_linear_loss_scratch_bytes() bytes; 0 = a workspace of the context that grows as needed.  A
- * call that is being captured into a graph must bring its own and keep it as long as the graph; graphs (or contexts) that
+ * scratch: 256-byte aligned, t0b_linear_loss_scratch_bytes() bytes; 0 = a workspace of the context that grows as needed and
+ * stays until the context ends.  A call that is being captured into a graph must bring its own and keep it as long as the graph; graphs (or contexts) that
  * may run at the same time need one each. */
 typedef struct t0b_linear_loss {
     uint64_t x, w;

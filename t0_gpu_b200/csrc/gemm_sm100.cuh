@@ -74,7 +74,7 @@ constexpr int kMaxDst = 8;
 // The tensor core's own sums drop what falls below the accumulator's last bit, at every 16 products; over a long contraction
 // that is a bias.  So a row's logit is summed in pieces of 512 products, in alternating accumulators, and the pieces are
 // added in the epilogue's registers, behind the next piece's products.  Losses over 50257 words at dim 2048 are then off by
-// 1.8e-7 of their norm, as with a product in f32 (pieces of 1024: 3.6e-7), for 1 % of the time or less.
+// 1.8e-7 of their norm, as with a product in f32 (pieces of 1024: 3.6e-7), for 1 to 3 % of an evaluation's time.
 constexpr int kHeadSumKb = 8;
 struct HeadParams {
     float2* part;            // [parts][part_ld]

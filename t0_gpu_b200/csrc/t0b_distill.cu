@@ -3,7 +3,8 @@
 //   p = softmax over the vocabulary of z_v / T                          (the student)
 //   loss = sum_k q_k (log q_k - log p_{id_k})                           (Kullback-Leibler divergence)
 //   d loss / d z_v = (p_v - sum_{k: id_k = v} q_k) / T
-// Loss and gradient come from one pass over HBM, which bounds the kernels: one read of z, one write of dz.  Three forms:
+// HBM bounds the kernels: one read of z, one write of dz (streamed rows and the general form read z again, from L2 where it is
+// still there: 644 MB for 2048 x 128000 bf16, of 524).  Three forms:
 //   rows in registers  a cluster of 1 to 8 CTAs per row; every thread keeps up to sixteen 16-byte groups, all loaded before
 //                      the first is used: maximum; exponentials, which replace the logits, and their sum; -- the CTAs
 //                      exchange (maximum, sum) over distributed shared memory -- gradient = exponential times one factor
